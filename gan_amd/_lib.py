@@ -102,6 +102,21 @@ SIGNATURES = {
     "gan_l1_mean": (I, [P, P, L, F, I, P, P, P]),
     "gan_l1_mean_workspace_bytes": (Z, [L]),
     "gan_l1_mean_ws": (I, [P, P, L, F, I, P, P, P, Z, P]),
+    "gan_rms_norm_fwd": (I, [I, L, I, P, L, P, L, P, F, P, P, P, P, P, P]),
+    "gan_rms_norm_workspace_bytes": (Z, [L, I]),
+    "gan_rms_norm_bwd": (I, [I, L, I, P, L, P, P, P, P, P, P, I, P, Z, P]),
+    "gan_mx_quantize": (I, [I, I, L, I, P, L, P, P, P]),
+    "gan_mx_dequantize": (I, [I, I, L, I, P, P, P, P]),
+    "gan_mx_pack": (I, [I, I, I, P, L, P, P, P]),
+    "gan_mx_unpack": (I, [I, I, I, P, P, P, P]),
+    "gan_mx_matmul_workspace_bytes": (Z, [I, I, I, I, I]),
+    "gan_mx_matmul": (I, [I, I, I, I, I, P, P, P, P, P, P, P, Z, P]),
+    "gan_mx_matmul_dgrad_workspace_bytes": (Z, [I, I, I, I]),
+    "gan_mx_matmul_dgrad": (I, [I, I, I, I, P, P, P, P, P, Z, P]),
+    "gan_mx_matmul_wgrad_workspace_bytes": (Z, [I, I, I, I]),
+    "gan_mx_matmul_wgrad": (I, [I, I, I, I, I, P, P, P, P, P, I, P, Z, P]),
+    "gan_distill_topk_workspace_bytes": (Z, [L]),
+    "gan_distill_topk_mean": (I, [I, L, I, P, L, I, P, P, I, I, P, P, F, F, I, P, P, P, Z, P]),
     "gan_adam_tf_step": (I, [P, P, P, P, L, F, F, F, F, F, P, P, P]),
     "gan_fill": (I, [P, L, F, P]),
     "gan_conv_plan_set": (I, [I, GeomP, I, I]),
@@ -150,6 +165,37 @@ def ptr(t):
     if not t.is_contiguous():
         raise ValueError("libgan_hip takes dense (contiguous) tensors")
     return t.data_ptr()
+
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # GAN_F32 / GAN_BF16 / GAN_F16
+MX_FORMATS = {'e4m3': 0, 'e2m1': 1}                                   # GAN_MX_E4M3 / GAN_MX_E2M1
+MX_MAX_IN = 1 << 22
+
+
+def dtype_code(dtype):
+    """GAN_F32 / GAN_BF16 / GAN_F16 of a torch type."""
+    code = DTYPES.get(dtype)
+    if code is None:
+        raise TypeError("expected a float32, bfloat16 or float16 tensor, got %s" % dtype)
+    return code
+
+
+def here(*tensors):
+    """The device the library is about to launch on; every tensor (None is skipped) has to live there."""
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise GanHipError("libgan_hip launches on the current device cuda:%d, got a tensor on %s" % (dev, t.device))
+    return dev
+
+
+def scratch(nbytes, device):
+    """Scratch of one call: (pointer, size, the tensor to keep until the call is queued).  It comes from the caching allocator,
+    so calls on two streams, or in two captured graphs, never share it."""
+    if not nbytes:
+        return None, 0, None
+    t = torch.empty(int(nbytes), dtype=torch.uint8, device=device)
+    return t.data_ptr(), int(nbytes), t
 
 
 def stream():

@@ -1,0 +1,412 @@
+// Distillation from a teacher's top logits: mean over rows of a Kullback-Leibler divergence, fused with its gradient.
+//
+//   z = s / tau, t' = t / tau; list entries whose class is outside [0, classes) or whose logit is -inf are left out
+//   p_i = softmax of t' over the list, or exp(t'_i - lse) where the teacher's log-sum-exp is given
+//   l = sum_i p_i (log p_i - log q_i)  [+ p_r (log p_r - log q_r)],   q = softmax z
+//   p_r = max(0, 1 - sum p), q_r = sum of q over the classes not listed (with lse only)
+//   dl/dz_j = P q_j - p_j (listed), P q_j - p_r q_j / q_r (others), P = sum p + p_r
+//
+// Memory-bound: the logits are read once, held in registers, and their gradient is written once.  One workgroup a row, its
+// threads hold the row in 16-byte chunks of the tensor's type; the maximum and the sum of exponentials come from one pass over
+// the registers (a thread rescales nothing: it takes its own maximum first), joined over the workgroup in one exchange.
+// q_r is never 1 - sum q_i, which cancels: a bit per class marks the list, and sums over the marked and the unmarked classes
+// are taken apart.  The same bits tell whether a class is listed twice, in which case its probabilities add up.
+// Statistics are fp32 with natural order fixed by the thread number, so results are deterministic.
+#include "mx.h"
+
+namespace gan {
+
+struct Distill {
+    const void* logits;
+    void* grad;             // dense [rows][classes], or null
+    const void* teacher;
+    const void* index;
+    const float* lse;
+    const float* weight;
+    const float* total;     // sum of the weights; null: the kernel adds them up itself
+    float* row_loss;
+    long ld, rows;
+    int classes, top, teacher_dtype, index64;
+    float inv_tau, grad_scale;
+};
+
+__device__ __forceinline__ float teacher_at(const Distill& p, long i) {
+    if (p.teacher_dtype == GAN_F32) return static_cast<const float*>(p.teacher)[i];
+    if (p.teacher_dtype == GAN_BF16) return (float)static_cast<const bf16_t*>(p.teacher)[i];
+    return (float)static_cast<const f16_t*>(p.teacher)[i];
+}
+
+__device__ __forceinline__ float wave_all_sum(float v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    return v;
+}
+__device__ __forceinline__ float wave_all_max(float v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+    return v;
+}
+
+// exp(x - m) with -inf as the maximum of nothing: exp(-inf - -inf) is 0 here
+__device__ __forceinline__ float exp_from(float x, float m) { return __expf(x - (m == -INFINITY ? 0.f : m)); }
+
+// Maximum and sum of exponentials, joined: (m, s) <- (max(m, m2), s e^(m - max) + s2 e^(m2 - max)).
+__device__ __forceinline__ void join_stats(float& m, float& s, float m2, float s2) {
+    const float mm = fmaxf(m, m2);
+    s = s * exp_from(m, mm) + s2 * exp_from(m2, mm);
+    m = mm;
+}
+
+template <int NT>
+__device__ __forceinline__ float block_sum(float v, float* red) {
+    v = wave_all_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.f;
+    for (int i = 0; i < NT / 64; ++i) v += red[i];
+    return v;
+}
+
+// NV chunks of eight values a thread in registers; NV = 0: the row does not fit and is read twice.
+template <typename T, int NT, int NV, bool REST>
+__global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
+    extern __shared__ __align__(16) unsigned char lds[];
+    __shared__ float red[2 * NT / 64];
+    __shared__ float told[6];       // statistics of the list: any, P, p_r, maximum, sum of exponentials; repeated classes
+    const int tid = threadIdx.x, lane = tid & 63, classes = p.classes;
+    const long row = blockIdx.x;
+    const T* x = static_cast<const T*>(p.logits) + row * p.ld;
+    T* gr = static_cast<T*>(p.grad) + (p.grad ? row * classes : 0);
+    // chunks start at 16-byte borders: chunk c holds the classes 8 c - a .. 8 c - a + 7
+    const int a = (int)((reinterpret_cast<size_t>(x) & 15) / sizeof(T));
+    const bool gvec = (reinterpret_cast<size_t>(gr) & 15) == (reinterpret_cast<size_t>(x) & 15);
+    const int chunks = (classes + a + 7) / 8;
+    unsigned* bits = reinterpret_cast<unsigned*>(lds);      // bit 8 c + j: class j of chunk c is listed
+    const int words = (chunks + 3) / 4;
+    int* l_id = reinterpret_cast<int*>(lds + ((words + 3) / 4) * 16);
+    float* l_p = reinterpret_cast<float*>(l_id + p.top);
+    float* l_lp = l_p + p.top;
+    float* l_z = l_lp + p.top;
+
+    typedef typename Vec8<T>::type Raw;
+    auto load = [&](int chunk) -> Raw {
+        const int e0 = chunk * 8 - a;
+        if (e0 >= 0 && e0 + 8 <= classes) return *reinterpret_cast<const Raw*>(x + e0);
+        Raw r;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] = e0 + j >= 0 && e0 + j < classes ? x[e0 + j] : (T)-INFINITY;
+        return r;
+    };
+    auto store = [&](int chunk, const float (&g)[8]) {
+        const int e0 = chunk * 8 - a;
+        if (gvec && e0 >= 0 && e0 + 8 <= classes) {
+            Raw r;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r[j] = (T)g[j];
+            *reinterpret_cast<Raw*>(gr + e0) = r;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (e0 + j >= 0 && e0 + j < classes) gr[e0 + j] = (T)g[j];
+        }
+    };
+
+    const float w = p.weight ? p.weight[row] : 1.f;
+    Raw raw[NV > 0 ? NV : 1];
+    if (w != 0.f) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int chunk = i * NT + tid;
+            if (chunk < chunks) raw[i] = load(chunk);
+            else
+#pragma unroll
+                for (int j = 0; j < 8; ++j) raw[i][j] = (T)-INFINITY;
+        }
+    }
+    for (int i = tid; i < words; i += NT) bits[i] = 0;
+    float total = (float)p.rows;
+    if (p.weight) {
+        if (p.total) {
+            total = p.total[0];
+        } else {
+            float s = 0.f;
+            for (long i = tid; i < p.rows; i += NT) s += p.weight[i];
+            total = block_sum<NT>(s, red);
+        }
+    }
+    __syncthreads();
+
+    if (w != 0.f && tid < 64) {     // the list, by the first wave
+        int any = 0, twice = 0;
+        float m = -INFINITY;
+        for (int i = lane; i < p.top; i += 64) {
+            const long at = row * p.top + i;
+            const long id64 = p.index64 ? static_cast<const long*>(p.index)[at] : static_cast<const int*>(p.index)[at];
+            const float t = teacher_at(p, at) * p.inv_tau;
+            const bool in = id64 >= 0 && id64 < classes && t != -INFINITY;
+            const int id = in ? (int)id64 : -1;
+            l_id[i] = id;
+            l_lp[i] = t;
+            l_z[i] = in ? (float)x[id] * p.inv_tau : 0.f;
+            if (in) {
+                any = 1;
+                m = fmaxf(m, t);
+                const unsigned bit = 1u << ((id + a) & 31);
+                twice |= (atomicOr(&bits[(id + a) >> 5], bit) & bit) != 0;
+            }
+        }
+        any = __any(any);
+        twice = __any(twice);
+        m = wave_all_max(m);
+        float norm = 0.f;
+        if (REST) {
+            norm = p.lse[row];
+        } else {
+            float s = 0.f;
+            for (int i = lane; i < p.top; i += 64)
+                if (l_id[i] >= 0) s += expf(l_lp[i] - m);
+            norm = m + logf(wave_all_sum(s));
+        }
+        float mass = 0.f;
+        for (int i = lane; i < p.top; i += 64) {
+            const float lp = l_lp[i] - norm, pr = l_id[i] >= 0 ? expf(lp) : 0.f;
+            l_lp[i] = lp;
+            l_p[i] = pr;
+            mass += pr;
+        }
+        mass = wave_all_sum(mass);
+        float ml = -INFINITY, sl = 0.f;
+        if (REST) {     // statistics of the listed classes, each once
+            for (int i = lane; i < p.top; i += 64)
+                if (l_id[i] >= 0) ml = fmaxf(ml, l_z[i]);
+            ml = wave_all_max(ml);
+            for (int i = lane; i < p.top; i += 64) {
+                bool first = l_id[i] >= 0;
+                if (twice)
+                    for (int j = 0; j < i && first; ++j) first = l_id[j] != l_id[i];
+                if (first) sl += exp_from(l_z[i], ml);
+            }
+            sl = wave_all_sum(sl);
+        }
+        if (lane == 0) {
+            const float rest = REST ? fmaxf(0.f, 1.f - mass) : 0.f;
+            told[0] = any ? 1.f : 0.f;
+            told[1] = REST ? mass + rest : 1.f;
+            told[2] = rest;
+            told[3] = ml;
+            told[4] = sl;
+            told[5] = twice ? 1.f : 0.f;
+        }
+    }
+    __syncthreads();
+    if (w == 0.f || told[0] == 0.f) {       // nothing to learn in this row
+        if (p.grad) {
+            const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            for (int c = tid; c < chunks; c += NT) store(c, zero);
+        }
+        if (tid == 0) p.row_loss[row] = 0.f;
+        return;
+    }
+
+    // maximum and sum of exponentials of the unlisted classes (REST) or of all
+    auto values = [&](const Raw& r, int chunk, float (&v)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (float)r[j] * p.inv_tau;
+        if (REST) {
+            const unsigned marked = chunk < chunks ? reinterpret_cast<const unsigned char*>(bits)[chunk] : 0;
+            if (marked) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (marked >> j & 1) v[j] = -INFINITY;
+            }
+        }
+    };
+    float m = -INFINITY, s = 0.f;
+    if (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float v[8];
+            values(raw[i], i * NT + tid, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = fmaxf(m, v[j]);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float v[8];
+            values(raw[i], i * NT + tid, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s += exp_from(v[j], m);
+        }
+    } else {
+        for (int c = tid; c < chunks; c += NT) {
+            float v[8], mc = -INFINITY, sc = 0.f;
+            values(load(c), c, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) mc = fmaxf(mc, v[j]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sc += exp_from(v[j], mc);
+            join_stats(m, s, mc, sc);
+        }
+    }
+    {
+        const float mw = wave_all_max(m);
+        s = wave_all_sum(s * exp_from(m, mw));
+        m = mw;
+        if (lane == 0) {
+            red[2 * (tid >> 6)] = m;
+            red[2 * (tid >> 6) + 1] = s;
+        }
+        __syncthreads();
+        m = red[0];
+        s = red[1];
+        for (int i = 1; i < NT / 64; ++i) join_stats(m, s, red[2 * i], red[2 * i + 1]);
+    }
+    const float P = told[1], rest = told[2];
+    float mall = m, sall = s;
+    if (REST) join_stats(mall, sall, told[3], told[4]);
+    const float lse = mall + logf(sall);
+    const bool there = REST && rest > 0.f && m > -INFINITY;
+    const float gs = total != 0.f ? p.grad_scale * (w / total) : 0.f;
+    if (p.grad) {
+        // e^(z - m) times one factor for every class that is not listed
+        const float f = gs * (REST ? P * __expf(m - lse) - (there ? rest / s : 0.f) : P / s);
+        if (NV > 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int chunk = i * NT + tid;
+                if (chunk < chunks) {
+                    float v[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = exp_from((float)raw[i][j] * p.inv_tau, m) * f;
+                    store(chunk, v);
+                }
+            }
+        } else {
+            for (int c = tid; c < chunks; c += NT) {
+                const Raw r = load(c);
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = exp_from((float)r[j] * p.inv_tau, m) * f;
+                store(c, v);
+            }
+        }
+        __syncthreads();        // (waits for the stores: the listed classes are written again)
+        const bool twice = told[5] != 0.f;
+        for (int i = tid; i < p.top; i += NT) {
+            const int id = l_id[i];
+            if (id < 0) continue;
+            float pi = l_p[i];
+            bool first = true;
+            if (twice) {
+                pi = 0.f;
+                for (int j = 0; j < p.top; ++j)
+                    if (l_id[j] == id) {
+                        if (j < i) first = false;
+                        pi += l_p[j];
+                    }
+            }
+            if (first) gr[id] = (T)(gs * (P * __expf(l_z[i] - lse) - pi));
+        }
+    }
+    if (tid < 64) {
+        float l = 0.f;
+        for (int i = lane; i < p.top; i += 64)
+            if (l_p[i] > 0.f || l_p[i] != l_p[i]) l += l_p[i] * (l_lp[i] - (l_z[i] - lse));
+        l = wave_all_sum(l);
+        if (there) l += rest * (logf(rest) - (m + logf(s) - lse));
+        if (lane == 0) p.row_loss[row] = w * l;
+    }
+}
+
+// out[0] = sum of x: one workgroup, fixed order.
+__device__ float sum_by_block(const float* __restrict__ x, long n, float* red) {
+    float s = 0.f;
+    for (long i = threadIdx.x; i < n; i += 1024) s += x[i];
+    return block_sum<1024>(s, red);
+}
+__global__ __launch_bounds__(1024) void distill_weights_kernel(const float* __restrict__ weight, long rows, float* out) {
+    __shared__ float red[16];
+    const float s = sum_by_block(weight, rows, red);
+    if (threadIdx.x == 0) out[0] = s;
+}
+__global__ __launch_bounds__(1024) void distill_mean_kernel(const float* __restrict__ row_loss, const float* __restrict__ weight,
+                                                            long rows, float scale, int accumulate, float* __restrict__ out) {
+    __shared__ float red[16];
+    const float s = sum_by_block(row_loss, rows, red);
+    const float total = weight ? sum_by_block(weight, rows, red) : (float)rows;
+    if (threadIdx.x == 0) out[0] = (accumulate ? out[0] : 0.f) + (total != 0.f ? scale * (s / total) : 0.f);
+}
+
+constexpr int kMaxClasses = 1 << 20, kMaxTop = 1024;
+
+template <typename T, int NT, int NV>
+static int launch_distill(const Distill& p, hipStream_t st) {
+    // (7 classes more than there are: a row may start inside a chunk)
+    const size_t lds = ((size_t)(p.classes + 7 + 7) / 8 + 16 + 15) / 16 * 16 + (size_t)p.top * 16;
+    auto go = [&](auto kernel) {
+        // the list's bits of the largest vocabulary and the longest list
+        constexpr int most = kMaxClasses / 8 + 64 + kMaxTop * 16;
+        const hipError_t set = lds > 65536 ? hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                                 hipFuncAttributeMaxDynamicSharedMemorySize, most) : hipSuccess;
+        if (set != hipSuccess) return fail("gan_distill_topk_mean: %zu bytes of LDS refused: %s", lds, hipGetErrorString(set));
+        hipLaunchKernelGGL(kernel, dim3((unsigned)p.rows), dim3(NT), lds, st, p);
+        return 0;
+    };
+    return p.lse ? go(distill_kernel<T, NT, NV, true>) : go(distill_kernel<T, NT, NV, false>);
+}
+
+}  // namespace gan
+
+using namespace gan;
+
+extern "C" {
+
+size_t gan_distill_topk_workspace_bytes(long rows) { return rows > 0 ? ((size_t)rows + 4) * sizeof(float) : 0; }
+
+int gan_distill_topk_mean(int dtype, long rows, int classes, const void* logits, long ld, int teacher_dtype, const void* teacher,
+                          const void* index, int index_bytes, int top, const float* teacher_lse, const float* row_weight,
+                          float temperature, float weight, int accumulate, float* loss_out, void* dlogits, void* ws,
+                          size_t ws_bytes, gan_stream_t stream) {
+    GAN_CHECK_ARG(dtype_ok(dtype) && dtype_ok(teacher_dtype), "gan_distill_topk_mean: unknown element type %d or %d", dtype, teacher_dtype);
+    GAN_CHECK_ARG(rows >= 1 && rows < (1L << 31), "gan_distill_topk_mean: %ld rows", rows);
+    GAN_CHECK_ARG(classes >= 1 && classes <= kMaxClasses, "gan_distill_topk_mean: %d classes (1..%d are served)", classes, kMaxClasses);
+    GAN_CHECK_ARG(top >= 1 && top <= kMaxTop, "gan_distill_topk_mean: lists of %d (1..%d are served)", top, kMaxTop);
+    GAN_CHECK_ARG(index_bytes == 4 || index_bytes == 8, "gan_distill_topk_mean: indices of %d bytes", index_bytes);
+    GAN_CHECK_ARG(temperature > 0.f && temperature < INFINITY, "gan_distill_topk_mean: temperature %g", (double)temperature);
+    GAN_CHECK_ARG(logits && teacher && index && loss_out, "gan_distill_topk_mean: null pointer");
+    GAN_CHECK_ARG(ld >= classes, "gan_distill_topk_mean: row stride %ld smaller than the row", ld);
+    GAN_CHECK_ARG(ws && ws_bytes >= gan_distill_topk_workspace_bytes(rows), "gan_distill_topk_mean: workspace of %zu bytes needed, %zu given",
+                  gan_distill_topk_workspace_bytes(rows), ws_bytes);
+    const hipStream_t st = as_stream(stream);
+    float* row_loss = static_cast<float*>(ws);
+    float* total = nullptr;
+    if (row_weight && rows > 4096) {    // (up to there every workgroup adds the weights up itself: 16 KB from the L2)
+        total = row_loss + rows;
+        hipLaunchKernelGGL(distill_weights_kernel, dim3(1), dim3(1024), 0, st, row_weight, rows, total);
+    }
+    const Distill p{logits, dlogits, teacher, index, teacher_lse, row_weight, total, row_loss, ld, rows, classes, top,
+                    teacher_dtype, index_bytes == 8, 1.f / temperature, weight * temperature};
+    const int rc = with_dtype(dtype, [&](auto* tag) {
+        typedef typename std::remove_pointer<decltype(tag)>::type T;
+        const int chunks = (classes + 7 + 7) / 8;     // (a row may start anywhere in its first chunk)
+        if (chunks <= 256) return launch_distill<T, 256, 1>(p, st);
+        if (chunks <= 512) return launch_distill<T, 256, 2>(p, st);
+        if (chunks <= 1024) return launch_distill<T, 256, 4>(p, st);
+        if (chunks <= 2048) return launch_distill<T, 512, 4>(p, st);
+        if (chunks <= 4096) return launch_distill<T, 1024, 4>(p, st);
+        if (chunks <= 8192) return launch_distill<T, 1024, 8>(p, st);
+        if constexpr (sizeof(T) == 2) {
+            // 64 of the 128 registers a thread has; aligned rows fill their chunks, so the border is exact for them
+            const bool whole = aligned16(logits) && ld % 8 == 0;
+            if ((whole ? (classes + 7) / 8 : chunks) <= 16384) return launch_distill<T, 1024, 16>(p, st);
+        }
+        return launch_distill<T, 1024, 0>(p, st);
+    });
+    if (rc) return rc;
+    hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(1024), 0, st, row_loss, row_weight, rows, weight * temperature * temperature,
+                       accumulate, loss_out);
+    return check_launch("gan_distill_topk_mean");
+}
+
+}  // extern "C"

@@ -1,0 +1,448 @@
+// The bf16-pipe product and the gradients of the microscaled product.
+//
+//   dA[r][k] = sum_n dY[r][n] W[k][n]      dW[k][n] = sum_r A[r][k] dY[r][n]      dbias[n] = sum_r dY[r][n]
+//
+// with A and W the quantised values (the gradient of the quantisers is passed straight through).  Quantised values are exact in
+// bf16; dY is split exactly into one (bf16), two (fp16: 11 = 8 + 3 bits) or three (fp32: 24 = 8 + 8 + 8) bf16 parts, whose
+// products are summed in fp32.  So a gradient carries the error of an fp32 sum of exact products whatever the type.
+//
+// All three products contract over rows that are contiguous in memory: memory-bound passes turn the operands into bf16 images
+// with the contraction axis innermost and filled up with zeros to a multiple of 64, then one compute-bound kernel runs.
+#include "mx_gemm.h"
+
+namespace gan {
+
+// C[i][j] over a tile of BI x BJ, WI x WJ waves, 32x32x16 instructions with Q as their first operand (a lane ends with four
+// consecutive j of one i).  A step is 64 deep: rows of 128 bytes, their 16-byte chunks swapped by row so that a fragment read
+// hits all banks; two stages, filled by direct copies one step ahead.
+template <typename T, int BI, int BJ, int WI, int WJ>
+__global__ __launch_bounds__(64 * WI * WJ) void bf16_product_kernel(Bf16Product p, T* out, float* slabs, int splits, bool vec) {
+    constexpr int THREADS = 64 * WI * WJ, FI = BI / WI / 32, FJ = BJ / WJ / 32, STAGE = (BI + BJ) * 128;
+    extern __shared__ __align__(16) unsigned char lds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wj = wave % WJ, wi = wave / WJ;
+    const int l32 = lane & 31, half = lane >> 5;
+    int ti, tj;
+    tile_of(blockIdx.x, (p.rows + BI - 1) / BI, (p.cols + BJ - 1) / BJ, ti, tj);
+    const int i0 = ti * BI, j0 = tj * BJ;
+    const int per = p.depth / 64;
+    const long steps = (long)per * p.parts;
+    const int s0 = (int)(steps * blockIdx.y / splits), s1 = (int)(steps * (blockIdx.y + 1) / splits);
+
+    auto fill = [&](int s, int buf) {
+        unsigned char* base = lds + buf * STAGE;
+        const int part = s / per, c = (s - part * per) * 64;
+        const bf16_t* ps = p.p + part * p.pstep + c;
+        const bf16_t* qs = p.q + part * p.qstep + c;
+#pragma unroll
+        for (int i = 0; i < BI * 8 / THREADS; ++i) {
+            const int at = (i * WI * WJ + wave) * 64, row = (at + lane) >> 3, chunk = (lane & 7) ^ (row & 7);
+            copy_to_lds16(ps + (long)min(i0 + row, p.rows - 1) * p.ldp + chunk * 8, base + at * 16);
+        }
+#pragma unroll
+        for (int i = 0; i < BJ * 8 / THREADS; ++i) {
+            const int at = (i * WI * WJ + wave) * 64, row = (at + lane) >> 3, chunk = (lane & 7) ^ (row & 7);
+            copy_to_lds16(qs + (long)min(j0 + row, p.cols - 1) * p.ldq + chunk * 8, base + BI * 128 + at * 16);
+        }
+    };
+
+    f32x16 acc[FJ][FI];
+#pragma unroll
+    for (int j = 0; j < FJ; ++j)
+#pragma unroll
+        for (int i = 0; i < FI; ++i)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) acc[j][i][k] = 0.f;
+    if (s0 < s1) fill(s0, 0);
+    for (int s = s0; s < s1; ++s) {
+        const int buf = (s - s0) & 1;
+        copies_done_barrier();
+        if (s + 1 < s1) fill(s + 1, buf ^ 1);
+        const unsigned char* lp = lds + buf * STAGE;
+        const unsigned char* lq = lp + BI * 128;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            bf16x8 fp[FI], fq[FJ];
+#pragma unroll
+            for (int j = 0; j < FJ; ++j) {
+                const int row = (wj * FJ + j) * 32 + l32;
+                fq[j] = *reinterpret_cast<const bf16x8*>(lq + row * 128 + (((2 * k + half) ^ (row & 7)) * 16));
+            }
+#pragma unroll
+            for (int i = 0; i < FI; ++i) {
+                const int row = (wi * FI + i) * 32 + l32;
+                fp[i] = *reinterpret_cast<const bf16x8*>(lp + row * 128 + (((2 * k + half) ^ (row & 7)) * 16));
+            }
+#pragma unroll
+            for (int j = 0; j < FJ; ++j)
+#pragma unroll
+                for (int i = 0; i < FI; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fq[j], fp[i], acc[j][i], 0, 0, 0);
+        }
+    }
+    const int n4 = (p.cols + 3) / 4 * 4;
+#pragma unroll
+    for (int i = 0; i < FI; ++i) {
+        const int row = i0 + (wi * FI + i) * 32 + l32;
+        if (row >= p.rows) continue;
+#pragma unroll
+        for (int j = 0; j < FJ; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int col = j0 + (wj * FJ + j) * 32 + 8 * q + 4 * half;
+                const f32x4 v = {acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
+                if (slabs) {
+                    if (col < p.cols) *reinterpret_cast<f32x4*>(slabs + ((long)blockIdx.y * p.rows + row) * n4 + col) = v;
+                } else {
+                    store4(out + (long)row * p.cols, col, p.cols, vec, v, p.bias, p.accumulate);
+                }
+            }
+    }
+}
+
+struct Bf16Plan {
+    bool large;
+    int splits;
+};
+static Bf16Plan bf16_plan(int rows, int cols, int parts, int depth) {
+    const long large = (long)((rows + 255) / 256) * ((cols + 255) / 256);
+    if (large >= 192) return {true, 1};
+    const long steps = (long)parts * (depth / 64);
+    return {false, contraction_splits((long)((rows + 127) / 128) * ((cols + 127) / 128), (int)(steps < (1 << 30) ? steps : 1 << 30), 8)};
+}
+
+size_t bf16_product_workspace(int rows, int cols, int parts, int depth) {
+    return slab_bytes(bf16_plan(rows, cols, parts, depth).splits, rows, cols);
+}
+
+template <typename T, int BI, int BJ, int WI, int WJ>
+static int launch_bf16(const Bf16Product& p, T* out, float* slabs, int splits, bool vec, hipStream_t st, const char* what) {
+    constexpr int LDS = 2 * (BI + BJ) * 128;
+    auto kernel = bf16_product_kernel<T, BI, BJ, WI, WJ>;
+    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                      hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (set != hipSuccess) return fail("%s: %d bytes of LDS refused: %s", what, LDS, hipGetErrorString(set));
+    const long tiles = (long)((p.rows + BI - 1) / BI) * ((p.cols + BJ - 1) / BJ);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, splits), dim3(64 * WI * WJ), LDS, st, p, out, slabs, splits, vec);
+    return 0;
+}
+
+template <typename T>
+int bf16_product(const Bf16Product& p, T* out, void* ws, hipStream_t st, const char* what) {
+    const Bf16Plan plan = bf16_plan(p.rows, p.cols, p.parts, p.depth);
+    const bool vec = p.cols % 4 == 0 && (reinterpret_cast<size_t>(out) & (4 * sizeof(T) - 1)) == 0 && aligned16(p.bias);
+    float* slabs = plan.splits > 1 ? static_cast<float*>(ws) : nullptr;
+    const int rc = plan.large ? launch_bf16<T, 256, 256, 4, 2>(p, out, slabs, plan.splits, vec, st, what)
+                              : launch_bf16<T, 128, 128, 2, 2>(p, out, slabs, plan.splits, vec, st, what);
+    if (rc) return rc;
+    if (slabs) join_slabs(slabs, plan.splits, out, (long)p.rows, p.cols, p.bias, p.accumulate, vec, st);
+    return check_launch(what);
+}
+template int bf16_product<float>(const Bf16Product&, float*, void*, hipStream_t, const char*);
+
+// ------------------------------------------------------------------------------------------------ operand images
+// Part `part` of the exact split of v into bf16 values, largest first.  By truncation: it cannot overflow, and what is left is
+// exact.  An infinity or a NaN is in part 0 alone.
+__device__ __forceinline__ bf16_t split_part(float v, int part) {
+    for (int i = 0; i < part; ++i) {
+        const unsigned u = __float_as_uint(v);
+        v = (u & 0x7f800000u) == 0x7f800000u ? 0.f : v - __uint_as_float(u & 0xffff0000u);
+    }
+    const unsigned u = __float_as_uint(v);
+    const unsigned nan = (u & 0x7fffffffu) > 0x7f800000u ? 0x400000u : 0u;
+    return __builtin_bit_cast(bf16_t, (unsigned short)((u | nan) >> 16));
+}
+
+template <typename T> struct Parts;
+template <> struct Parts<bf16_t> { static constexpr int n = 1; };
+template <> struct Parts<f16_t> { static constexpr int n = 2; };
+template <> struct Parts<float> { static constexpr int n = 3; };
+
+__host__ __device__ __forceinline__ long to64(long n) { return (n + 63) / 64 * 64; }
+
+// dY [rows][n] -> parts [rows][n filled up to 64] bf16.
+template <typename T>
+__global__ __launch_bounds__(256) void split_rows_kernel(const T* __restrict__ y, bf16_t* __restrict__ out, long rows, int n,
+                                                         bool vec) {
+    const long np = to64(n), chunks = np / 8, total = rows * chunks;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+        const long row = i / chunks;
+        const int i0 = (int)(i - row * chunks) * 8;
+        float v[8];
+        load8(y + row * n, i0, i0 < n ? n : 0, vec, v);
+#pragma unroll
+        for (int part = 0; part < Parts<T>::n; ++part) {
+            bf16x8 b;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) b[j] = split_part(v[j], part);
+            *reinterpret_cast<bf16x8*>(out + (part * rows + row) * np + i0) = b;
+        }
+    }
+}
+
+// dY [rows][n] -> parts [n][rows filled up to 64] bf16, and the sums of 64 rows of each column (dbias).  64 x 64 tiles through
+// LDS.
+template <typename T>
+__global__ __launch_bounds__(256) void split_transpose_kernel(const T* __restrict__ y, bf16_t* __restrict__ out,
+                                                              float* __restrict__ colsum, int rows, int n, bool vec) {
+    __shared__ float tile[64][65];
+    const long rp = to64(rows);
+    const int n0 = blockIdx.x * 64, r0 = blockIdx.y * 64, t = threadIdx.x;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int row = h * 32 + t / 8, i0 = n0 + (t % 8) * 8;
+        float v[8];
+        load8(y + (long)min(r0 + row, rows - 1) * n, i0, r0 + row < rows && i0 < n ? n : 0, vec, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) tile[row][(t % 8) * 8 + j] = v[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int col = h * 32 + t / 8, r8 = (t % 8) * 8;
+        float v[8], s = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j] = tile[r8 + j][col];
+            s += v[j];
+        }
+        if (n0 + col < n) {
+#pragma unroll
+            for (int part = 0; part < Parts<T>::n; ++part) {
+                bf16x8 b;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) b[j] = split_part(v[j], part);
+                *reinterpret_cast<bf16x8*>(out + ((long)part * n + n0 + col) * rp + r0 + r8) = b;
+            }
+        }
+        s += __shfl_xor(s, 1, 64);
+        s += __shfl_xor(s, 2, 64);
+        s += __shfl_xor(s, 4, 64);
+        if (colsum && (t & 7) == 0 && n0 + col < n) colsum[(long)blockIdx.y * n + n0 + col] = s;
+    }
+}
+
+// A [rows][in] microscaled -> [in][rows filled up to 64] bf16, 64 rows x 64 values a workgroup.
+template <int FMT>
+__global__ __launch_bounds__(256) void mx_rows_transpose_kernel(const unsigned char* __restrict__ codes,
+                                                                const unsigned char* __restrict__ scales, bf16_t* __restrict__ out,
+                                                                int rows, int in_dim) {
+    __shared__ bf16_t tile[64][66];
+    const long rp = to64(rows), pitch = mx_groups(in_dim) * 16L;
+    const int k0 = blockIdx.x * 64, r0 = blockIdx.y * 64, t = threadIdx.x;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int row = h * 32 + t / 8;
+        bf16x8 b;
+        if (r0 + row < rows) {
+            const long at = (long)(r0 + row) * pitch + k0 / 8 + t % 8;
+            const float s = mx_scale(scales[at / 4]);
+            if constexpr (FMT == GAN_MX_E4M3) {
+                const uint2 u = *reinterpret_cast<const uint2*>(codes + at * 8);
+                b = e4m3_to_bf16(u.x, u.y, s);
+            } else {
+                b = e2m1_to_bf16(*reinterpret_cast<const unsigned*>(codes + at * 4), s);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) b[j] = (bf16_t)0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) tile[row][(t % 8) * 8 + j] = b[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int col = h * 32 + t / 8, r8 = (t % 8) * 8;
+        if (k0 + col >= in_dim) continue;
+        bf16x8 b;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) b[j] = tile[r8 + j][col];
+        *reinterpret_cast<bf16x8*>(out + (long)(k0 + col) * rp + r0 + r8) = b;
+    }
+}
+
+template <int FMT>
+__global__ __launch_bounds__(256) void mx_rows_bf16_kernel(const unsigned char* __restrict__ codes,
+                                                           const unsigned char* __restrict__ scales, bf16_t* __restrict__ out,
+                                                           long total) {
+    for (long at = (long)blockIdx.x * 256 + threadIdx.x; at < total; at += (long)gridDim.x * 256) {
+        const float s = mx_scale(scales[at / 4]);
+        bf16x8 b;
+        if constexpr (FMT == GAN_MX_E4M3) {
+            const uint2 u = *reinterpret_cast<const uint2*>(codes + at * 8);
+            b = e4m3_to_bf16(u.x, u.y, s);
+        } else {
+            b = e2m1_to_bf16(*reinterpret_cast<const unsigned*>(codes + at * 4), s);
+        }
+        *reinterpret_cast<bf16x8*>(out + at * 8) = b;
+    }
+}
+
+// Packed W -> [out][groups * 128] bf16: a lane writes one block, 64 bytes.
+__global__ __launch_bounds__(256) void mx_weights_bf16_kernel(const unsigned char* __restrict__ codes,
+                                                              const unsigned char* __restrict__ scales, bf16_t* __restrict__ out,
+                                                              int groups, int out_dim) {
+    // 4 blocks of 64 outputs; neighbouring lanes take the four blocks of one output, so that 256 bytes of a row are written
+    const int q = threadIdx.x & 3, n = blockIdx.x * 64 + threadIdx.x / 4, g = blockIdx.y;
+    if (n >= out_dim) return;
+    const uint4 u = reinterpret_cast<const uint4*>(codes)[((long)g * 4 + q) * out_dim + n];
+    const float s = mx_scale(scales[((long)g * out_dim + n) * 4 + q]);
+    bf16x8* o = reinterpret_cast<bf16x8*>(out + ((long)n * groups + g) * 128 + q * 32);
+    o[0] = e2m1_to_bf16(u.x, s);
+    o[1] = e2m1_to_bf16(u.y, s);
+    o[2] = e2m1_to_bf16(u.z, s);
+    o[3] = e2m1_to_bf16(u.w, s);
+}
+
+// Packed W -> [in][out filled up to 64] bf16: a lane takes one block of one output; the lanes of a wave are neighbouring
+// outputs, so each of the 32 stores is contiguous.
+__global__ __launch_bounds__(256) void mx_weights_transpose_kernel(const unsigned char* __restrict__ codes,
+                                                                   const unsigned char* __restrict__ scales,
+                                                                   bf16_t* __restrict__ out, int in_dim, int out_dim) {
+    const long np = to64(out_dim);
+    const int n = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6, k0 = blockIdx.y * 128 + q * 32;
+    uint4 u = make_uint4(0, 0, 0, 0);
+    float s = 1.f;
+    if (n < out_dim) {
+        u = reinterpret_cast<const uint4*>(codes)[((long)blockIdx.y * 4 + q) * out_dim + n];
+        s = mx_scale(scales[((long)blockIdx.y * out_dim + n) * 4 + q]);
+    }
+    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bf16x8 b = e2m1_to_bf16(w[i], s);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (k0 + i * 8 + j < in_dim) out[(long)(k0 + i * 8 + j) * np + n] = b[j];
+    }
+}
+
+// dbias[n] (+)= sum over blocks of 64 rows.
+__global__ __launch_bounds__(256) void mx_dbias_kernel(const float* __restrict__ colsum, float* __restrict__ out, int blocks, int n,
+                                                       int accumulate) {
+    __shared__ float red[8][33];
+    const int col = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
+    float s = 0.f;
+    if (col < n)
+        for (int i = part; i < blocks; i += 8) s += colsum[(long)i * n + col];
+    red[part][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (part == 0 && col < n) {
+        s = 0.f;
+        for (int i = 0; i < 8; ++i) s += red[i][threadIdx.x];
+        out[col] = (accumulate ? out[col] : 0.f) + s;
+    }
+}
+
+static dim3 flat_grid(long items) {
+    const long blocks = (items + 255) / 256;
+    return dim3((unsigned)(blocks < 8192 ? (blocks < 1 ? 1 : blocks) : 8192));
+}
+
+void mx_rows_to_bf16(int fmt, const void* codes, const void* scales, bf16_t* out, long rows, int in_dim, hipStream_t st) {
+    const long total = rows * mx_groups(in_dim) * 16;
+    const unsigned char* c = static_cast<const unsigned char*>(codes);
+    const unsigned char* s = static_cast<const unsigned char*>(scales);
+    if (fmt == GAN_MX_E4M3) hipLaunchKernelGGL(mx_rows_bf16_kernel<GAN_MX_E4M3>, flat_grid(total), dim3(256), 0, st, c, s, out, total);
+    else hipLaunchKernelGGL(mx_rows_bf16_kernel<GAN_MX_E2M1>, flat_grid(total), dim3(256), 0, st, c, s, out, total);
+}
+
+void mx_weights_to_bf16(const void* codes, const void* scales, bf16_t* out, int in_dim, int out_dim, hipStream_t st) {
+    hipLaunchKernelGGL(mx_weights_bf16_kernel, dim3((out_dim + 63) / 64, mx_groups(in_dim)), dim3(256), 0, st,
+                       static_cast<const unsigned char*>(codes), static_cast<const unsigned char*>(scales), out, mx_groups(in_dim),
+                       out_dim);
+}
+
+static int parts_of(int dtype) { return dtype == GAN_BF16 ? 1 : dtype == GAN_F16 ? 2 : 3; }
+
+// dY itself is the operand of dA when it is bf16 in whole 64s.
+static bool dy_as_is(int dtype, int out_dim) { return dtype == GAN_BF16 && out_dim % 64 == 0; }
+
+}  // namespace gan
+
+using namespace gan;
+
+extern "C" {
+
+size_t gan_mx_matmul_dgrad_workspace_bytes(int dtype, int rows, int in_dim, int out_dim) {
+    if (rows < 1 || rows > GAN_MX_MAX_ROWS || in_dim < 1 || in_dim > GAN_MX_MAX_IN || out_dim < 1 || !dtype_ok(dtype)) return 0;
+    const size_t np = to64(out_dim), parts = parts_of(dtype);
+    return in_dim * np * 2 + (dy_as_is(dtype, out_dim) ? 0 : parts * rows * np * 2) +
+           bf16_product_workspace(rows, in_dim, (int)parts, (int)np);
+}
+
+int gan_mx_matmul_dgrad(int dtype, int rows, int in_dim, int out_dim, const void* dy, const void* w_codes, const void* w_scales,
+                        void* dx, void* ws, size_t ws_bytes, gan_stream_t stream) {
+    GAN_CHECK_ARG(dtype_ok(dtype), "gan_mx_matmul_dgrad: unknown element type %d", dtype);
+    GAN_CHECK_ARG(rows >= 0 && rows <= GAN_MX_MAX_ROWS && in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1,
+                  "gan_mx_matmul_dgrad: %d rows, %d inputs, %d outputs (up to %d rows and inputs are served)", rows, in_dim, out_dim, GAN_MX_MAX_IN);
+    if (rows == 0) return 0;
+    GAN_CHECK_ARG(dy && w_codes && w_scales && dx, "gan_mx_matmul_dgrad: null pointer");
+    GAN_CHECK_ARG(aligned16(dy) && aligned16(w_codes) && (reinterpret_cast<size_t>(w_scales) & 3) == 0,
+                  "gan_mx_matmul_dgrad: dy and codes have to be 16-byte and scales 4-byte aligned");
+    const size_t need = gan_mx_matmul_dgrad_workspace_bytes(dtype, rows, in_dim, out_dim);
+    GAN_CHECK_ARG(ws && aligned16(ws) && ws_bytes >= need,
+                  "gan_mx_matmul_dgrad: workspace of %zu bytes needed (16-byte aligned), %zu given", need, ws_bytes);
+    const hipStream_t st = as_stream(stream);
+    const long np = to64(out_dim);
+    const int parts = parts_of(dtype);
+    bf16_t* w = static_cast<bf16_t*>(ws);
+    bf16_t* y = w + in_dim * np;
+    hipLaunchKernelGGL(mx_weights_transpose_kernel, dim3((unsigned)(np / 64), mx_groups(in_dim)), dim3(256), 0, st,
+                       static_cast<const unsigned char*>(w_codes), static_cast<const unsigned char*>(w_scales), w, in_dim, out_dim);
+    return with_dtype(dtype, [&](auto* tag) {
+        typedef typename std::remove_pointer<decltype(tag)>::type T;
+        const bf16_t* dyp = static_cast<const bf16_t*>(dy);
+        bf16_t* end = y;
+        if (!dy_as_is(dtype, out_dim)) {
+            hipLaunchKernelGGL((split_rows_kernel<T>), flat_grid(rows * np / 8), dim3(256), 0, st, static_cast<const T*>(dy), y,
+                               (long)rows, out_dim, out_dim * sizeof(T) % 16 == 0);
+            dyp = y;
+            end = y + (long)parts * rows * np;
+        }
+        const Bf16Product p{dyp, w, np, np, rows * np, 0, parts, (int)np, rows, in_dim, nullptr, 0};
+        return bf16_product(p, static_cast<T*>(dx), end, st, "gan_mx_matmul_dgrad");
+    });
+}
+
+size_t gan_mx_matmul_wgrad_workspace_bytes(int dtype, int rows, int in_dim, int out_dim) {
+    if (rows < 1 || rows > GAN_MX_MAX_ROWS || in_dim < 1 || in_dim > GAN_MX_MAX_IN || out_dim < 1 || !dtype_ok(dtype)) return 0;
+    const size_t rp = to64(rows), parts = parts_of(dtype);
+    return (in_dim + parts * out_dim) * rp * 2 + (rp / 64 * out_dim * 4 + 15) / 16 * 16 +
+           bf16_product_workspace(in_dim, out_dim, (int)parts, (int)rp);
+}
+
+int gan_mx_matmul_wgrad(int dtype, int fmt, int rows, int in_dim, int out_dim, const void* a_codes, const void* a_scales,
+                        const void* dy, float* dmatrix, float* dbias, int accumulate, void* ws, size_t ws_bytes,
+                        gan_stream_t stream) {
+    GAN_CHECK_ARG(dtype_ok(dtype) && mx_fmt_ok(fmt), "gan_mx_matmul_wgrad: unknown element type %d or format %d", dtype, fmt);
+    GAN_CHECK_ARG(rows >= 1 && rows <= GAN_MX_MAX_ROWS && in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1,
+                  "gan_mx_matmul_wgrad: %d rows, %d inputs, %d outputs (up to %d rows and inputs are served)", rows, in_dim, out_dim, GAN_MX_MAX_IN);
+    GAN_CHECK_ARG(dy && a_codes && a_scales && dmatrix, "gan_mx_matmul_wgrad: null pointer");
+    GAN_CHECK_ARG(aligned16(dy) && aligned16(a_codes), "gan_mx_matmul_wgrad: dy and codes have to be 16-byte aligned");
+    const size_t need = gan_mx_matmul_wgrad_workspace_bytes(dtype, rows, in_dim, out_dim);
+    GAN_CHECK_ARG(ws && aligned16(ws) && ws_bytes >= need,
+                  "gan_mx_matmul_wgrad: workspace of %zu bytes needed (16-byte aligned), %zu given", need, ws_bytes);
+    const hipStream_t st = as_stream(stream);
+    const long rp = to64(rows);
+    const int parts = parts_of(dtype), blocks = (int)(rp / 64);
+    bf16_t* a = static_cast<bf16_t*>(ws);
+    bf16_t* y = a + in_dim * rp;
+    float* colsum = reinterpret_cast<float*>(y + (long)parts * out_dim * rp);
+    void* end = reinterpret_cast<char*>(colsum) + ((size_t)blocks * out_dim * 4 + 15) / 16 * 16;
+    const dim3 ga((in_dim + 63) / 64, blocks), gy((out_dim + 63) / 64, blocks);
+    const unsigned char* c = static_cast<const unsigned char*>(a_codes);
+    const unsigned char* s = static_cast<const unsigned char*>(a_scales);
+    if (fmt == GAN_MX_E4M3) hipLaunchKernelGGL(mx_rows_transpose_kernel<GAN_MX_E4M3>, ga, dim3(256), 0, st, c, s, a, rows, in_dim);
+    else hipLaunchKernelGGL(mx_rows_transpose_kernel<GAN_MX_E2M1>, ga, dim3(256), 0, st, c, s, a, rows, in_dim);
+    return with_dtype(dtype, [&](auto* tag) {
+        typedef typename std::remove_pointer<decltype(tag)>::type T;
+        hipLaunchKernelGGL((split_transpose_kernel<T>), gy, dim3(256), 0, st, static_cast<const T*>(dy), y,
+                           dbias ? colsum : nullptr, rows, out_dim, out_dim * sizeof(T) % 16 == 0);
+        if (dbias)
+            hipLaunchKernelGGL(mx_dbias_kernel, dim3((out_dim + 31) / 32), dim3(256), 0, st, colsum, dbias, blocks, out_dim, accumulate);
+        const Bf16Product p{a, y, rp, rp, 0, out_dim * rp, parts, (int)rp, in_dim, out_dim, nullptr, accumulate};
+        return bf16_product(p, dmatrix, end, st, "gan_mx_matmul_wgrad");
+    });
+}
+
+}  // extern "C"

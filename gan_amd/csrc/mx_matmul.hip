@@ -1,0 +1,326 @@
+// y[r][n] = sum_k A[r][k] W[k][n] + bias[n] with microscaled A (e4m3 or e2m1, rows) and W (e2m1, packed); fp32 accumulation.
+//
+// Which pipe: the scaled matrix instruction multiplies the codes as they are, at 2 (e4m3 x e2m1) or 4 (e2m1 x e2m1) times the
+// bf16 rate.  Its sum over the 64 deep products of one instruction drops what lies far below the largest of them: with normally
+// distributed operands 4e-6 of a result for e4m3 x e2m1, 6e-5 where the values of a block span 2^16; none seen for
+// e2m1 x e2m1.  That is far below the rounding of a 16-bit result (2^-9, 2^-12), but not fp32: e4m3 products with fp32 results
+// take the bf16 pipe instead, where every operand value is exact and sums are fp32.
+#include "mx_gemm.h"
+
+namespace gan {
+
+struct MxProduct {
+    const unsigned char* a;         // [rows][groups][128 or 64 bytes]
+    const unsigned char* as;        // [rows][groups][4]
+    const unsigned char* w;         // [groups * 4][n][16]
+    const unsigned char* ws;        // [groups][n][4]
+    const float* bias;
+    void* y;
+    float* slabs;                   // split contraction: [splits][rows][n rounded up to 4]
+    int rows, n, groups, splits;
+    bool vec;
+};
+
+// ------------------------------------------------------------------------------------------------ many rows
+// Tile of BN outputs x BR rows, WN x WR waves; the weights are the first operand of the 32x32x64 instruction, so that a lane ends
+// with four consecutive outputs of one row.  A step is one group (128 deep): weights 4 blocks x BN x 16 bytes, contiguous as
+// packed and as read back (a lane's fragment is one block); rows 128 (64) bytes each, their 16-byte chunks swapped by row so
+// that the 32 rows of a fragment read hit all banks.  Two stages in LDS, filled by direct copies one step ahead; the scale
+// dwords go to registers one step ahead.
+template <typename T, int FMT, int BN, int BR, int WN, int WR>
+__global__ __launch_bounds__(64 * WN * WR) void mx_tile_kernel(MxProduct p) {
+    constexpr int THREADS = 64 * WN * WR, FN = BN / WN / 32, FR = BR / WR / 32;
+    constexpr int ROW = FMT == GAN_MX_E4M3 ? 128 : 64, CH = ROW / 16;
+    constexpr int W_BYTES = BN * 64, STAGE = W_BYTES + BR * ROW;
+    extern __shared__ __align__(16) unsigned char lds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wn = wave % WN, wr = wave / WN;
+    const int l32 = lane & 31, half = lane >> 5;
+    const int tr = (p.rows + BR - 1) / BR, tn = (p.n + BN - 1) / BN;
+    int ir, in;
+    tile_of(blockIdx.x, tr, tn, ir, in);
+    const int r0 = ir * BR, n0 = in * BN;
+    const int g0 = (int)((long)p.groups * blockIdx.y / p.splits), g1 = (int)((long)p.groups * (blockIdx.y + 1) / p.splits);
+
+    auto fill = [&](int g, int buf) {
+        unsigned char* base = lds + buf * STAGE;
+#pragma unroll
+        for (int i = 0; i < W_BYTES / 16 / THREADS; ++i) {
+            const int at = (i * WN * WR + wave) * 64;            // 64 blocks, one kb
+            const int kb = at / BN, n = min(n0 + at % BN + lane, p.n - 1);
+            copy_to_lds16(p.w + (((long)g * 4 + kb) * p.n + n) * 16, base + at * 16);
+        }
+#pragma unroll
+        for (int i = 0; i < BR * CH / THREADS; ++i) {
+            const int at = (i * WN * WR + wave) * 64, s = at + lane, row = s / CH;
+            const int chunk = (s % CH) ^ (CH == 8 ? row & 7 : (row >> 2) & 3);
+            const int r = min(r0 + row, p.rows - 1);
+            copy_to_lds16(p.a + ((long)r * p.groups + g) * ROW + chunk * 16, base + W_BYTES + at * 16);
+        }
+    };
+    int sw[FN], sa[FR], nw[FN], na[FR];
+    auto scales = [&](int g, int (&w)[FN], int (&a)[FR]) {
+#pragma unroll
+        for (int f = 0; f < FN; ++f)
+            w[f] = reinterpret_cast<const int*>(p.ws)[(long)g * p.n + min(n0 + (wn * FN + f) * 32 + l32, p.n - 1)];
+#pragma unroll
+        for (int f = 0; f < FR; ++f)
+            a[f] = reinterpret_cast<const int*>(p.as)[(long)min(r0 + (wr * FR + f) * 32 + l32, p.rows - 1) * p.groups + g];
+    };
+
+    f32x16 acc[FN][FR];
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FR; ++j)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) acc[i][j][k] = 0.f;
+
+    if (g0 < g1) {
+        fill(g0, 0);
+        scales(g0, nw, na);
+    }
+    for (int g = g0; g < g1; ++g) {
+        const int buf = (g - g0) & 1;
+        copies_done_barrier();
+        // bytes 0 and 2 become this half's blocks of the two 64-deep halves of the step
+#pragma unroll
+        for (int f = 0; f < FN; ++f) sw[f] = (int)((unsigned)nw[f] >> (8 * half));
+#pragma unroll
+        for (int f = 0; f < FR; ++f) sa[f] = (int)((unsigned)na[f] >> (8 * half));
+        if (g + 1 < g1) {
+            fill(g + 1, buf ^ 1);
+            scales(g + 1, nw, na);
+        }
+        const unsigned char* lw = lds + buf * STAGE;
+        const unsigned char* la = lw + W_BYTES;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            i32x8 fw[FN], fa[FR];
+#pragma unroll
+            for (int f = 0; f < FN; ++f) {
+                const i32x4 t = *reinterpret_cast<const i32x4*>(lw + ((2 * s + half) * BN + (wn * FN + f) * 32 + l32) * 16);
+                fw[f] = i32x8{t[0], t[1], t[2], t[3], 0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int f = 0; f < FR; ++f) {
+                const int row = (wr * FR + f) * 32 + l32;
+                const unsigned char* rp = la + row * ROW;
+                if constexpr (FMT == GAN_MX_E4M3) {
+                    // the 8-bit operand holds 16 values of each 32-deep quarter: chunks h and 2 + h of the half step
+                    const i32x4 t = *reinterpret_cast<const i32x4*>(rp + (((4 * s + half) ^ (row & 7)) * 16));
+                    const i32x4 u = *reinterpret_cast<const i32x4*>(rp + (((4 * s + 2 + half) ^ (row & 7)) * 16));
+                    fa[f] = i32x8{t[0], t[1], t[2], t[3], u[0], u[1], u[2], u[3]};
+                } else {
+                    const i32x4 t = *reinterpret_cast<const i32x4*>(rp + (((2 * s + half) ^ ((row >> 2) & 3)) * 16));
+                    fa[f] = i32x8{t[0], t[1], t[2], t[3], 0, 0, 0, 0};
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < FN; ++i)
+#pragma unroll
+                for (int j = 0; j < FR; ++j) {
+                    constexpr int kB = FMT == GAN_MX_E4M3 ? 0 : 4;
+                    acc[i][j] = s == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[i], fa[j], acc[i][j], 4, kB, 0, sw[i], 0, sa[j])
+                                       : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[i], fa[j], acc[i][j], 4, kB, 2, sw[i], 2, sa[j]);
+                }
+        }
+        // (the barrier at the top of the next step is also what lets its copies overwrite the stage read here one step later)
+    }
+    const int n4 = (p.n + 3) / 4 * 4;
+#pragma unroll
+    for (int j = 0; j < FR; ++j) {
+        const int r = r0 + (wr * FR + j) * 32 + l32;
+        if (r >= p.rows) continue;
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int n = n0 + (wn * FN + i) * 32 + 8 * q + 4 * half;
+                const f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                if (p.slabs) {
+                    if (n < p.n) *reinterpret_cast<f32x4*>(p.slabs + ((long)blockIdx.y * p.rows + r) * n4 + n) = v;
+                } else {
+                    store4(static_cast<T*>(p.y) + (long)r * p.n, n, p.n, p.vec, v, p.bias, 0);
+                }
+            }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ few rows
+// The weights' bytes bind.  A wave takes NT x 16 outputs and every WAVES-th group; its lanes load weight fragments (one block of
+// 16 bytes each) straight from global memory, turn codes into bf16 and multiply on the bf16 pipe, which also makes the sums
+// fp32 for every result type.  RT tiles of 16 rows share each converted fragment.  The waves' sums meet in LDS.
+template <typename T, int FMT, int NT, int RT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void mx_few_kernel(MxProduct p) {
+    constexpr int ROW = FMT == GAN_MX_E4M3 ? 128 : 64, BLK = ROW / 4;
+    __shared__ f32x4 red[WAVES][NT * RT][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, q = lane >> 4;
+    const int n0 = blockIdx.x * NT * 16, r0 = blockIdx.z * RT * 16;
+    const int g0 = (int)((long)p.groups * blockIdx.y / p.splits), g1 = (int)((long)p.groups * (blockIdx.y + 1) / p.splits);
+    f32x4 acc[NT][RT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < RT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    int n[NT], r[RT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) n[i] = min(n0 + i * 16 + l16, p.n - 1);
+#pragma unroll
+    for (int j = 0; j < RT; ++j) r[j] = min(r0 + j * 16 + l16, p.rows - 1);
+    for (int g = g0 + wave; g < g1; g += WAVES) {
+        uint4 cw[NT];
+        unsigned sw[NT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            cw[i] = reinterpret_cast<const uint4*>(p.w)[((long)g * 4 + q) * p.n + n[i]];
+            sw[i] = p.ws[((long)g * p.n + n[i]) * 4 + q];
+        }
+        bf16x8 a[RT][4];
+#pragma unroll
+        for (int j = 0; j < RT; ++j) {
+            const unsigned char* at = p.a + ((long)r[j] * p.groups + g) * ROW + q * BLK;
+            const float s = mx_scale(p.as[((long)r[j] * p.groups + g) * 4 + q]);
+            const uint4 u = *reinterpret_cast<const uint4*>(at);
+            if constexpr (FMT == GAN_MX_E4M3) {
+                const uint4 v = *reinterpret_cast<const uint4*>(at + 16);
+                a[j][0] = e4m3_to_bf16(u.x, u.y, s);
+                a[j][1] = e4m3_to_bf16(u.z, u.w, s);
+                a[j][2] = e4m3_to_bf16(v.x, v.y, s);
+                a[j][3] = e4m3_to_bf16(v.z, v.w, s);
+            } else {
+                a[j][0] = e2m1_to_bf16(u.x, s);
+                a[j][1] = e2m1_to_bf16(u.y, s);
+                a[j][2] = e2m1_to_bf16(u.z, s);
+                a[j][3] = e2m1_to_bf16(u.w, s);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const float s = mx_scale(sw[i]);
+            const unsigned u[4] = {cw[i].x, cw[i].y, cw[i].z, cw[i].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const bf16x8 b = e2m1_to_bf16(u[k], s);
+#pragma unroll
+                for (int j = 0; j < RT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, a[j][k], acc[i][j], 0, 0, 0);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < RT; ++j) red[wave][i * RT + j][lane] = acc[i][j];
+    __syncthreads();
+    const int n4 = (p.n + 3) / 4 * 4;
+    for (int e = wave; e < NT * RT; e += WAVES) {
+        f32x4 v = red[0][e][lane];
+        for (int w = 1; w < WAVES; ++w) v += red[w][e][lane];
+        const int row = r0 + (e % RT) * 16 + l16, col = n0 + (e / RT) * 16 + 4 * q;
+        if (row >= p.rows || col >= p.n) continue;
+        if (p.slabs) *reinterpret_cast<f32x4*>(p.slabs + ((long)blockIdx.y * p.rows + row) * n4 + col) = v;
+        else store4(static_cast<T*>(p.y) + (long)row * p.n, col, p.n, p.vec, v, p.bias, 0);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ choice of the kernel
+enum { MX_FEW, MX_TILE_SMALL, MX_TILE_LARGE, MX_VIA_BF16 };
+struct MxPlan {
+    int kind, splits;
+};
+
+constexpr int kFewRows = 64;
+
+static MxPlan mx_plan(int dtype, int fmt, int rows, int in_dim, int out_dim) {
+    const int groups = mx_groups(in_dim);
+    if (rows <= kFewRows) {
+        const long wgs = (long)((out_dim + 15) / 16) * ((rows + 31) / 32);
+        long s = wgs >= 256 ? 1 : 256 / wgs;
+        if (s > groups / 8) s = groups / 8;
+        return {MX_FEW, s < 1 ? 1 : (int)s};
+    }
+    if (fmt == GAN_MX_E4M3 && dtype == GAN_F32) return {MX_VIA_BF16, 1};
+    const long large = (long)((rows + 255) / 256) * ((out_dim + 255) / 256);
+    if (large >= 192) return {MX_TILE_LARGE, 1};
+    return {MX_TILE_SMALL, contraction_splits((long)((rows + 127) / 128) * ((out_dim + 127) / 128), groups, 4)};
+}
+
+template <typename T, int FMT, int BN, int BR, int WN, int WR>
+static int launch_tile(const MxProduct& p, hipStream_t st) {
+    constexpr int LDS = 2 * (BN * 64 + BR * (FMT == GAN_MX_E4M3 ? 128 : 64));
+    auto kernel = mx_tile_kernel<T, FMT, BN, BR, WN, WR>;
+    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                      hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (set != hipSuccess) return fail("gan_mx_matmul: %d bytes of LDS refused: %s", LDS, hipGetErrorString(set));
+    const long tiles = (long)((p.rows + BR - 1) / BR) * ((p.n + BN - 1) / BN);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, p.splits), dim3(64 * WN * WR), LDS, st, p);
+    return 0;
+}
+
+template <typename T, int FMT>
+static int launch_few(const MxProduct& p, hipStream_t st) {
+    const dim3 grid((p.n + 15) / 16, p.splits, (p.rows + 31) / 32);
+    if (p.rows <= 16) hipLaunchKernelGGL((mx_few_kernel<T, FMT, 1, 1, 8>), grid, dim3(512), 0, st, p);
+    else hipLaunchKernelGGL((mx_few_kernel<T, FMT, 1, 2, 8>), grid, dim3(512), 0, st, p);
+    return 0;
+}
+
+static size_t mx_bf16_bytes(long rows, int in_dim) { return (size_t)rows * mx_groups(in_dim) * 256; }
+
+}  // namespace gan
+
+using namespace gan;
+
+extern "C" {
+
+size_t gan_mx_matmul_workspace_bytes(int dtype, int fmt, int rows, int in_dim, int out_dim) {
+    if (rows < 1 || rows > GAN_MX_MAX_ROWS || in_dim < 1 || in_dim > GAN_MX_MAX_IN || out_dim < 1 || !dtype_ok(dtype) || !mx_fmt_ok(fmt)) return 0;
+    const MxPlan plan = mx_plan(dtype, fmt, rows, in_dim, out_dim);
+    if (plan.kind == MX_VIA_BF16)
+        return mx_bf16_bytes(rows, in_dim) + mx_bf16_bytes(out_dim, in_dim) +
+               bf16_product_workspace(rows, out_dim, 1, mx_groups(in_dim) * 128);
+    return slab_bytes(plan.splits, rows, out_dim);
+}
+
+int gan_mx_matmul(int dtype, int fmt, int rows, int in_dim, int out_dim, const void* a_codes, const void* a_scales,
+                  const void* w_codes, const void* w_scales, const float* bias, void* y, void* ws, size_t ws_bytes,
+                  gan_stream_t stream) {
+    GAN_CHECK_ARG(dtype_ok(dtype) && mx_fmt_ok(fmt), "gan_mx_matmul: unknown element type %d or format %d", dtype, fmt);
+    GAN_CHECK_ARG(rows >= 0 && rows <= GAN_MX_MAX_ROWS && in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1,
+                  "gan_mx_matmul: %d rows, %d inputs, %d outputs (up to %d rows and inputs are served)", rows, in_dim, out_dim, GAN_MX_MAX_IN);
+    if (rows == 0) return 0;
+    GAN_CHECK_ARG(a_codes && a_scales && w_codes && w_scales && y, "gan_mx_matmul: null pointer");
+    GAN_CHECK_ARG(aligned16(a_codes) && aligned16(w_codes) && ((reinterpret_cast<size_t>(a_scales) | reinterpret_cast<size_t>(w_scales)) & 3) == 0,
+                  "gan_mx_matmul: codes have to be 16-byte and scales 4-byte aligned");
+    const size_t need = gan_mx_matmul_workspace_bytes(dtype, fmt, rows, in_dim, out_dim);
+    GAN_CHECK_ARG(ws_bytes >= need && (need == 0 || (ws && aligned16(ws))),
+                  "gan_mx_matmul: workspace of %zu bytes needed (16-byte aligned), %zu given", need, ws_bytes);
+    const MxPlan plan = mx_plan(dtype, fmt, rows, in_dim, out_dim);
+    const hipStream_t st = as_stream(stream);
+    if (plan.kind == MX_VIA_BF16) {
+        const int kp = mx_groups(in_dim) * 128;
+        bf16_t* a = static_cast<bf16_t*>(ws);
+        bf16_t* w = a + (long)rows * kp;
+        mx_rows_to_bf16(fmt, a_codes, a_scales, a, rows, in_dim, st);
+        mx_weights_to_bf16(w_codes, w_scales, w, in_dim, out_dim, st);
+        const Bf16Product p{a, w, kp, kp, 0, 0, 1, kp, rows, out_dim, bias, 0};
+        return bf16_product(p, static_cast<float*>(y), w + (long)out_dim * kp, st, "gan_mx_matmul");
+    }
+    return with_dtype(dtype, [&](auto* tag) {
+        typedef typename std::remove_pointer<decltype(tag)>::type T;
+        const bool vec = out_dim % 4 == 0 && (reinterpret_cast<size_t>(y) & (4 * sizeof(T) - 1)) == 0 && aligned16(bias);
+        MxProduct p{static_cast<const unsigned char*>(a_codes), static_cast<const unsigned char*>(a_scales),
+                    static_cast<const unsigned char*>(w_codes), static_cast<const unsigned char*>(w_scales),
+                    bias, y, plan.splits > 1 ? static_cast<float*>(ws) : nullptr, rows, out_dim, mx_groups(in_dim), plan.splits, vec};
+        int rc;
+        if (plan.kind == MX_FEW) rc = fmt == GAN_MX_E4M3 ? launch_few<T, GAN_MX_E4M3>(p, st) : launch_few<T, GAN_MX_E2M1>(p, st);
+        else if (plan.kind == MX_TILE_LARGE)
+            rc = fmt == GAN_MX_E4M3 ? launch_tile<T, GAN_MX_E4M3, 256, 256, 2, 4>(p, st) : launch_tile<T, GAN_MX_E2M1, 256, 256, 2, 4>(p, st);
+        else
+            rc = fmt == GAN_MX_E4M3 ? launch_tile<T, GAN_MX_E4M3, 128, 128, 2, 2>(p, st) : launch_tile<T, GAN_MX_E2M1, 128, 128, 2, 2>(p, st);
+        if (rc) return rc;
+        if (plan.splits > 1) join_slabs(p.slabs, plan.splits, static_cast<T*>(y), (long)rows, out_dim, bias, 0, vec, st);
+        return check_launch("gan_mx_matmul");
+    });
+}
+
+}  // extern "C"

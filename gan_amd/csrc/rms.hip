@@ -1,0 +1,295 @@
+// Root-mean-square norm with the residual's addition, forward and backward.
+//
+//   h = T(x + r)   s = 1 / sqrt(mean(h^2) + eps)   y = h s gamma
+//   g = dy gamma   n = h s   dx = dr = s (g - n mean(g n)) + dh   dgamma = sum over rows of dy n
+//
+// h is rounded to the tensors' type before it is normalised: it is the residual stream that is stored and that the backward
+// pass reads again, so forward and backward see one h.  Sums are fp32; in front of the 8-bit output they, and y, are fp64:
+// the row is one division away from a grid with steps of 1/8, and with y rounded once from 64 bits a value next to a border
+// falls on its own side (fp64 runs at the fp32 rate here, and the kernel waits for memory: no cost was measurable).
+//
+// Memory-bound.  A team of 64, 256 or 1024 threads keeps a whole row in registers, eight values a chunk, so every tensor is
+// read and written once.
+#include "mx.h"
+
+namespace gan {
+
+template <typename S>
+__device__ __forceinline__ S team_sum(S v, int tpr, S* red) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    if (tpr > 64) {
+        const int wave = threadIdx.x >> 6, waves = tpr >> 6;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) red[wave] = v;
+        __syncthreads();
+        v = 0;
+        for (int i = 0; i < waves; ++i) v += red[i];
+    }
+    return v;
+}
+
+struct RmsFwd {
+    const void* x;
+    const void* res;
+    const float* gamma;
+    void* h;
+    void* y;
+    unsigned char* codes;
+    unsigned char* scales;
+    float* rstd;
+    long rows, ldx, ldr;
+    int c;
+    float eps;
+    bool vec_x, vec_r, vec_o, vec_g;
+};
+
+template <typename T, int TPR, int NV, bool MX>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(RmsFwd p) {
+    constexpr int TEAMS = TPR < 256 ? 256 / TPR : 1;
+    __shared__ double red_d[TPR / 64];
+    __shared__ float red_f[TPR / 64];
+    const int t = threadIdx.x % TPR, team = threadIdx.x / TPR;
+    const int c = p.c, chunks = MX ? mx_groups(c) * 16 : (c + 7) / 8;
+    for (long row0 = (long)blockIdx.x * TEAMS; row0 < p.rows; row0 += (long)gridDim.x * TEAMS) {
+        const long row = row0 + team;
+        const bool live = row < p.rows;
+        const T* xr = static_cast<const T*>(p.x) + (live ? row : 0) * p.ldx;
+        const T* rr = p.res ? static_cast<const T*>(p.res) + (live ? row : 0) * p.ldr : nullptr;
+        float v[NV][8];
+        double sd = 0;
+        float sf = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int i0 = (i * TPR + t) * 8;
+            load8(xr, i0, i0 < c ? c : 0, p.vec_x, v[i]);
+            if (rr) {
+                float r[8];
+                load8(rr, i0, i0 < c ? c : 0, p.vec_r, r);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] = (float)(T)(v[i][j] + r[j]);
+                if (live && i0 < c) store8(static_cast<T*>(p.h) + row * c, i0, c, p.vec_o, v[i]);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (MX) sd = fma((double)v[i][j], (double)v[i][j], sd);
+                else sf = fmaf(v[i][j], v[i][j], sf);
+            }
+        }
+        float rstd;
+        double inv = 0;
+        if (MX) {
+            inv = 1.0 / sqrt(team_sum(sd, TPR, red_d) / c + (double)p.eps);
+            rstd = (float)inv;
+        } else {
+            rstd = 1.f / sqrtf(team_sum(sf, TPR, red_f) / c + p.eps);
+        }
+        if (!live) continue;    // (a team of 64 takes no barrier, a larger one is the whole block)
+        if (p.rstd && t == 0) p.rstd[row] = rstd;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int chunk = i * TPR + t, i0 = chunk * 8;
+            float g[8], y[8];
+            load8(p.gamma, i0, i0 < c ? c : 0, p.vec_g, g);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                y[j] = MX ? (float)((double)v[i][j] * inv * (double)g[j]) : v[i][j] * rstd * g[j];
+            if (MX) {
+                unsigned code[2];
+                const unsigned byte = mx_quantize_lane8<GAN_MX_E4M3>(y, code);   // (all lanes: the block's four exchange maxima)
+                if (chunk < chunks) {
+                    *reinterpret_cast<uint2*>(p.codes + row * (chunks * 8L) + i0) = make_uint2(code[0], code[1]);
+                    if ((chunk & 3) == 0) p.scales[row * (chunks / 4L) + chunk / 4] = (unsigned char)byte;
+                }
+            } else if (i0 < c) {
+                store8(static_cast<T*>(p.y) + row * c, i0, c, p.vec_o, y);
+            }
+        }
+    }
+}
+
+struct RmsBwd {
+    const void* h;
+    const float* gamma;
+    const float* rstd;
+    const void* dy;
+    const void* dh;
+    void* dx;
+    float* partial;     // [teams of the grid][c], or null
+    long rows, ldh;
+    int c;
+    bool vec_h, vec_o, vec_g;
+};
+
+// Every team walks the rows from its own number on in steps of the number of teams and adds dy n up in registers (the
+// columns of a thread are the same in every row); rms_dgamma_kernel joins the teams in a fixed order.
+template <typename T, int TPR, int NV>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(RmsBwd p) {
+    constexpr int TEAMS = TPR < 256 ? 256 / TPR : 1;
+    __shared__ float red[TPR / 64];
+    const int t = threadIdx.x % TPR, c = p.c;
+    const long team = (long)blockIdx.x * TEAMS + threadIdx.x / TPR, teams = (long)gridDim.x * TEAMS;
+    float acc[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[i][j] = 0.f;
+    for (long row = team; row < p.rows; row += teams) {
+        const T* hr = static_cast<const T*>(p.h) + row * p.ldh;
+        const T* yr = static_cast<const T*>(p.dy) + row * c;
+        const float rstd = p.rstd[row];
+        float n[NV][8], g[NV][8], s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int i0 = (i * TPR + t) * 8, cc = i0 < c ? c : 0;
+            float w[8];
+            load8(hr, i0, cc, p.vec_h, n[i]);
+            load8(yr, i0, cc, p.vec_o, g[i]);
+            load8(p.gamma, i0, cc, p.vec_g, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                n[i][j] *= rstd;
+                acc[i][j] = fmaf(g[i][j], n[i][j], acc[i][j]);
+                g[i][j] *= w[j];
+                s = fmaf(g[i][j], n[i][j], s);
+            }
+        }
+        if (!p.dx) continue;
+        const float m = team_sum(s, TPR, red) / c;
+        const T* dhr = p.dh ? static_cast<const T*>(p.dh) + row * c : nullptr;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int i0 = (i * TPR + t) * 8;
+            if (i0 >= c) continue;
+            float d[8];
+            if (dhr) load8(dhr, i0, c, p.vec_o, d);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float v = rstd * (g[i][j] - n[i][j] * m);
+                d[j] = dhr ? v + d[j] : v;
+            }
+            store8(static_cast<T*>(p.dx) + row * c, i0, c, p.vec_o, d);
+        }
+    }
+    if (p.partial) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int i0 = (i * TPR + t) * 8;
+            if (i0 < c) store8(p.partial + team * c, i0, c, (c & 3) == 0, acc[i]);
+        }
+    }
+}
+
+// dgamma[col] (+)= sum over teams of partial[team][col]: 16 columns a block, 16 teams side by side, joined in LDS.
+__global__ __launch_bounds__(256) void rms_dgamma_kernel(const float* __restrict__ partial, float* __restrict__ out, int teams,
+                                                         int c, int accumulate) {
+    __shared__ float red[16][17];
+    const int col = blockIdx.x * 16 + (threadIdx.x & 15), part = threadIdx.x >> 4;
+    float s = 0.f;
+    if (col < c)
+        for (int i = part; i < teams; i += 16) s += partial[(long)i * c + col];
+    red[part][threadIdx.x & 15] = s;
+    __syncthreads();
+    if (part == 0 && col < c) {
+        s = 0.f;
+        for (int i = 0; i < 16; ++i) s += red[i][threadIdx.x];
+        out[col] = (accumulate ? out[col] : 0.f) + s;
+    }
+}
+
+// Teams of the backward grid.
+static int rms_bwd_teams(long rows, int c) {
+    const int per = c <= 2048 ? 4 : 1;
+    long teams = c <= 2048 ? 1024 : c <= 16384 ? 512 : 256;
+    if (teams > rows) teams = rows;
+    return (int)((teams + per - 1) / per * per);
+}
+
+// Calls f(threads a row, chunks a thread) with the smallest shape that holds `chunks` chunks of eight.
+template <typename F>
+static void with_shape(int chunks, F f) {
+    if (chunks <= 64) f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
+    else if (chunks <= 128) f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
+    else if (chunks <= 256) f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
+    else if (chunks <= 512) f(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
+    else if (chunks <= 1024) f(std::integral_constant<int, 256>(), std::integral_constant<int, 4>());
+    else if (chunks <= 2048) f(std::integral_constant<int, 256>(), std::integral_constant<int, 8>());
+    else f(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
+}
+
+constexpr int kRmsMaxWidth = 32768;
+
+}  // namespace gan
+
+using namespace gan;
+
+extern "C" {
+
+int gan_rms_norm_fwd(int dtype, long rows, int c, const void* x, long ldx, const void* residual, long ldr, const float* gamma,
+                     float eps, void* h, void* y, void* mx_codes, void* mx_scales, float* rstd, gan_stream_t stream) {
+    GAN_CHECK_ARG(dtype_ok(dtype), "gan_rms_norm_fwd: unknown element type %d", dtype);
+    GAN_CHECK_ARG(rows >= 0 && rows < (1L << 31) && c >= 1 && c <= kRmsMaxWidth,
+                  "gan_rms_norm_fwd: %ld rows of %d values (1..%d values are served)", rows, c, kRmsMaxWidth);
+    const bool mx = mx_codes != nullptr;
+    GAN_CHECK_ARG(gamma && (rows == 0 || (x && (mx ? mx_scales && !y : y != nullptr) && (residual != nullptr) == (h != nullptr))),
+                  "gan_rms_norm_fwd: null pointer (x, gamma, one of y or mx_codes with mx_scales; h exactly with a residual)");
+    GAN_CHECK_ARG(ldx >= c && (!residual || ldr >= c), "gan_rms_norm_fwd: row stride smaller than the row");
+    GAN_CHECK_ARG(!mx || ((reinterpret_cast<size_t>(mx_codes) & 7) == 0), "gan_rms_norm_fwd: mx_codes is not 8-byte aligned");
+    if (rows == 0) return 0;
+    return with_dtype(dtype, [&](auto* tag) {
+        typedef typename std::remove_pointer<decltype(tag)>::type T;
+        RmsFwd p{x, residual, gamma, h, y, static_cast<unsigned char*>(mx_codes), static_cast<unsigned char*>(mx_scales), rstd,
+                 rows, ldx, ldr, c, eps,
+                 aligned16(x) && ldx * sizeof(T) % 16 == 0, aligned16(residual) && ldr * sizeof(T) % 16 == 0,
+                 c * sizeof(T) % 16 == 0 && aligned16(h) && aligned16(y), aligned16(gamma)};
+        with_shape(mx ? mx_groups(c) * 16 : (c + 7) / 8, [&](auto tpr, auto nv) {
+            constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, TEAMS = TPR < 256 ? 256 / TPR : 1;
+            const dim3 grid((unsigned)((rows + TEAMS - 1) / TEAMS)), block(TPR < 256 ? 256 : TPR);
+            if (mx) hipLaunchKernelGGL((rms_fwd_kernel<T, TPR, NV, true>), grid, block, 0, as_stream(stream), p);
+            else hipLaunchKernelGGL((rms_fwd_kernel<T, TPR, NV, false>), grid, block, 0, as_stream(stream), p);
+        });
+        return check_launch("gan_rms_norm_fwd");
+    });
+}
+
+size_t gan_rms_norm_workspace_bytes(long rows, int c) {
+    if (rows <= 0 || c < 1) return 0;
+    return (size_t)rms_bwd_teams(rows, c) * c * sizeof(float);
+}
+
+int gan_rms_norm_bwd(int dtype, long rows, int c, const void* h, long ldh, const float* gamma, const float* rstd, const void* dy,
+                     const void* dh, void* dx, float* dgamma, int accumulate, void* ws, size_t ws_bytes, gan_stream_t stream) {
+    GAN_CHECK_ARG(dtype_ok(dtype), "gan_rms_norm_bwd: unknown element type %d", dtype);
+    GAN_CHECK_ARG(rows >= 0 && rows < (1L << 31) && c >= 1 && c <= kRmsMaxWidth,
+                  "gan_rms_norm_bwd: %ld rows of %d values (1..%d values are served)", rows, c, kRmsMaxWidth);
+    GAN_CHECK_ARG(gamma && (rows == 0 || (h && rstd && dy)) && (dx || dgamma), "gan_rms_norm_bwd: null pointer");
+    GAN_CHECK_ARG(ldh >= c, "gan_rms_norm_bwd: row stride smaller than the row");
+    const size_t need = dgamma ? gan_rms_norm_workspace_bytes(rows, c) : 0;
+    GAN_CHECK_ARG(ws_bytes >= need && (need == 0 || (ws && aligned16(ws))),
+                  "gan_rms_norm_bwd: workspace of %zu bytes needed (16-byte aligned), %zu given", need, ws_bytes);
+    const int teams = rows ? rms_bwd_teams(rows, c) : 0;
+    float* partial = dgamma ? static_cast<float*>(ws) : nullptr;
+    if (rows) {
+        const int rc = with_dtype(dtype, [&](auto* tag) {
+            typedef typename std::remove_pointer<decltype(tag)>::type T;
+            RmsBwd p{h, gamma, rstd, dy, dh, dx, partial, rows, ldh, c,
+                     aligned16(h) && ldh * sizeof(T) % 16 == 0,
+                     c * sizeof(T) % 16 == 0 && aligned16(dy) && aligned16(dh) && aligned16(dx), aligned16(gamma)};
+            with_shape((c + 7) / 8, [&](auto tpr, auto nv) {
+                constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, TEAMS = TPR < 256 ? 256 / TPR : 1;
+                hipLaunchKernelGGL((rms_bwd_kernel<T, TPR, NV>), dim3(teams / TEAMS), dim3(TPR < 256 ? 256 : TPR), 0,
+                                   as_stream(stream), p);
+            });
+            return check_launch("gan_rms_norm_bwd");
+        });
+        if (rc) return rc;
+    }
+    if (dgamma) {
+        hipLaunchKernelGGL(rms_dgamma_kernel, dim3((c + 15) / 16), dim3(256), 0, as_stream(stream), partial, dgamma, teams, c,
+                           accumulate);
+        return check_launch("gan_rms_norm_bwd");
+    }
+    return 0;
+}
+
+}  // extern "C"

@@ -9,9 +9,12 @@ Drop-in surface (names, positional order and defaults as in the reference, ops.p
     linear(input_, output_size, scope_name=None, stddev=0.02, bias_start=0.0, with_w=False, reuse=None)
     concat(tensors, axis)
 plus what the model files take from TensorFlow directly (relu, tanh, sigmoid, reflect pad, the
-losses) and `instance_norm`, which the reference does not have.
+losses) and `instance_norm`, which the reference does not have.  Further extensions, in fp32, bf16 or fp16:
+    rms_norm(x, name="rms_norm", epsilon=1e-6, residual=None, mx=False)
+    linear_mx(input_, output_size, ...) / mx_matmul(x, w, bias=None) / mx_pack / mx_quantize / mx_dequantize
+    distill_topk_mean(logits, teacher_logits, teacher_index, temperature=1.0, ...)
 
-Tensors are dense fp32 NHWC torch tensors in GPU memory.  torch.autograd only sequences the
+Tensors are dense fp32 NHWC torch tensors in GPU memory unless a function says otherwise.  torch.autograd only sequences the
 backward; every forward and backward computation is a call into the HIP library.  Weight
 gradients are not returned through autograd: the backward of each layer writes them straight into
 the owning optimiser group's gradient arena when that variable is being trained in the current
@@ -797,6 +800,322 @@ def instance_norm(x, name="instance_norm", epsilon=1e-5, act=None, act_param=0.2
 
 
 # --------------------------------------------------------------------------------------------
+# root-mean-square norm (extension): fp32 / bf16 / fp16, with the residual's addition and an 8-bit output
+# --------------------------------------------------------------------------------------------
+def _rows_of(t):
+    """(tensor, rows, columns, row stride) of t seen as rows along its last axis: a rank-2 view with its columns side by side
+    is taken as it is, everything else made dense."""
+    c = t.shape[-1]
+    if t.dim() == 2 and t.shape[0] > 1 and t.stride(1) == 1 and t.stride(0) >= c:
+        return t, t.shape[0], c, t.stride(0)
+    t = t.contiguous()
+    return t, t.numel() // c if c else 0, c, c
+
+
+def _dense16(t):
+    """t dense and on a 16-byte border."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() & 15 else t
+
+
+def _rms_fwd(x, residual, gamma, eps, mx, want_rstd):
+    """(y or MxTensor, h or None, rstd or None, the stream's tensor and row stride)"""
+    code = _lib.dtype_code(x.dtype)
+    _lib.here(x, residual, gamma.data)
+    xs, rows, c, ldx = _rows_of(x)
+    rs, ldr, h = None, 0, None
+    if residual is not None:
+        rs, _, _, ldr = _rows_of(residual)
+        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if want_rstd else None
+    out = _mx_empty(x.shape, 'e4m3', x.dtype, x.device) if mx else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    check(lib.gan_rms_norm_fwd(code, rows, c, xs.data_ptr(), ldx, None if rs is None else rs.data_ptr(), ldr, ptr(gamma.data), eps,
+                               None if h is None else h.data_ptr(), None if mx else out.data_ptr(),
+                               out.codes.data_ptr() if mx else None, out.scales.data_ptr() if mx else None, ptr(rstd), stream()))
+    return out, h, rstd, ((xs, ldx) if h is None else (h, c))
+
+
+class _RmsNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, token, gamma, eps, mx, made):
+        ctx.set_materialize_grads(False)
+        out, h, rstd, (kept, ctx.ld) = _rms_fwd(x, residual, gamma, eps, mx, True)
+        ctx.save_for_backward(kept, rstd)
+        ctx.gamma = gamma
+        if mx:      # autograd sees a stand-in of the norm's shape and type; the codes go around it
+            made.append(out)
+            out = torch.empty(1, dtype=x.dtype, device=x.device).expand(x.shape)
+        return out if h is None else (out, h)
+
+    @staticmethod
+    def backward(ctx, dy, dh=None):
+        kept, rstd = ctx.saved_tensors
+        gamma = ctx.gamma
+        want = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+        if dy is None:                      # only the stream itself was used
+            dx = dh if want else None
+        else:
+            _lib.here(dy, dh, kept)
+            c = kept.shape[-1]
+            rows = rstd.numel()
+            dy = dy.contiguous()
+            dh = None if dh is None or not want else dh.contiguous()
+            dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device) if want else None
+            dg, acc, wp, wn, hold = None, 0, None, 0, None
+            if gamma.wants_grad:
+                dg, acc = gamma.grad_target()
+                wp, wn, hold = _lib.scratch(lib.gan_rms_norm_workspace_bytes(rows, c), dy.device)
+            if dx is not None or dg is not None:
+                check(lib.gan_rms_norm_bwd(_lib.dtype_code(dy.dtype), rows, c, kept.data_ptr(), ctx.ld, ptr(gamma.data), ptr(rstd),
+                                           dy.data_ptr(), None if dh is None else dh.data_ptr(),
+                                           None if dx is None else dx.data_ptr(), ptr(dg), acc, wp, wn, stream()))
+        return (dx if ctx.needs_input_grad[0] else None, dx if ctx.needs_input_grad[1] else None) + (None,) * 5
+
+
+def rms_norm(x, name="rms_norm", epsilon=1e-6, residual=None, mx=False):
+    """Extension: y = h / sqrt(mean(h^2) + epsilon) * gamma over the last axis, h = x + residual rounded to x's type; gamma
+    (fp32, ones at first) is created under the caller's scope + name.  x and residual: fp32, bf16 or fp16, one shape and
+    type, up to 32768 values on the last axis.
+
+    Returns y, or (y, h) with a residual: h is the next residual.  mx=True returns y as an e4m3 `MxTensor`, the form
+    `linear_mx` and `mx_matmul` multiply; gradients pass straight through its rounding."""
+    st = V.default_store()
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("rms_norm: nothing to normalise in shape %s" % (tuple(x.shape),))
+    _lib.dtype_code(x.dtype)
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError("rms_norm: residual %s %s does not match x %s %s" % (tuple(residual.shape), residual.dtype, tuple(x.shape), x.dtype))
+    with st.variable_scope(name):
+        gamma = st.get_variable('gamma', [x.shape[-1]], V.constant_initializer(1.0))
+    eps, mx = float(epsilon), bool(mx)
+    token = _grad_token(x.device, gamma) if torch.is_grad_enabled() else None
+    if token is None and not (torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad))):
+        out, h, _, _ = _rms_fwd(x, residual, gamma, eps, mx, False)
+        return out if h is None else (out, h)
+    made = []
+    out = _RmsNormFn.apply(x, residual, token, gamma, eps, mx, made)
+    y, h = out if residual is not None else (out, None)
+    if mx:
+        made[0].ticket = y
+        y = made[0]
+    return y if h is None else (y, h)
+
+
+# --------------------------------------------------------------------------------------------
+# microscaled values and products (extension)
+# --------------------------------------------------------------------------------------------
+def _mx_groups(c):
+    return (c + 127) // 128
+
+
+class MxTensor(object):
+    """Rows of microscaled values: blocks of 32 along the last axis with one power-of-two scale each, filled up with zeros to
+    whole groups of 128.
+        codes   e4m3: float8_e4m3fn [..., groups * 128]; e2m1: uint8 [..., groups * 64], two values a byte, the first in the low half
+        scales  float8_e8m0fnu [..., groups * 4]
+        width   values of a row; fmt 'e4m3' or 'e2m1'; dtype: type of what was quantised, and of a product's result
+    """
+    __slots__ = ('codes', 'scales', 'width', 'fmt', 'dtype', 'ticket')
+
+    def __init__(self, codes, scales, width, fmt='e4m3', dtype=torch.float32):
+        if fmt not in _lib.MX_FORMATS:
+            raise ValueError("MxTensor: unknown format %r (e4m3 or e2m1)" % (fmt,))
+        _lib.dtype_code(dtype)
+        g = _mx_groups(int(width))
+        if width < 1 or codes.element_size() != 1 or scales.element_size() != 1 or codes.dim() < 1 or \
+                codes.shape[-1] != g * (128 if fmt == 'e4m3' else 64) or \
+                tuple(scales.shape) != tuple(codes.shape[:-1]) + (g * 4,):
+            raise ValueError("MxTensor: codes %s %s / scales %s %s do not hold rows of %d %s values"
+                             % (tuple(codes.shape), codes.dtype, tuple(scales.shape), scales.dtype, width, fmt))
+        if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() & 15 or scales.data_ptr() & 3:
+            raise ValueError("MxTensor: codes and scales have to be dense, on 16- and 4-byte borders")
+        self.codes = codes.view(torch.float8_e4m3fn if fmt == 'e4m3' else torch.uint8)
+        self.scales = scales.view(torch.float8_e8m0fnu)
+        self.width, self.fmt, self.dtype, self.ticket = int(width), fmt, dtype, None
+
+    @property
+    def shape(self):
+        return self.codes.shape[:-1] + (self.width,)
+
+    def __repr__(self):
+        return "MxTensor(%s, %s, of %s)" % (tuple(self.shape), self.fmt, self.dtype)
+
+
+class MxMatrix(object):
+    """A weight matrix [in_dim, out_dim] in packed e2m1: codes uint8 [groups * 4, out_dim, 16] (a block of 32 inputs of one output
+    is 16 bytes), scales uint8 [groups, out_dim, 4]; groups of 128 inputs, filled up with zeros.  `mx_pack` makes one."""
+    __slots__ = ('codes', 'scales', 'in_dim', 'out_dim')
+
+    def __init__(self, codes, scales, in_dim, out_dim):
+        g = _mx_groups(int(in_dim))
+        if in_dim < 1 or out_dim < 1 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or \
+                tuple(codes.shape) != (g * 4, out_dim, 16) or tuple(scales.shape) != (g, out_dim, 4):
+            raise ValueError("MxMatrix: codes %s %s / scales %s %s do not hold a %d x %d matrix"
+                             % (tuple(codes.shape), codes.dtype, tuple(scales.shape), scales.dtype, in_dim, out_dim))
+        if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() & 15 or scales.data_ptr() & 3:
+            raise ValueError("MxMatrix: codes and scales have to be dense, on 16- and 4-byte borders")
+        self.codes, self.scales, self.in_dim, self.out_dim = codes, scales, int(in_dim), int(out_dim)
+
+    @property
+    def shape(self):
+        return (self.in_dim, self.out_dim)
+
+    def __repr__(self):
+        return "MxMatrix(%d x %d)" % (self.in_dim, self.out_dim)
+
+
+def _mx_empty(shape, fmt, dtype, device):
+    """An MxTensor to be filled by the library."""
+    g = _mx_groups(shape[-1])
+    q = MxTensor.__new__(MxTensor)
+    if fmt == 'e4m3':
+        q.codes = torch.empty(tuple(shape[:-1]) + (g * 128,), dtype=torch.float8_e4m3fn, device=device)
+    else:
+        q.codes = torch.empty(tuple(shape[:-1]) + (g * 64,), dtype=torch.uint8, device=device)
+    q.scales = torch.empty(tuple(shape[:-1]) + (g * 4,), dtype=torch.float8_e8m0fnu, device=device)
+    q.width, q.fmt, q.dtype, q.ticket = shape[-1], fmt, dtype, None
+    return q
+
+
+def mx_quantize(x, fmt='e4m3'):
+    """x (fp32, bf16 or fp16) as an `MxTensor` in blocks of 32 along its last axis (include/gan_hip.h has the rounding rule)."""
+    if fmt not in _lib.MX_FORMATS:
+        raise ValueError("mx_quantize: unknown format %r (e4m3 or e2m1)" % (fmt,))
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("mx_quantize: nothing to quantise in shape %s" % (tuple(x.shape),))
+    code = _lib.dtype_code(x.dtype)
+    _lib.here(x)
+    xs, rows, c, ld = _rows_of(x.detach())
+    q = _mx_empty(x.shape, fmt, x.dtype, x.device)
+    check(lib.gan_mx_quantize(code, _lib.MX_FORMATS[fmt], rows, c, xs.data_ptr(), ld, q.codes.data_ptr(), q.scales.data_ptr(), stream()))
+    return q
+
+
+def mx_pack(matrix):
+    """A weight matrix [in_dim, out_dim] (fp32, bf16 or fp16; `linear`'s Matrix) quantised to e2m1 in blocks of 32 inputs, in the
+    layout the products read.  A serving program packs its weights once and keeps the `MxMatrix`."""
+    if matrix.dim() != 2 or matrix.shape[0] < 1 or matrix.shape[1] < 1:
+        raise ValueError("mx_pack expects a rank-2 matrix, got shape %s" % (tuple(matrix.shape),))
+    code = _lib.dtype_code(matrix.dtype)
+    _lib.here(matrix)
+    m, k, n, ld = _rows_of(matrix.detach())
+    g = _mx_groups(k)
+    codes = torch.empty((g * 4, n, 16), dtype=torch.uint8, device=m.device)
+    scales = torch.empty((g, n, 4), dtype=torch.uint8, device=m.device)
+    check(lib.gan_mx_pack(code, k, n, m.data_ptr(), ld, codes.data_ptr(), scales.data_ptr(), stream()))
+    return MxMatrix(codes, scales, k, n)
+
+
+def mx_dequantize(q, dtype=None):
+    """The values an `MxTensor` (in its own type unless `dtype` is given) or an `MxMatrix` (fp32) stands for, dense."""
+    if isinstance(q, MxMatrix):
+        dtype = torch.float32 if dtype is None else dtype
+        code = _lib.dtype_code(dtype)
+        _lib.here(q.codes, q.scales)
+        out = torch.empty(q.shape, dtype=dtype, device=q.codes.device)
+        check(lib.gan_mx_unpack(code, q.in_dim, q.out_dim, q.codes.data_ptr(), q.scales.data_ptr(), out.data_ptr(), stream()))
+        return out
+    dtype = q.dtype if dtype is None else dtype
+    code = _lib.dtype_code(dtype)
+    _lib.here(q.codes, q.scales)
+    out = torch.empty(tuple(q.shape), dtype=dtype, device=q.codes.device)
+    check(lib.gan_mx_dequantize(code, _lib.MX_FORMATS[q.fmt], out.numel() // q.width, q.width, q.codes.data_ptr(), q.scales.data_ptr(),
+                                out.data_ptr(), stream()))
+    return out
+
+
+def _mx_product(q, w, bias):
+    """q W + bias in q's type."""
+    _lib.here(q.codes, q.scales, w.codes, w.scales, bias)
+    code, fmt = _lib.DTYPES[q.dtype], _lib.MX_FORMATS[q.fmt]
+    lead = tuple(q.codes.shape[:-1])
+    y = torch.empty(lead + (w.out_dim,), dtype=q.dtype, device=q.codes.device)
+    rows = y.numel() // w.out_dim
+    wp, wn, hold = _lib.scratch(lib.gan_mx_matmul_workspace_bytes(code, fmt, rows, w.in_dim, w.out_dim), y.device)
+    check(lib.gan_mx_matmul(code, fmt, rows, w.in_dim, w.out_dim, q.codes.data_ptr(), q.scales.data_ptr(), w.codes.data_ptr(),
+                            w.scales.data_ptr(), ptr(bias), y.data_ptr(), wp, wn, stream()))
+    return y
+
+
+class _MxMatmulFn(torch.autograd.Function):
+    """x: what carries the gradient -- the float input, or the stand-in of an MxTensor.  matrix / bias_var: the variables behind
+    the packed weights (None: frozen)."""
+
+    @staticmethod
+    def forward(ctx, x, token, q, w, bias, matrix, bias_var, fmt):
+        q = mx_quantize(x, fmt) if q is None else q
+        y = _mx_product(q, w, bias)
+        ctx.save_for_backward(q.codes, q.scales, w.codes, w.scales)
+        ctx.q, ctx.w = (q.fmt, q.width), (w.in_dim, w.out_dim)
+        ctx.matrix, ctx.bias = matrix, bias_var
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        ac, asc, wc, wsc = ctx.saved_tensors
+        in_dim, out_dim = ctx.w
+        dy = _dense16(dy)
+        _lib.here(dy, ac)
+        code, rows = _lib.dtype_code(dy.dtype), dy.numel() // out_dim
+        if ctx.matrix is not None and ctx.matrix.wants_grad and rows:
+            dm, acc = ctx.matrix.grad_target()
+            db, accb = ctx.bias.grad_target()
+            assert acc == accb
+            wp, wn, hold = _lib.scratch(lib.gan_mx_matmul_wgrad_workspace_bytes(code, rows, in_dim, out_dim), dy.device)
+            check(lib.gan_mx_matmul_wgrad(code, _lib.MX_FORMATS[ctx.q[0]], rows, in_dim, out_dim, ac.data_ptr(), asc.data_ptr(),
+                                          dy.data_ptr(), ptr(dm), ptr(db), acc, wp, wn, stream()))
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dx = torch.empty(tuple(dy.shape[:-1]) + (in_dim,), dtype=dy.dtype, device=dy.device)
+            wp, wn, hold = _lib.scratch(lib.gan_mx_matmul_dgrad_workspace_bytes(code, rows, in_dim, out_dim), dy.device)
+            check(lib.gan_mx_matmul_dgrad(code, rows, in_dim, out_dim, dy.data_ptr(), wc.data_ptr(), wsc.data_ptr(), dx.data_ptr(),
+                                          wp, wn, stream()))
+        return (dx,) + (None,) * 7
+
+
+def _mx_apply(x, w, bias, fmt, token=None, matrix=None, bias_var=None):
+    if isinstance(x, MxTensor):
+        q, carrier, width = x, x.ticket, x.width
+    else:
+        if fmt not in _lib.MX_FORMATS:
+            raise ValueError("unknown microscaled format %r (e4m3 or e2m1)" % (fmt,))
+        q, carrier, width = None, x, x.shape[-1] if x.dim() else 0
+        _lib.dtype_code(x.dtype)
+    if width != w.in_dim:
+        raise ValueError("microscaled product: rows of %d values against a %d x %d matrix" % (width, w.in_dim, w.out_dim))
+    if bias is not None and (tuple(bias.shape) != (w.out_dim,) or bias.dtype != torch.float32):
+        raise ValueError("microscaled product: bias %s %s for %d outputs" % (tuple(bias.shape), bias.dtype, w.out_dim))
+    if torch.is_grad_enabled() and (token is not None or (carrier is not None and carrier.requires_grad)):
+        return _MxMatmulFn.apply(carrier, token, q, w, bias, matrix, bias_var, fmt)
+    return _mx_product(mx_quantize(x, fmt) if q is None else q, w, bias)
+
+
+def mx_matmul(x, w, bias=None, fmt='e4m3'):
+    """Extension: x W + bias with packed 4-bit weights (`mx_pack`) and microscaled activations; sums are fp32, the result has x's
+    type.  x: fp32, bf16 or fp16 [..., in_dim], quantised to `fmt` ('e4m3' or 'e2m1') on the way, or an `MxTensor` (its own
+    format counts).  bias: fp32 [out_dim].  The weights are frozen here: the backward pass gives x its gradient, straight
+    through the rounding of x."""
+    return _mx_apply(x, w, bias, fmt)
+
+
+def linear_mx(input_, output_size, scope_name=None, stddev=0.02, bias_start=0.0, with_w=False, reuse=None, *, fmt='e4m3'):
+    """`linear` (the same variables: Matrix [in,out] and bias, fp32) multiplied in 4 bits: Matrix is quantised to e2m1 in every call,
+    the input -- fp32, bf16, fp16 or an `MxTensor` of any rank -- to `fmt`.  Gradients are those of the product of the quantised
+    values, passed straight through both quantisers."""
+    st = V.default_store()
+    width = int(input_.shape[-1])
+    with st.variable_scope(scope_name or "Linear", reuse=reuse):
+        matrix = st.get_variable("Matrix", [width, output_size], V.random_normal_initializer(stddev))
+        bias = st.get_variable("bias", [output_size], V.constant_initializer(bias_start))
+    device = input_.codes.device if isinstance(input_, MxTensor) else input_.device
+    token = _grad_token(device, matrix) if torch.is_grad_enabled() else None
+    y = _mx_apply(input_, mx_pack(matrix.data), bias.data, fmt, token, matrix, bias)
+    if with_w:
+        return y, matrix, bias
+    return y
+
+
+# --------------------------------------------------------------------------------------------
 # activations, add, concat, reflect pad
 # --------------------------------------------------------------------------------------------
 class _ActFn(torch.autograd.Function):
@@ -1062,6 +1381,57 @@ def l1_mean(a, b, weight=1.0):
     if a.shape != b.shape:
         raise ValueError("l1_mean: shapes %s and %s differ" % (tuple(a.shape), tuple(b.shape)))
     return _LossFn.apply('l1', a, b, 0.0, float(weight))
+
+
+class _DistillFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, teacher, index, lse, row_weight, tau, weight):
+        _lib.here(logits, teacher, index, lse, row_weight)
+        x, rows, classes, ld = _rows_of(logits)
+        dev = x.device
+        loss = torch.empty(1, dtype=torch.float32, device=dev)
+        grad = torch.empty(logits.shape, dtype=x.dtype, device=dev) if ctx.needs_input_grad[0] else None
+        wp, wn, hold = _lib.scratch(lib.gan_distill_topk_workspace_bytes(rows), dev)
+        check(lib.gan_distill_topk_mean(_lib.dtype_code(x.dtype), rows, classes, x.data_ptr(), ld, _lib.dtype_code(teacher.dtype),
+                                        teacher.data_ptr(), index.data_ptr(), index.element_size(), teacher.shape[-1], ptr(lse),
+                                        ptr(row_weight), tau, weight, 0, ptr(loss), None if grad is None else grad.data_ptr(), wp, wn,
+                                        stream()))
+        ctx.grad = grad
+        return loss
+
+    @staticmethod
+    def backward(ctx, _one):
+        return (ctx.grad,) + (None,) * 6
+
+
+def distill_topk_mean(logits, teacher_logits, teacher_index, temperature=1.0, weight=1.0, row_weight=None, teacher_lse=None):
+    """Extension: mean divergence of the student's softmax from a teacher known by its top logits, times weight * temperature^2;
+    a root for `backward` like the losses above.
+
+    logits [..., classes] (fp32, bf16, fp16); teacher_logits (any of the three types) and teacher_index (int32 / int64) [..., top]:
+    the teacher's highest logits and their classes, in any order.  Entries with an index outside [0, classes) (-1 fills a short
+    list) or a logit of -inf are left out.  Without teacher_lse the list is taken for the whole distribution; with it (fp32
+    [...], log-sum-exp of ALL the teacher's logits / temperature) the mass that is not listed is one more class, held against
+    the student's whole mass outside the list.
+    row_weight (fp32 [...]): the mean is sum(w l) / sum(w).  Rows of weight 0 and rows with an empty list have loss and gradient 0."""
+    lead = tuple(logits.shape[:-1])
+    if logits.dim() < 1 or logits.numel() == 0:
+        raise ValueError("distill_topk_mean: no logits in shape %s" % (tuple(logits.shape),))
+    _lib.dtype_code(logits.dtype)
+    _lib.dtype_code(teacher_logits.dtype)
+    if teacher_logits.shape != teacher_index.shape or tuple(teacher_logits.shape[:-1]) != lead or teacher_logits.dim() != logits.dim():
+        raise ValueError("distill_topk_mean: logits %s, teacher logits %s and indices %s do not go together"
+                         % (tuple(logits.shape), tuple(teacher_logits.shape), tuple(teacher_index.shape)))
+    if teacher_index.dtype not in (torch.int32, torch.int64):
+        raise TypeError("distill_topk_mean: indices have to be int32 or int64, got %s" % teacher_index.dtype)
+    for what, t in (("row_weight", row_weight), ("teacher_lse", teacher_lse)):
+        if t is not None and (tuple(t.shape) != lead or t.dtype != torch.float32):
+            raise ValueError("distill_topk_mean: %s %s %s for rows %s (float32 expected)" % (what, tuple(t.shape), t.dtype, lead))
+    if not 0.0 < float(temperature) < float('inf'):
+        raise ValueError("distill_topk_mean: temperature %r" % (temperature,))
+    dense = lambda t: None if t is None else t.detach().contiguous()
+    return _DistillFn.apply(logits, dense(teacher_logits), dense(teacher_index), dense(teacher_lse), dense(row_weight),
+                            float(temperature), float(weight))
 
 
 _ones = {}

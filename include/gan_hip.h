@@ -7,7 +7,8 @@
  * cited as the reference call site (file:line under the reference root).
  *
  * Conventions
- *   - All tensors are dense fp32, NHWC, in device memory owned by the caller.
+ *   - All tensors are dense fp32, NHWC, in device memory owned by the caller (the
+ *     entry points that take a `dtype` say what theirs are).
  *   - The library never allocates or frees device memory and never
  *     synchronises; every launch is asynchronous on the caller's stream.
  *   - `ws` is a caller-provided scratch buffer of at least the number of bytes
@@ -317,6 +318,82 @@ int gan_l1_mean(const float* a, const float* b, long n, float weight, int accumu
 size_t gan_l1_mean_workspace_bytes(long n);
 int gan_l1_mean_ws(const float* a, const float* b, long n, float weight, int accumulate,
                    float* loss_out, float* db, void* ws, size_t ws_bytes, gan_stream_t stream);
+
+/* ---- element types and microscaled formats of the entry points below (the tensors of all others are fp32) --------------- */
+enum { GAN_F32 = 0, GAN_BF16 = 1, GAN_F16 = 2 };
+/* A microscaled row holds blocks of 32 values that share one power-of-two scale, filled up with zeros to whole groups of 128:
+ *   codes   e4m3: one byte a value (OCP fp8, largest 448), [rows][groups * 128]
+ *           e2m1: two values a byte (0 .5 1 1.5 2 3 4 6 and a sign; the first in the low half), [rows][groups * 64]
+ *   scales  one byte e + 127 a block, [rows][groups * 4]
+ * e is the smallest integer in [-126, 127] with max |x| <= largest * 2^e (so no element saturates), codes are rounded to
+ * nearest even; a block that holds an infinity or a NaN has scale byte 255 and stands for NaN throughout.
+ * A packed weight matrix [in][out] is e2m1 in blocks along `in`: codes [groups * 4][out][16], scales [groups][out][4], groups of
+ * 128 inputs.  Magnitudes within a rounding step of the largest float may stand for infinity. */
+enum { GAN_MX_E4M3 = 0, GAN_MX_E2M1 = 1 };
+#define GAN_MX_MAX_IN (1 << 22)   /* longest contraction served */
+#define GAN_MX_MAX_ROWS (1 << 22)
+
+/* ---- root-mean-square norm with the residual's addition (extension: the reference norms with batch_norm only, ops.py:30-44)
+ *   h = T(x + residual), s = 1 / sqrt(mean(h^2) + eps) over the c values of a row, y = h s gamma
+ * x and residual have row strides ldx, ldr (in values); h and y are dense, all of type dtype; gamma fp32.  h is written exactly
+ * when a residual is given.  Output either y, or mx_codes / mx_scales: y in e4m3 (the product's operand; y is then computed
+ * in 64 bits, and nothing is stored in T).  rstd (fp32 [rows], may be NULL) receives s for the backward.  c <= 32768.
+ * Backward, from the stored stream h (x itself without a residual), with g = dy gamma, n = h s:
+ *   dx = s (g - n mean(g n)) + dh      dgamma (+)= sum over rows of dy n
+ * dh (the gradient that reaches h from elsewhere), dx and dgamma may be NULL. */
+int gan_rms_norm_fwd(int dtype, long rows, int c, const void* x, long ldx, const void* residual, long ldr,
+                     const float* gamma, float eps, void* h, void* y, void* mx_codes, void* mx_scales, float* rstd,
+                     gan_stream_t stream);
+size_t gan_rms_norm_workspace_bytes(long rows, int c);
+int gan_rms_norm_bwd(int dtype, long rows, int c, const void* h, long ldh, const float* gamma, const float* rstd,
+                     const void* dy, const void* dh, void* dx, float* dgamma, int accumulate, void* ws,
+                     size_t ws_bytes, gan_stream_t stream);
+
+/* ---- microscaled quantisation (extension) ------------------------------------------------------------------------------
+ * rows: [rows][c] of type dtype (row stride ldx) <-> microscaled rows; pack / unpack: a matrix [in][out] (row stride ld)
+ * <-> packed weights. */
+int gan_mx_quantize(int dtype, int fmt, long rows, int c, const void* x, long ldx, void* codes, void* scales,
+                    gan_stream_t stream);
+int gan_mx_dequantize(int dtype, int fmt, long rows, int c, const void* codes, const void* scales, void* y,
+                      gan_stream_t stream);
+int gan_mx_pack(int dtype, int in_dim, int out_dim, const void* matrix, long ld, void* codes, void* scales,
+                gan_stream_t stream);
+int gan_mx_unpack(int dtype, int in_dim, int out_dim, const void* codes, const void* scales, void* matrix,
+                  gan_stream_t stream);
+
+/* ---- product of microscaled rows with packed 4-bit weights (extension of tf.matmul + bias, ops.py:113-115) --------------
+ *   y[r][n] = sum_k A[r][k] W[k][n] + bias[n], fp32 accumulation, y dense of type dtype; bias fp32, may be NULL.
+ * Gradients, with the quantised values A and W (straight through the quantisers), dY dense of type dtype:
+ *   dx[r][k] = sum_n dY[r][n] W[k][n] (type dtype)   dmatrix[k][n] (+)= sum_r A[r][k] dY[r][n]   dbias[n] (+)= sum_r dY[r][n]
+ * (fp32; dbias may be NULL).  Their sums carry fp32-level error for every dtype. */
+size_t gan_mx_matmul_workspace_bytes(int dtype, int fmt, int rows, int in_dim, int out_dim);
+int gan_mx_matmul(int dtype, int fmt, int rows, int in_dim, int out_dim, const void* a_codes, const void* a_scales,
+                  const void* w_codes, const void* w_scales, const float* bias, void* y, void* ws, size_t ws_bytes,
+                  gan_stream_t stream);
+size_t gan_mx_matmul_dgrad_workspace_bytes(int dtype, int rows, int in_dim, int out_dim);
+int gan_mx_matmul_dgrad(int dtype, int rows, int in_dim, int out_dim, const void* dy, const void* w_codes,
+                        const void* w_scales, void* dx, void* ws, size_t ws_bytes, gan_stream_t stream);
+size_t gan_mx_matmul_wgrad_workspace_bytes(int dtype, int rows, int in_dim, int out_dim);
+int gan_mx_matmul_wgrad(int dtype, int fmt, int rows, int in_dim, int out_dim, const void* a_codes,
+                        const void* a_scales, const void* dy, float* dmatrix, float* dbias, int accumulate, void* ws,
+                        size_t ws_bytes, gan_stream_t stream);
+
+/* ---- distillation from a teacher's top logits, fused with its gradient (extension; conventions of the losses above) ------
+ * logits [rows][classes] of type dtype, row stride ld; teacher and index [rows][top], dense, index int32 or int64 by
+ * index_bytes.  List entries with a class outside [0, classes) or a teacher logit of -inf are left out; a class listed twice
+ * counts with both probabilities.  With z = logits / temperature, t = teacher / temperature, q = softmax z:
+ *   p = softmax of t over the list (teacher_lse NULL), or exp(t - teacher_lse[row]) with p_r = max(0, 1 - sum p) left for all
+ *   other classes together (teacher_lse: the log-sum-exp of all the teacher's logits / temperature)
+ *   l = sum_i p_i (log p_i - log q_i) [+ p_r (log p_r - log q_r)], the last term where p_r > 0 and some other class has q > 0
+ *   loss_out[0] = (accumulate ? loss_out[0] : 0) + weight temperature^2 sum_r w_r l_r / sum_r w_r
+ * dlogits (dense, type dtype, may be NULL) = its gradient.  row_weight NULL: all 1.  A row of weight 0 or without a list entry
+ * has loss 0 and gradient 0 whatever its logits hold; weights that add up to 0 give loss 0 and gradient 0.
+ * classes <= 2^20, top <= 1024. */
+size_t gan_distill_topk_workspace_bytes(long rows);
+int gan_distill_topk_mean(int dtype, long rows, int classes, const void* logits, long ld, int teacher_dtype,
+                          const void* teacher, const void* index, int index_bytes, int top, const float* teacher_lse,
+                          const float* row_weight, float temperature, float weight, int accumulate, float* loss_out,
+                          void* dlogits, void* ws, size_t ws_bytes, gan_stream_t stream);
 
 /* ---- tf.train.AdamOptimizer(lr, beta1).minimize (dcgan.py:154-157) ----------------------
  * One fused step over a flat parameter group.  step_dev[0] (device int32) holds the number of
