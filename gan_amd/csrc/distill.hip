@@ -7,11 +7,12 @@
 //   dl/dz_j = P q_j - p_j (listed), P q_j - p_r q_j / q_r (others), P = sum p + p_r
 //
 // Memory-bound: the logits are read once, held in registers, and their gradient is written once.  One workgroup a row, its
-// threads hold the row in 16-byte chunks of the tensor's type; the maximum and the sum of exponentials come from one pass over
-// the registers (a thread rescales nothing: it takes its own maximum first), joined over the workgroup in one exchange.
+// threads hold the row in 16-byte chunks of the tensor's type; maximum and sum of exponentials come from two passes over the
+// registers, joined over the workgroup in one exchange; a third pass writes the gradient.
 // q_r is never 1 - sum q_i, which cancels: a bit per class marks the list, and sums over the marked and the unmarked classes
-// are taken apart.  The same bits tell whether a class is listed twice, in which case its probabilities add up.
-// Statistics are fp32 with natural order fixed by the thread number, so results are deterministic.
+// are taken apart.  The same bits tell whether a class is listed twice (its probabilities add up), and which values the chunks
+// leave to the first wave, which writes the listed classes: nobody waits for another's stores.
+// Statistics are fp32 in an order fixed by the thread number, so results are deterministic.
 #include "mx.h"
 
 namespace gan {
@@ -47,14 +48,49 @@ __device__ __forceinline__ float wave_all_max(float v) {
     return v;
 }
 
-// exp(x - m) with -inf as the maximum of nothing: exp(-inf - -inf) is 0 here
-__device__ __forceinline__ float exp_from(float x, float m) { return __expf(x - (m == -INFINITY ? 0.f : m)); }
+// e^((x - m) / tau) as 2^((x - m) c2), c2 = log2(e) / tau, with -inf as the maximum of nothing: of -inf and -inf it is 0 here.
+// Maxima stay in the logits' own units: a mask of the type's lowest value times log2(e) would be an infinity.
+__device__ __forceinline__ float power(float x, float m, float c2) {
+    return __builtin_amdgcn_exp2f((x - (m == -INFINITY ? 0.f : m)) * c2);
+}
 
-// Maximum and sum of exponentials, joined: (m, s) <- (max(m, m2), s e^(m - max) + s2 e^(m2 - max)).
-__device__ __forceinline__ void join_stats(float& m, float& s, float m2, float s2) {
+// Maximum and sum of powers, joined: (m, s) <- (max(m, m2), s e^((m - max) / tau) + s2 e^((m2 - max) / tau)).
+__device__ __forceinline__ void join_stats(float& m, float& s, float m2, float s2, float c2) {
     const float mm = fmaxf(m, m2);
-    s = s * exp_from(m, mm) + s2 * exp_from(m2, mm);
+    s = s * power(m, mm, c2) + s2 * power(m2, mm, c2);
     m = mm;
+}
+
+// 16 bytes of a row.
+template <typename T> struct Chunk {
+    static constexpr int n = 16 / sizeof(T);
+};
+__device__ __forceinline__ void unpack(const i32x4& r, float (&v)[4], float) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __int_as_float(r[j]);
+}
+__device__ __forceinline__ void unpack(const i32x4& r, float (&v)[8], bf16_t) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        v[2 * j] = __int_as_float(r[j] << 16);
+        v[2 * j + 1] = __int_as_float(r[j] & 0xffff0000);
+    }
+}
+__device__ __forceinline__ void unpack(const i32x4& r, float (&v)[8], f16_t) {
+    const f16x8 h = __builtin_bit_cast(f16x8, r);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (float)h[j];
+}
+// -inf in the places `marked` names
+template <typename T>
+__device__ __forceinline__ void strike(i32x4& r, unsigned marked) {
+    constexpr int n = Chunk<T>::n;
+#pragma unroll
+    for (int j = 0; j < n; ++j) {
+        if (!(marked >> j & 1)) continue;
+        if (n == 4) r[j] = 0xff800000;
+        else r[j / 2] = (r[j / 2] & (j & 1 ? 0x0000ffff : 0xffff0000)) | (std::is_same<T, bf16_t>::value ? 0xff80u : 0xfc00u) << (16 * (j & 1));
+    }
 }
 
 template <int NT>
@@ -68,76 +104,54 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
     return v;
 }
 
-// NV chunks of eight values a thread in registers; NV = 0: the row does not fit and is read twice.
+// NV chunks a thread in registers; NV = 0: the row does not fit and is read twice.
 template <typename T, int NT, int NV, bool REST>
 __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
+    constexpr int N = Chunk<T>::n;
     extern __shared__ __align__(16) unsigned char lds[];
     __shared__ float red[2 * NT / 64];
-    __shared__ float told[6];       // statistics of the list: any, P, p_r, maximum, sum of exponentials; repeated classes
+    // of the list: any, P, p_r, maximum, sum of powers, repeated classes; sum of the weights
+    __shared__ float told[7];
     const int tid = threadIdx.x, lane = tid & 63, classes = p.classes;
     const long row = blockIdx.x;
     const T* x = static_cast<const T*>(p.logits) + row * p.ld;
     T* gr = static_cast<T*>(p.grad) + (p.grad ? row * classes : 0);
-    // chunks start at 16-byte borders: chunk c holds the classes 8 c - a .. 8 c - a + 7
-    const int a = (int)((reinterpret_cast<size_t>(x) & 15) / sizeof(T));
-    const bool gvec = (reinterpret_cast<size_t>(gr) & 15) == (reinterpret_cast<size_t>(x) & 15);
-    const int chunks = (classes + a + 7) / 8;
-    unsigned* bits = reinterpret_cast<unsigned*>(lds);      // bit 8 c + j: class j of chunk c is listed
-    const int words = (chunks + 3) / 4;
-    int* l_id = reinterpret_cast<int*>(lds + ((words + 3) / 4) * 16);
+    // the row: up to N - 1 values before its first 16-byte border, whole chunks, up to N - 1 values behind them; of the loose
+    // values a thread has at most one
+    const int head = min(classes, (int)((16 - (reinterpret_cast<size_t>(x) & 15)) & 15) / (int)sizeof(T));
+    const int chunks = (classes - head) / N, tail = head + chunks * N;
+    const bool gvec = ((reinterpret_cast<size_t>(gr) ^ reinterpret_cast<size_t>(x)) & 15) == 0;
+    const int loose = tid < head ? tid : tid >= 8 && tail + tid - 8 < classes && tid < 16 ? tail + tid - 8 : -1;
+    unsigned* bits = reinterpret_cast<unsigned*>(lds);      // bit e - head + 8: class e is listed
+    const int words = (classes + 8 + 127) / 128 * 4;
+    int* l_id = reinterpret_cast<int*>(bits + words);
     float* l_p = reinterpret_cast<float*>(l_id + p.top);
     float* l_lp = l_p + p.top;
     float* l_z = l_lp + p.top;
-
-    typedef typename Vec8<T>::type Raw;
-    auto load = [&](int chunk) -> Raw {
-        const int e0 = chunk * 8 - a;
-        if (e0 >= 0 && e0 + 8 <= classes) return *reinterpret_cast<const Raw*>(x + e0);
-        Raw r;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) r[j] = e0 + j >= 0 && e0 + j < classes ? x[e0 + j] : (T)-INFINITY;
-        return r;
+    auto marks = [&](int chunk) -> unsigned {
+        const int at = chunk * N + 8;
+        return bits[at >> 5] >> (at & 31) & ((1u << N) - 1);
     };
-    auto store = [&](int chunk, const float (&g)[8]) {
-        const int e0 = chunk * 8 - a;
-        if (gvec && e0 >= 0 && e0 + 8 <= classes) {
-            Raw r;
+    auto store = [&](int chunk, unsigned skip, const float (&g)[N]) {
+        T* to = gr + head + chunk * N;
+        if (gvec && skip == 0) {
+            typedef T vec __attribute__((ext_vector_type(N)));
+            vec r;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) r[j] = (T)g[j];
-            *reinterpret_cast<Raw*>(gr + e0) = r;
+            for (int j = 0; j < N; ++j) r[j] = (T)g[j];
+            *reinterpret_cast<vec*>(to) = r;
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (e0 + j >= 0 && e0 + j < classes) gr[e0 + j] = (T)g[j];
+            for (int j = 0; j < N; ++j)
+                if (!(skip >> j & 1)) to[j] = (T)g[j];
         }
     };
 
     const float w = p.weight ? p.weight[row] : 1.f;
-    Raw raw[NV > 0 ? NV : 1];
-    if (w != 0.f) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int chunk = i * NT + tid;
-            if (chunk < chunks) raw[i] = load(chunk);
-            else
-#pragma unroll
-                for (int j = 0; j < 8; ++j) raw[i][j] = (T)-INFINITY;
-        }
-    }
-    for (int i = tid; i < words; i += NT) bits[i] = 0;
-    float total = (float)p.rows;
-    if (p.weight) {
-        if (p.total) {
-            total = p.total[0];
-        } else {
-            float s = 0.f;
-            for (long i = tid; i < p.rows; i += NT) s += p.weight[i];
-            total = block_sum<NT>(s, red);
-        }
-    }
-    __syncthreads();
-
-    if (w != 0.f && tid < 64) {     // the list, by the first wave
+    const float c2 = p.inv_tau * 1.44269504f;
+    if (w != 0.f && tid < 64) {     // the list, by the first wave, before its share of the row
+        for (int i = lane; i < words / 4; i += 64) reinterpret_cast<uint4*>(bits)[i] = make_uint4(0, 0, 0, 0);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         int any = 0, twice = 0;
         float m = -INFINITY;
         for (int i = lane; i < p.top; i += 64) {
@@ -148,21 +162,23 @@ __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
             const int id = in ? (int)id64 : -1;
             l_id[i] = id;
             l_lp[i] = t;
-            l_z[i] = in ? (float)x[id] * p.inv_tau : 0.f;
+            l_z[i] = in ? (float)x[id] : 0.f;
             if (in) {
                 any = 1;
                 m = fmaxf(m, t);
-                const unsigned bit = 1u << ((id + a) & 31);
-                twice |= (atomicOr(&bits[(id + a) >> 5], bit) & bit) != 0;
+                const int place = id - head + 8;
+                const unsigned bit = 1u << (place & 31);
+                twice |= (atomicOr(&bits[place >> 5], bit) & bit) != 0;
             }
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         any = __any(any);
         twice = __any(twice);
-        m = wave_all_max(m);
         float norm = 0.f;
         if (REST) {
             norm = p.lse[row];
         } else {
+            m = wave_all_max(m);
             float s = 0.f;
             for (int i = lane; i < p.top; i += 64)
                 if (l_id[i] >= 0) s += expf(l_lp[i] - m);
@@ -175,9 +191,9 @@ __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
             l_p[i] = pr;
             mass += pr;
         }
-        mass = wave_all_sum(mass);
         float ml = -INFINITY, sl = 0.f;
         if (REST) {     // statistics of the listed classes, each once
+            mass = wave_all_sum(mass);
             for (int i = lane; i < p.top; i += 64)
                 if (l_id[i] >= 0) ml = fmaxf(ml, l_z[i]);
             ml = wave_all_max(ml);
@@ -185,7 +201,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
                 bool first = l_id[i] >= 0;
                 if (twice)
                     for (int j = 0; j < i && first; ++j) first = l_id[j] != l_id[i];
-                if (first) sl += exp_from(l_z[i], ml);
+                if (first) sl += power(l_z[i], ml, c2);
             }
             sl = wave_all_sum(sl);
         }
@@ -199,59 +215,88 @@ __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
             told[5] = twice ? 1.f : 0.f;
         }
     }
+    i32x4 raw[NV > 0 ? NV : 1];
+    float lone = -INFINITY;         // the thread's loose value
+    if (w != 0.f) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int chunk = i * NT + tid;
+            if (chunk < chunks) {
+                raw[i] = *reinterpret_cast<const i32x4*>(x + head + chunk * N);
+            } else {
+                raw[i] = i32x4{0, 0, 0, 0};
+                strike<T>(raw[i], (1u << N) - 1);
+            }
+        }
+        if (loose >= 0) lone = (float)x[loose];
+    }
+    if (p.weight && tid >= 64 && tid < 128) {
+        float s = 0.f;
+        if (p.total) s = p.total[0];
+        else {
+            for (long i = lane; i < p.rows; i += 64) s += p.weight[i];
+            s = wave_all_sum(s);
+        }
+        if (lane == 0) told[6] = s;
+    }
     __syncthreads();
     if (w == 0.f || told[0] == 0.f) {       // nothing to learn in this row
         if (p.grad) {
-            const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            for (int c = tid; c < chunks; c += NT) store(c, zero);
+            const float zero[N] = {};
+            for (int c = tid; c < chunks; c += NT) store(c, 0, zero);
+            if (loose >= 0) gr[loose] = (T)0.f;
         }
         if (tid == 0) p.row_loss[row] = 0.f;
         return;
     }
+    const float total = p.weight ? told[6] : (float)p.rows;
+    const bool lone_listed = loose >= 0 && (bits[(loose - head + 8) >> 5] >> ((loose - head + 8) & 31) & 1);
+    if (REST && lone_listed) lone = -INFINITY;
 
-    // maximum and sum of exponentials of the unlisted classes (REST) or of all
-    auto values = [&](const Raw& r, int chunk, float (&v)[8]) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = (float)r[j] * p.inv_tau;
-        if (REST) {
-            const unsigned marked = chunk < chunks ? reinterpret_cast<const unsigned char*>(bits)[chunk] : 0;
-            if (marked) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (marked >> j & 1) v[j] = -INFINITY;
-            }
-        }
-    };
-    float m = -INFINITY, s = 0.f;
+    // maximum and sum of powers of the unlisted classes (REST) or of all
+    float m = lone, s = 0.f;
     if (NV > 0) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            float v[8];
-            values(raw[i], i * NT + tid, v);
+            if (REST && i * NT + tid < chunks) {
+                const unsigned marked = marks(i * NT + tid);
+                if (marked) strike<T>(raw[i], marked);
+            }
+            float v[N];
+            unpack(raw[i], v, T());
 #pragma unroll
-            for (int j = 0; j < 8; ++j) m = fmaxf(m, v[j]);
+            for (int j = 0; j < N; ++j) m = fmaxf(m, v[j]);
         }
+        const float off = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            float v[8];
-            values(raw[i], i * NT + tid, v);
+            asm volatile("" : "+v"(raw[i]));        // unpack again here: keeping every pass's values costs more registers than there are
+            float v[N];
+            unpack(raw[i], v, T());
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s += exp_from(v[j], m);
+            for (int j = 0; j < N; ++j) s += __builtin_amdgcn_exp2f((v[j] - off) * c2);
         }
+        s += __builtin_amdgcn_exp2f((lone - off) * c2);
     } else {
+        s = power(lone, lone, c2);
         for (int c = tid; c < chunks; c += NT) {
-            float v[8], mc = -INFINITY, sc = 0.f;
-            values(load(c), c, v);
+            i32x4 r = *reinterpret_cast<const i32x4*>(x + head + c * N);
+            if (REST) {
+                const unsigned marked = marks(c);
+                if (marked) strike<T>(r, marked);
+            }
+            float v[N], mc = -INFINITY, sc = 0.f;
+            unpack(r, v, T());
 #pragma unroll
-            for (int j = 0; j < 8; ++j) mc = fmaxf(mc, v[j]);
+            for (int j = 0; j < N; ++j) mc = fmaxf(mc, v[j]);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sc += exp_from(v[j], mc);
-            join_stats(m, s, mc, sc);
+            for (int j = 0; j < N; ++j) sc += power(v[j], mc, c2);
+            join_stats(m, s, mc, sc, c2);
         }
     }
     {
         const float mw = wave_all_max(m);
-        s = wave_all_sum(s * exp_from(m, mw));
+        s = wave_all_sum(s * power(m, mw, c2));
         m = mw;
         if (lane == 0) {
             red[2 * (tid >> 6)] = m;
@@ -260,42 +305,44 @@ __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
         __syncthreads();
         m = red[0];
         s = red[1];
-        for (int i = 1; i < NT / 64; ++i) join_stats(m, s, red[2 * i], red[2 * i + 1]);
+        for (int i = 1; i < NT / 64; ++i) join_stats(m, s, red[2 * i], red[2 * i + 1], c2);
     }
     const float P = told[1], rest = told[2];
     float mall = m, sall = s;
-    if (REST) join_stats(mall, sall, told[3], told[4]);
-    const float lse = mall + logf(sall);
+    if (REST) join_stats(mall, sall, told[3], told[4], c2);
+    const float log_sall = logf(sall);
     const bool there = REST && rest > 0.f && m > -INFINITY;
     const float gs = total != 0.f ? p.grad_scale * (w / total) : 0.f;
     if (p.grad) {
-        // e^(z - m) times one factor for every class that is not listed
-        const float f = gs * (REST ? P * __expf(m - lse) - (there ? rest / s : 0.f) : P / s);
+        // e^((x - m) / tau) times one factor for every class that is not listed
+        const float f = gs * (REST ? P * power(m, mall, c2) / sall - (there ? rest / s : 0.f) : P / s);
+        const float off = m == -INFINITY ? 0.f : m;
+        auto gradient = [&](int chunk, const i32x4& r) {
+            float v[N];
+            unpack(r, v, T());
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] = __builtin_amdgcn_exp2f((v[j] - off) * c2) * f;
+            store(chunk, marks(chunk), v);
+        };
         if (NV > 0) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int chunk = i * NT + tid;
-                if (chunk < chunks) {
-                    float v[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = exp_from((float)raw[i][j] * p.inv_tau, m) * f;
-                    store(chunk, v);
-                }
+                asm volatile("" : "+v"(raw[i]));
+                if (i * NT + tid < chunks) gradient(i * NT + tid, raw[i]);
             }
         } else {
-            for (int c = tid; c < chunks; c += NT) {
-                const Raw r = load(c);
-                float v[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = exp_from((float)r[j] * p.inv_tau, m) * f;
-                store(c, v);
-            }
+            for (int c = tid; c < chunks; c += NT) gradient(c, *reinterpret_cast<const i32x4*>(x + head + c * N));
         }
-        __syncthreads();        // (waits for the stores: the listed classes are written again)
+        if (loose >= 0 && !lone_listed) gr[loose] = (T)(__builtin_amdgcn_exp2f((lone - off) * c2) * f);
+    }
+    if (tid < 64) {
         const bool twice = told[5] != 0.f;
-        for (int i = tid; i < p.top; i += NT) {
+        float l = 0.f;
+        for (int i = lane; i < p.top; i += 64) {
             const int id = l_id[i];
             if (id < 0) continue;
+            if (l_p[i] > 0.f || l_p[i] != l_p[i]) l += l_p[i] * (l_lp[i] - ((l_z[i] - mall) * p.inv_tau - log_sall));
+            if (!p.grad) continue;
             float pi = l_p[i];
             bool first = true;
             if (twice) {
@@ -306,15 +353,10 @@ __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
                         pi += l_p[j];
                     }
             }
-            if (first) gr[id] = (T)(gs * (P * __expf(l_z[i] - lse) - pi));
+            if (first) gr[id] = (T)(gs * (P * power(l_z[i], mall, c2) / sall - pi));
         }
-    }
-    if (tid < 64) {
-        float l = 0.f;
-        for (int i = lane; i < p.top; i += 64)
-            if (l_p[i] > 0.f || l_p[i] != l_p[i]) l += l_p[i] * (l_lp[i] - (l_z[i] - lse));
         l = wave_all_sum(l);
-        if (there) l += rest * (logf(rest) - (m + logf(s) - lse));
+        if (there) l += rest * (logf(rest) - ((m - mall) * p.inv_tau + logf(s) - log_sall));
         if (lane == 0) p.row_loss[row] = w * l;
     }
 }
@@ -342,8 +384,7 @@ constexpr int kMaxClasses = 1 << 20, kMaxTop = 1024;
 
 template <typename T, int NT, int NV>
 static int launch_distill(const Distill& p, hipStream_t st) {
-    // (7 classes more than there are: a row may start inside a chunk)
-    const size_t lds = ((size_t)(p.classes + 7 + 7) / 8 + 16 + 15) / 16 * 16 + (size_t)p.top * 16;
+    const size_t lds = ((size_t)p.classes + 8 + 127) / 128 * 16 + (size_t)p.top * 16;
     auto go = [&](auto kernel) {
         // the list's bits of the largest vocabulary and the longest list
         constexpr int most = kMaxClasses / 8 + 64 + kMaxTop * 16;
@@ -389,18 +430,14 @@ int gan_distill_topk_mean(int dtype, long rows, int classes, const void* logits,
                     teacher_dtype, index_bytes == 8, 1.f / temperature, weight * temperature};
     const int rc = with_dtype(dtype, [&](auto* tag) {
         typedef typename std::remove_pointer<decltype(tag)>::type T;
-        const int chunks = (classes + 7 + 7) / 8;     // (a row may start anywhere in its first chunk)
+        const int chunks = classes / Chunk<T>::n;
         if (chunks <= 256) return launch_distill<T, 256, 1>(p, st);
         if (chunks <= 512) return launch_distill<T, 256, 2>(p, st);
         if (chunks <= 1024) return launch_distill<T, 256, 4>(p, st);
         if (chunks <= 2048) return launch_distill<T, 512, 4>(p, st);
         if (chunks <= 4096) return launch_distill<T, 1024, 4>(p, st);
         if (chunks <= 8192) return launch_distill<T, 1024, 8>(p, st);
-        if constexpr (sizeof(T) == 2) {
-            // 64 of the 128 registers a thread has; aligned rows fill their chunks, so the border is exact for them
-            const bool whole = aligned16(logits) && ld % 8 == 0;
-            if ((whole ? (classes + 7) / 8 : chunks) <= 16384) return launch_distill<T, 1024, 16>(p, st);
-        }
+        if (chunks <= 16384) return launch_distill<T, 1024, 16>(p, st);     // 64 of the 128 registers a thread has
         return launch_distill<T, 1024, 0>(p, st);
     });
     if (rc) return rc;

@@ -8,7 +8,7 @@
 // the row is one division away from a grid with steps of 1/8, and with y rounded once from 64 bits a value next to a border
 // falls on its own side (fp64 runs at the fp32 rate here, and the kernel waits for memory: no cost was measurable).
 //
-// Memory-bound.  A team of 64, 256 or 1024 threads keeps a whole row in registers, eight values a chunk, so every tensor is
+// Memory-bound.  A team of 64 to 1024 threads keeps a whole row in registers, eight values a chunk, so every tensor is
 // read and written once.
 #include "mx.h"
 
@@ -51,59 +51,60 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(RmsFwd p
     __shared__ float red_f[TPR / 64];
     const int t = threadIdx.x % TPR, team = threadIdx.x / TPR;
     const int c = p.c, chunks = MX ? mx_groups(c) * 16 : (c + 7) / 8;
-    for (long row0 = (long)blockIdx.x * TEAMS; row0 < p.rows; row0 += (long)gridDim.x * TEAMS) {
-        const long row = row0 + team;
-        const bool live = row < p.rows;
-        const T* xr = static_cast<const T*>(p.x) + (live ? row : 0) * p.ldx;
-        const T* rr = p.res ? static_cast<const T*>(p.res) + (live ? row : 0) * p.ldr : nullptr;
-        float v[NV][8];
-        double sd = 0;
-        float sf = 0;
+    const long row = (long)blockIdx.x * TEAMS + team;
+    const bool live = row < p.rows;
+    const T* xr = static_cast<const T*>(p.x) + (live ? row : 0) * p.ldx;
+    const T* rr = p.res ? static_cast<const T*>(p.res) + (live ? row : 0) * p.ldr : nullptr;
+    float v[NV][8], g[NV][8];
+    double sd = 0;
+    float sf = 0;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int i0 = (i * TPR + t) * 8;
-            load8(xr, i0, i0 < c ? c : 0, p.vec_x, v[i]);
-            if (rr) {
-                float r[8];
-                load8(rr, i0, i0 < c ? c : 0, p.vec_r, r);
+    for (int i = 0; i < NV; ++i) {
+        const int i0 = (i * TPR + t) * 8;
+        load8(xr, i0, i0 < c ? c : 0, p.vec_x, v[i]);
+        if (rr) load8(rr, i0, i0 < c ? c : 0, p.vec_r, g[i]);
+    }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[i][j] = (float)(T)(v[i][j] + r[j]);
-                if (live && i0 < c) store8(static_cast<T*>(p.h) + row * c, i0, c, p.vec_o, v[i]);
-            }
+    for (int i = 0; i < NV; ++i) {
+        const int i0 = (i * TPR + t) * 8;
+        if (rr) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (MX) sd = fma((double)v[i][j], (double)v[i][j], sd);
-                else sf = fmaf(v[i][j], v[i][j], sf);
-            }
+            for (int j = 0; j < 8; ++j) v[i][j] = (float)(T)(v[i][j] + g[i][j]);
+            if (live && i0 < c) store8(static_cast<T*>(p.h) + row * c, i0, c, p.vec_o, v[i]);
         }
-        float rstd;
-        double inv = 0;
+        load8(p.gamma, i0, i0 < c ? c : 0, p.vec_g, g[i]);      // (on its way while the row is summed)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (MX) sd = fma((double)v[i][j], (double)v[i][j], sd);
+            else sf = fmaf(v[i][j], v[i][j], sf);
+        }
+    }
+    float rstd;
+    double inv = 0;
+    if (MX) {
+        inv = 1.0 / sqrt(team_sum(sd, TPR, red_d) / c + (double)p.eps);
+        rstd = (float)inv;
+    } else {
+        rstd = 1.f / sqrtf(team_sum(sf, TPR, red_f) / c + p.eps);
+    }
+    if (!live) return;
+    if (p.rstd && t == 0) p.rstd[row] = rstd;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int chunk = i * TPR + t, i0 = chunk * 8;
+        float y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            y[j] = MX ? (float)((double)v[i][j] * inv * (double)g[i][j]) : v[i][j] * rstd * g[i][j];
         if (MX) {
-            inv = 1.0 / sqrt(team_sum(sd, TPR, red_d) / c + (double)p.eps);
-            rstd = (float)inv;
-        } else {
-            rstd = 1.f / sqrtf(team_sum(sf, TPR, red_f) / c + p.eps);
-        }
-        if (!live) continue;    // (a team of 64 takes no barrier, a larger one is the whole block)
-        if (p.rstd && t == 0) p.rstd[row] = rstd;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int chunk = i * TPR + t, i0 = chunk * 8;
-            float g[8], y[8];
-            load8(p.gamma, i0, i0 < c ? c : 0, p.vec_g, g);
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                y[j] = MX ? (float)((double)v[i][j] * inv * (double)g[j]) : v[i][j] * rstd * g[j];
-            if (MX) {
-                unsigned code[2];
-                const unsigned byte = mx_quantize_lane8<GAN_MX_E4M3>(y, code);   // (all lanes: the block's four exchange maxima)
-                if (chunk < chunks) {
-                    *reinterpret_cast<uint2*>(p.codes + row * (chunks * 8L) + i0) = make_uint2(code[0], code[1]);
-                    if ((chunk & 3) == 0) p.scales[row * (chunks / 4L) + chunk / 4] = (unsigned char)byte;
-                }
-            } else if (i0 < c) {
-                store8(static_cast<T*>(p.y) + row * c, i0, c, p.vec_o, y);
+            unsigned code[2];
+            const unsigned byte = mx_quantize_lane8<GAN_MX_E4M3>(y, code);   // (all lanes: the block's four exchange maxima)
+            if (chunk < chunks) {
+                *reinterpret_cast<uint2*>(p.codes + row * (chunks * 8L) + i0) = make_uint2(code[0], code[1]);
+                if ((chunk & 3) == 0) p.scales[row * (chunks / 4L) + chunk / 4] = (unsigned char)byte;
             }
+        } else if (i0 < c) {
+            store8(static_cast<T*>(p.y) + row * c, i0, c, p.vec_o, y);
         }
     }
 }
@@ -129,46 +130,53 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(RmsBwd p
     __shared__ float red[TPR / 64];
     const int t = threadIdx.x % TPR, c = p.c;
     const long team = (long)blockIdx.x * TEAMS + threadIdx.x / TPR, teams = (long)gridDim.x * TEAMS;
-    float acc[NV][8];
+    constexpr bool kHold = TPR < 1024;      // gamma stays in registers, and dh comes with the row (1024 threads have 128 registers each)
+    float acc[NV][8], w[NV][8];
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+        const int i0 = (i * TPR + t) * 8;
+        if (kHold) load8(p.gamma, i0, i0 < c ? c : 0, p.vec_g, w[i]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[i][j] = 0.f;
+    }
     for (long row = team; row < p.rows; row += teams) {
         const T* hr = static_cast<const T*>(p.h) + row * p.ldh;
         const T* yr = static_cast<const T*>(p.dy) + row * c;
+        const T* dhr = p.dh && p.dx ? static_cast<const T*>(p.dh) + row * c : nullptr;
         const float rstd = p.rstd[row];
-        float n[NV][8], g[NV][8], s = 0.f;
+        float n[NV][8], g[NV][8], d[NV][8], s = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int i0 = (i * TPR + t) * 8, cc = i0 < c ? c : 0;
-            float w[8];
             load8(hr, i0, cc, p.vec_h, n[i]);
             load8(yr, i0, cc, p.vec_o, g[i]);
-            load8(p.gamma, i0, cc, p.vec_g, w);
+            if (kHold && dhr) load8(dhr, i0, cc, p.vec_o, d[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (!kHold) load8(p.gamma, (i * TPR + t) * 8, (i * TPR + t) * 8 < c ? c : 0, p.vec_g, w[0]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 n[i][j] *= rstd;
                 acc[i][j] = fmaf(g[i][j], n[i][j], acc[i][j]);
-                g[i][j] *= w[j];
+                g[i][j] *= w[kHold ? i : 0][j];
                 s = fmaf(g[i][j], n[i][j], s);
             }
         }
         if (!p.dx) continue;
         const float m = team_sum(s, TPR, red) / c;
-        const T* dhr = p.dh ? static_cast<const T*>(p.dh) + row * c : nullptr;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int i0 = (i * TPR + t) * 8;
             if (i0 >= c) continue;
-            float d[8];
-            if (dhr) load8(dhr, i0, c, p.vec_o, d);
+            float o[8];
+            if (!kHold && dhr) load8(dhr, i0, c, p.vec_o, d[i]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float v = rstd * (g[i][j] - n[i][j] * m);
-                d[j] = dhr ? v + d[j] : v;
+                o[j] = rstd * (g[i][j] - n[i][j] * m);
+                if (dhr) o[j] += d[i][j];
             }
-            store8(static_cast<T*>(p.dx) + row * c, i0, c, p.vec_o, d);
+            store8(static_cast<T*>(p.dx) + row * c, i0, c, p.vec_o, o);
         }
     }
     if (p.partial) {
@@ -180,41 +188,44 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(RmsBwd p
     }
 }
 
-// dgamma[col] (+)= sum over teams of partial[team][col]: 16 columns a block, 16 teams side by side, joined in LDS.
-__global__ __launch_bounds__(256) void rms_dgamma_kernel(const float* __restrict__ partial, float* __restrict__ out, int teams,
-                                                         int c, int accumulate) {
-    __shared__ float red[16][17];
-    const int col = blockIdx.x * 16 + (threadIdx.x & 15), part = threadIdx.x >> 4;
+// dgamma[col] (+)= sum over teams of partial[team][col]: 32 columns a block, 32 teams side by side, joined in LDS.
+__global__ __launch_bounds__(1024) void rms_dgamma_kernel(const float* __restrict__ partial, float* __restrict__ out, int teams,
+                                                          int c, int accumulate) {
+    __shared__ float red[32][33];
+    const int col = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
     float s = 0.f;
-    if (col < c)
-        for (int i = part; i < teams; i += 16) s += partial[(long)i * c + col];
-    red[part][threadIdx.x & 15] = s;
+    if (col < c) {
+#pragma unroll 8
+        for (int i = part; i < teams; i += 32) s += partial[(long)i * c + col];
+    }
+    red[part][threadIdx.x & 31] = s;
     __syncthreads();
     if (part == 0 && col < c) {
         s = 0.f;
-        for (int i = 0; i < 16; ++i) s += red[i][threadIdx.x];
+        for (int i = 0; i < 32; ++i) s += red[i][threadIdx.x];
         out[col] = (accumulate ? out[col] : 0.f) + s;
     }
 }
 
-// Teams of the backward grid.
-static int rms_bwd_teams(long rows, int c) {
-    const int per = c <= 2048 ? 4 : 1;
-    long teams = c <= 2048 ? 1024 : c <= 16384 ? 512 : 256;
-    if (teams > rows) teams = rows;
-    return (int)((teams + per - 1) / per * per);
-}
-
-// Calls f(threads a row, chunks a thread) with the smallest shape that holds `chunks` chunks of eight.
+// Calls f(threads a row, chunks a thread) with a shape that holds `chunks` chunks of eight.  Few chunks a thread: a row then
+// takes few registers, and many rows are in flight on a CU.
 template <typename F>
 static void with_shape(int chunks, F f) {
     if (chunks <= 64) f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
     else if (chunks <= 128) f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
-    else if (chunks <= 256) f(std::integral_constant<int, 64>(), std::integral_constant<int, 4>());
+    else if (chunks <= 256) f(std::integral_constant<int, 256>(), std::integral_constant<int, 1>());
     else if (chunks <= 512) f(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
-    else if (chunks <= 1024) f(std::integral_constant<int, 256>(), std::integral_constant<int, 4>());
-    else if (chunks <= 2048) f(std::integral_constant<int, 256>(), std::integral_constant<int, 8>());
+    else if (chunks <= 1024) f(std::integral_constant<int, 512>(), std::integral_constant<int, 2>());
+    else if (chunks <= 2048) f(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
     else f(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
+}
+
+// Teams of the backward grid: enough to fill the chip, and few, since each leaves a row of partial sums.
+static int rms_bwd_teams(long rows, int c) {
+    const int per = c <= 1024 ? 4 : 1;      // (teams a workgroup, as with_shape gives them)
+    long teams = c <= 1024 ? 4096 : c <= 4096 ? 1024 : 512;
+    if (teams > (rows + 3) / 4) teams = (rows + 3) / 4;
+    return (int)((teams + per - 1) / per * per);
 }
 
 constexpr int kRmsMaxWidth = 32768;
@@ -285,7 +296,7 @@ int gan_rms_norm_bwd(int dtype, long rows, int c, const void* h, long ldh, const
         if (rc) return rc;
     }
     if (dgamma) {
-        hipLaunchKernelGGL(rms_dgamma_kernel, dim3((c + 15) / 16), dim3(256), 0, as_stream(stream), partial, dgamma, teams, c,
+        hipLaunchKernelGGL(rms_dgamma_kernel, dim3((c + 31) / 32), dim3(1024), 0, as_stream(stream), partial, dgamma, teams, c,
                            accumulate);
         return check_launch("gan_rms_norm_bwd");
     }

@@ -1396,12 +1396,14 @@ class _DistillFn(torch.autograd.Function):
                                         teacher.data_ptr(), index.data_ptr(), index.element_size(), teacher.shape[-1], ptr(lse),
                                         ptr(row_weight), tau, weight, 0, ptr(loss), None if grad is None else grad.data_ptr(), wp, wn,
                                         stream()))
-        ctx.grad = grad
+        # kept as a saved tensor, which autograd lets go of before the gradient reaches a leaf: the leaf then takes it over
+        # instead of copying it
+        ctx.save_for_backward(*(() if grad is None else (grad,)))
         return loss
 
     @staticmethod
     def backward(ctx, _one):
-        return (ctx.grad,) + (None,) * 6
+        return (ctx.saved_tensors[0],) + (None,) * 6
 
 
 def distill_topk_mean(logits, teacher_logits, teacher_index, temperature=1.0, weight=1.0, row_weight=None, teacher_lse=None):

@@ -83,7 +83,10 @@ def distill(logits, teacher, index, tau=1.0, weight=1.0, row_weight=None, lse=No
             lqr = torch.logsumexp(logq[outside], 0) if bool(outside.any()) else torch.tensor(-math.inf)
             if rest > 0 and float(lqr) > -math.inf:
                 l += rest * (math.log(rest) - float(lqr))
-                share = torch.where(outside, torch.exp(logq - lqr), torch.zeros_like(q))
+                # shares of the mass outside add up to 1, also where all of z is the type's lowest value and lqr has no room for
+                # the log of their number
+                share = torch.where(outside, torch.exp(z - z[outside].max()), torch.zeros_like(q))
+                share = share / share.sum()
                 g = g - rest * share
                 used = used + rest * share
         for (i, _), pi in zip(at, p):

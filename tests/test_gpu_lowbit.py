@@ -599,3 +599,15 @@ def test_gpu_calls_that_are_refused():
     with layer(rms_norm__gamma=torch.ones(40000)):
         with pytest.raises(GanHipError):
             ops.rms_norm(torch.zeros(1, 40000, device='cuda'))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_distillation_with_everything_outside_the_list_masked(dtype):
+    """All other classes at the type's lowest value: their share of the remaining mass is still theirs."""
+    g = gen(31)
+    logits = normal(g, 2, 300).to(dtype)
+    index, teacher = _lists(g, 2, 300, 5, torch.float32)
+    keep = logits.gather(1, index)
+    logits.fill_(torch.finfo(dtype).min)
+    logits.scatter_(1, index, keep)
+    _check_distill(logits, teacher, index, 2.0, 1.0, None, torch.logsumexp(teacher / 2, 1) + 0.3)
