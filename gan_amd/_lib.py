@@ -111,6 +111,8 @@ SIGNATURES = {
     "gan_mx_unpack": (I, [I, I, I, P, P, P, P]),
     "gan_mx_matmul_workspace_bytes": (Z, [I, I, I, I, I]),
     "gan_mx_matmul": (I, [I, I, I, I, I, P, P, P, P, P, P, P, Z, P]),
+    "gan_mx_linear_workspace_bytes": (Z, [I, I, I, I, I]),
+    "gan_mx_linear": (I, [I, I, I, I, I, P, L, P, P, P, P, P, Z, P]),
     "gan_mx_matmul_dgrad_workspace_bytes": (Z, [I, I, I, I]),
     "gan_mx_matmul_dgrad": (I, [I, I, I, I, P, P, P, P, P, Z, P]),
     "gan_mx_matmul_wgrad_workspace_bytes": (Z, [I, I, I, I]),
@@ -182,7 +184,7 @@ def dtype_code(dtype):
 
 def here(*tensors):
     """The device the library is about to launch on; every tensor (None is skipped) has to live there."""
-    dev = torch.cuda.current_device()
+    dev = _current_device()
     for t in tensors:
         if t is not None and t.get_device() != dev:
             raise GanHipError("libgan_hip launches on the current device cuda:%d, got a tensor on %s" % (dev, t.device))
@@ -198,7 +200,20 @@ def scratch(nbytes, device):
     return t.data_ptr(), int(nbytes), t
 
 
+# The two queries every call makes, without the Python layers of torch.cuda (2.5 us a call) where this torch has them.
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+_raw_device = getattr(torch._C, '_cuda_getDevice', None)
+
+
+def _current_device():
+    if _raw_device is not None and torch.cuda.is_initialized():
+        return _raw_device()
+    return torch.cuda.current_device()
+
+
 def stream():
+    if _raw_stream is not None and torch.cuda.is_initialized():
+        return _raw_stream(_raw_device())
     return torch.cuda.current_stream().cuda_stream
 
 

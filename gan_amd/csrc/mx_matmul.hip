@@ -19,6 +19,10 @@ struct MxProduct {
     float* slabs;                   // split contraction: [splits][rows][n rounded up to 4]
     int rows, n, groups, splits;
     bool vec;
+    const void* x;                  // floats, quantised on the way: [rows][in_dim], row stride ldx
+    long ldx;
+    int in_dim;
+    bool vec_x;
 };
 
 // ------------------------------------------------------------------------------------------------ many rows
@@ -147,75 +151,115 @@ __global__ __launch_bounds__(64 * WN * WR) void mx_tile_kernel(MxProduct p) {
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
-// The weights' bytes bind.  A wave takes NT x 16 outputs and every WAVES-th group; its lanes load weight fragments (one block of
-// 16 bytes each) straight from global memory, turn codes into bf16 and multiply on the bf16 pipe, which also makes the sums
-// fp32 for every result type.  RT tiles of 16 rows share each converted fragment.  The waves' sums meet in LDS.
-template <typename T, int FMT, int NT, int RT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void mx_few_kernel(MxProduct p) {
-    constexpr int ROW = FMT == GAN_MX_E4M3 ? 128 : 64, BLK = ROW / 4;
-    __shared__ f32x4 red[WAVES][NT * RT][64];
+// The weights' bytes bind, and for one token the wait for them.  A wave takes 16 outputs and every WAVES-th group of its
+// workgroup's range; its lanes load weight fragments (one block of 16 bytes each) straight from global memory, AHEAD groups at
+// once, turn codes into bf16 and multiply on the bf16 pipe, which also makes the sums fp32 for every result type.  RT tiles of 16
+// rows share each converted fragment.  The waves' sums meet in LDS.
+// FUSED: the activations are still floats.  The workgroup quantises its range of the contraction first, each value once, and
+// keeps the quantised values as bf16 in LDS: one launch instead of two.  Every workgroup repeats that work, so this is for few
+// values (kFusedValues).
+template <typename T, int FMT, int RT, bool FUSED>
+__global__ __launch_bounds__(512) void mx_few_kernel(MxProduct p) {
+    constexpr int WAVES = 8, AHEAD = 4, ROW = FMT == GAN_MX_E4M3 ? 128 : 64, BLK = ROW / 4;
+    __shared__ f32x4 red[WAVES][RT][64];
+    extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, q = lane >> 4;
-    const int n0 = blockIdx.x * NT * 16, r0 = blockIdx.z * RT * 16;
+    const int n0 = blockIdx.x * 16, r0 = blockIdx.z * RT * 16;
     const int g0 = (int)((long)p.groups * blockIdx.y / p.splits), g1 = (int)((long)p.groups * (blockIdx.y + 1) / p.splits);
-    f32x4 acc[NT][RT];
+    const int n = min(n0 + l16, p.n - 1);
+    f32x4 acc[RT];
+    int r[RT];
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+    for (int j = 0; j < RT; ++j) {
+        acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        r[j] = min(r0 + j * 16 + l16, p.rows - 1);
+    }
+    constexpr int CODES = FUSED ? 0 : FMT == GAN_MX_E4M3 ? 2 : 1;     // 16-byte loads of a row's codes
+    uint4 cw[AHEAD], ca[AHEAD][RT][CODES ? CODES : 1];
+    unsigned sw[AHEAD], sa[AHEAD][RT];
+    auto fetch = [&](int u, int g) {
+        const int gu = min(g, g1 - 1);
+        cw[u] = reinterpret_cast<const uint4*>(p.w)[((long)gu * 4 + q) * p.n + n];
+        sw[u] = p.ws[((long)gu * p.n + n) * 4 + q];
+        if constexpr (!FUSED) {
 #pragma unroll
-        for (int j = 0; j < RT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    int n[NT], r[RT];
+            for (int j = 0; j < RT; ++j) {
+                const uint4* at = reinterpret_cast<const uint4*>(p.a + ((long)r[j] * p.groups + gu) * ROW + q * BLK);
 #pragma unroll
-    for (int i = 0; i < NT; ++i) n[i] = min(n0 + i * 16 + l16, p.n - 1);
-#pragma unroll
-    for (int j = 0; j < RT; ++j) r[j] = min(r0 + j * 16 + l16, p.rows - 1);
-    for (int g = g0 + wave; g < g1; g += WAVES) {
-        uint4 cw[NT];
-        unsigned sw[NT];
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            cw[i] = reinterpret_cast<const uint4*>(p.w)[((long)g * 4 + q) * p.n + n[i]];
-            sw[i] = p.ws[((long)g * p.n + n[i]) * 4 + q];
-        }
-        bf16x8 a[RT][4];
-#pragma unroll
-        for (int j = 0; j < RT; ++j) {
-            const unsigned char* at = p.a + ((long)r[j] * p.groups + g) * ROW + q * BLK;
-            const float s = mx_scale(p.as[((long)r[j] * p.groups + g) * 4 + q]);
-            const uint4 u = *reinterpret_cast<const uint4*>(at);
-            if constexpr (FMT == GAN_MX_E4M3) {
-                const uint4 v = *reinterpret_cast<const uint4*>(at + 16);
-                a[j][0] = e4m3_to_bf16(u.x, u.y, s);
-                a[j][1] = e4m3_to_bf16(u.z, u.w, s);
-                a[j][2] = e4m3_to_bf16(v.x, v.y, s);
-                a[j][3] = e4m3_to_bf16(v.z, v.w, s);
-            } else {
-                a[j][0] = e2m1_to_bf16(u.x, s);
-                a[j][1] = e2m1_to_bf16(u.y, s);
-                a[j][2] = e2m1_to_bf16(u.z, s);
-                a[j][3] = e2m1_to_bf16(u.w, s);
+                for (int k = 0; k < CODES; ++k) ca[u][j][k] = at[k];
+                sa[u][j] = p.as[((long)r[j] * p.groups + gu) * 4 + q];
             }
         }
+    };
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            const float s = mx_scale(sw[i]);
-            const unsigned u[4] = {cw[i].x, cw[i].y, cw[i].z, cw[i].w};
+    for (int u = 0; u < AHEAD; ++u) fetch(u, g0 + wave + u * WAVES);
+    const int span = (g1 - g0) * 128, pitch = span + 8;     // (LDS rows 16 bytes apart in their banks)
+    bf16_t* values = reinterpret_cast<bf16_t*>(lds);
+    if constexpr (FUSED) {
+        const T* x = static_cast<const T*>(p.x);
+        const int per = span / 8, total = p.rows * per;     // (a multiple of 4: the lanes of a block stay together)
+        for (int i = threadIdx.x; i < total; i += 512) {
+            const int row = i / per, c = (i - row * per) * 8, i0 = g0 * 128 + c;
+            float v[8];
+            load8(x + row * p.ldx, i0, i0 < p.in_dim ? p.in_dim : 0, p.vec_x, v);
+            unsigned code[2];
+            const float s = mx_scale(mx_quantize_lane8<FMT>(v, code));
+            bf16x8 b;
+            if constexpr (FMT == GAN_MX_E4M3) b = e4m3_to_bf16(code[0], code[1], s);
+            else b = e2m1_to_bf16(code[0], s);
+            *reinterpret_cast<bf16x8*>(values + row * pitch + c) = b;
+        }
+        __syncthreads();
+    }
+    for (int g = g0 + wave; g < g1; g += WAVES * AHEAD) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int gu = g + u * WAVES;
+            if (gu >= g1) break;
+            bf16x8 a[RT][4];
+#pragma unroll
+            for (int j = 0; j < RT; ++j) {
+                if constexpr (FUSED) {
+                    const bf16x8* at = reinterpret_cast<const bf16x8*>(values + r[j] * pitch + (gu - g0) * 128 + q * 32);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) a[j][k] = at[k];
+                } else {
+                    const float s = mx_scale(sa[u][j]);
+                    const uint4 c = ca[u][j][0];
+                    if constexpr (FMT == GAN_MX_E4M3) {
+                        const uint4 d = ca[u][j][1];
+                        a[j][0] = e4m3_to_bf16(c.x, c.y, s);
+                        a[j][1] = e4m3_to_bf16(c.z, c.w, s);
+                        a[j][2] = e4m3_to_bf16(d.x, d.y, s);
+                        a[j][3] = e4m3_to_bf16(d.z, d.w, s);
+                    } else {
+                        a[j][0] = e2m1_to_bf16(c.x, s);
+                        a[j][1] = e2m1_to_bf16(c.y, s);
+                        a[j][2] = e2m1_to_bf16(c.z, s);
+                        a[j][3] = e2m1_to_bf16(c.w, s);
+                    }
+                }
+            }
+            const float s = mx_scale(sw[u]);
+            const unsigned c[4] = {cw[u].x, cw[u].y, cw[u].z, cw[u].w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const bf16x8 b = e2m1_to_bf16(u[k], s);
+                const bf16x8 b = e2m1_to_bf16(c[k], s);
 #pragma unroll
-                for (int j = 0; j < RT; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, a[j][k], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < RT; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, a[j][k], acc[j], 0, 0, 0);
             }
+            if (gu + WAVES * AHEAD < g1) fetch(u, gu + WAVES * AHEAD);      // (all lanes alike)
         }
     }
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int j = 0; j < RT; ++j) red[wave][i * RT + j][lane] = acc[i][j];
+    for (int j = 0; j < RT; ++j) red[wave][j][lane] = acc[j];
     __syncthreads();
     const int n4 = (p.n + 3) / 4 * 4;
-    for (int e = wave; e < NT * RT; e += WAVES) {
+    for (int e = wave; e < RT; e += WAVES) {
         f32x4 v = red[0][e][lane];
+#pragma unroll
         for (int w = 1; w < WAVES; ++w) v += red[w][e][lane];
-        const int row = r0 + (e % RT) * 16 + l16, col = n0 + (e / RT) * 16 + 4 * q;
+        const int row = r0 + e * 16 + l16, col = n0 + 4 * q;
         if (row >= p.rows || col >= p.n) continue;
         if (p.slabs) *reinterpret_cast<f32x4*>(p.slabs + ((long)blockIdx.y * p.rows + row) * n4 + col) = v;
         else store4(static_cast<T*>(p.y) + (long)row * p.n, col, p.n, p.vec, v, p.bias, 0);
@@ -234,8 +278,9 @@ static MxPlan mx_plan(int dtype, int fmt, int rows, int in_dim, int out_dim) {
     const int groups = mx_groups(in_dim);
     if (rows <= kFewRows) {
         const long wgs = (long)((out_dim + 15) / 16) * ((rows + 31) / 32);
+        // (a workgroup takes 64 groups, 8 a wave, in the time that a second launch for the joining costs)
         long s = wgs >= 256 ? 1 : 256 / wgs;
-        if (s > groups / 8) s = groups / 8;
+        if (s > groups / 64) s = groups / 64;
         return {MX_FEW, s < 1 ? 1 : (int)s};
     }
     if (fmt == GAN_MX_E4M3 && dtype == GAN_F32) return {MX_VIA_BF16, 1};
@@ -256,11 +301,25 @@ static int launch_tile(const MxProduct& p, hipStream_t st) {
     return 0;
 }
 
+// A workgroup quantises up to this many floats itself: 4 rounds of its 512 threads by 8 values, about 1 us; as a launch of its own
+// the quantisation takes 3 us and the gap between the two.
+constexpr int kFusedValues = 16384;
+
+static bool mx_fused(const MxPlan& plan, int rows, int in_dim) {
+    return plan.kind == MX_FEW && rows <= 16 &&
+           (long)rows * ((mx_groups(in_dim) + plan.splits - 1) / plan.splits) * 128 <= kFusedValues;
+}
+
 template <typename T, int FMT>
 static int launch_few(const MxProduct& p, hipStream_t st) {
-    const dim3 grid((p.n + 15) / 16, p.splits, (p.rows + 31) / 32);
-    if (p.rows <= 16) hipLaunchKernelGGL((mx_few_kernel<T, FMT, 1, 1, 8>), grid, dim3(512), 0, st, p);
-    else hipLaunchKernelGGL((mx_few_kernel<T, FMT, 1, 2, 8>), grid, dim3(512), 0, st, p);
+    if (p.x) {
+        const size_t lds = (size_t)p.rows * ((p.groups + p.splits - 1) / p.splits * 128 + 8) * 2;
+        hipLaunchKernelGGL((mx_few_kernel<T, FMT, 1, true>), dim3((p.n + 15) / 16, p.splits), dim3(512), lds, st, p);
+    } else if (p.rows <= 16) {
+        hipLaunchKernelGGL((mx_few_kernel<T, FMT, 1, false>), dim3((p.n + 15) / 16, p.splits), dim3(512), 0, st, p);
+    } else {
+        hipLaunchKernelGGL((mx_few_kernel<T, FMT, 2, false>), dim3((p.n + 15) / 16, p.splits, (p.rows + 31) / 32), dim3(512), 0, st, p);
+    }
     return 0;
 }
 
@@ -281,6 +340,38 @@ size_t gan_mx_matmul_workspace_bytes(int dtype, int fmt, int rows, int in_dim, i
     return slab_bytes(plan.splits, rows, out_dim);
 }
 
+static int mx_product(int dtype, int fmt, int rows, int in_dim, int out_dim, const void* x, long ldx, const void* a_codes,
+                      const void* a_scales, const void* w_codes, const void* w_scales, const float* bias, void* y, void* ws,
+                      hipStream_t st, const char* what) {
+    const MxPlan plan = mx_plan(dtype, fmt, rows, in_dim, out_dim);
+    if (plan.kind == MX_VIA_BF16) {
+        const int kp = mx_groups(in_dim) * 128;
+        bf16_t* a = static_cast<bf16_t*>(ws);
+        bf16_t* w = a + (long)rows * kp;
+        mx_rows_to_bf16(fmt, a_codes, a_scales, a, rows, in_dim, st);
+        mx_weights_to_bf16(w_codes, w_scales, w, in_dim, out_dim, st);
+        const Bf16Product p{a, w, kp, kp, 0, 0, 1, kp, rows, out_dim, bias, 0};
+        return bf16_product(p, static_cast<float*>(y), w + (long)out_dim * kp, st, what);
+    }
+    return with_dtype(dtype, [&](auto* tag) {
+        typedef typename std::remove_pointer<decltype(tag)>::type T;
+        const bool vec = out_dim % 4 == 0 && (reinterpret_cast<size_t>(y) & (4 * sizeof(T) - 1)) == 0 && aligned16(bias);
+        MxProduct p{static_cast<const unsigned char*>(a_codes), static_cast<const unsigned char*>(a_scales),
+                    static_cast<const unsigned char*>(w_codes), static_cast<const unsigned char*>(w_scales),
+                    bias, y, plan.splits > 1 ? static_cast<float*>(ws) : nullptr, rows, out_dim, mx_groups(in_dim), plan.splits, vec,
+                    x, ldx, in_dim, aligned16(x) && ldx * sizeof(T) % 16 == 0};
+        int rc;
+        if (plan.kind == MX_FEW) rc = fmt == GAN_MX_E4M3 ? launch_few<T, GAN_MX_E4M3>(p, st) : launch_few<T, GAN_MX_E2M1>(p, st);
+        else if (plan.kind == MX_TILE_LARGE)
+            rc = fmt == GAN_MX_E4M3 ? launch_tile<T, GAN_MX_E4M3, 256, 256, 2, 4>(p, st) : launch_tile<T, GAN_MX_E2M1, 256, 256, 2, 4>(p, st);
+        else
+            rc = fmt == GAN_MX_E4M3 ? launch_tile<T, GAN_MX_E4M3, 128, 128, 2, 2>(p, st) : launch_tile<T, GAN_MX_E2M1, 128, 128, 2, 2>(p, st);
+        if (rc) return rc;
+        if (plan.splits > 1) join_slabs(p.slabs, plan.splits, static_cast<T*>(y), (long)rows, out_dim, bias, 0, vec, st);
+        return check_launch(what);
+    });
+}
+
 int gan_mx_matmul(int dtype, int fmt, int rows, int in_dim, int out_dim, const void* a_codes, const void* a_scales,
                   const void* w_codes, const void* w_scales, const float* bias, void* y, void* ws, size_t ws_bytes,
                   gan_stream_t stream) {
@@ -294,33 +385,43 @@ int gan_mx_matmul(int dtype, int fmt, int rows, int in_dim, int out_dim, const v
     const size_t need = gan_mx_matmul_workspace_bytes(dtype, fmt, rows, in_dim, out_dim);
     GAN_CHECK_ARG(ws_bytes >= need && (need == 0 || (ws && aligned16(ws))),
                   "gan_mx_matmul: workspace of %zu bytes needed (16-byte aligned), %zu given", need, ws_bytes);
-    const MxPlan plan = mx_plan(dtype, fmt, rows, in_dim, out_dim);
-    const hipStream_t st = as_stream(stream);
-    if (plan.kind == MX_VIA_BF16) {
-        const int kp = mx_groups(in_dim) * 128;
-        bf16_t* a = static_cast<bf16_t*>(ws);
-        bf16_t* w = a + (long)rows * kp;
-        mx_rows_to_bf16(fmt, a_codes, a_scales, a, rows, in_dim, st);
-        mx_weights_to_bf16(w_codes, w_scales, w, in_dim, out_dim, st);
-        const Bf16Product p{a, w, kp, kp, 0, 0, 1, kp, rows, out_dim, bias, 0};
-        return bf16_product(p, static_cast<float*>(y), w + (long)out_dim * kp, st, "gan_mx_matmul");
-    }
-    return with_dtype(dtype, [&](auto* tag) {
-        typedef typename std::remove_pointer<decltype(tag)>::type T;
-        const bool vec = out_dim % 4 == 0 && (reinterpret_cast<size_t>(y) & (4 * sizeof(T) - 1)) == 0 && aligned16(bias);
-        MxProduct p{static_cast<const unsigned char*>(a_codes), static_cast<const unsigned char*>(a_scales),
-                    static_cast<const unsigned char*>(w_codes), static_cast<const unsigned char*>(w_scales),
-                    bias, y, plan.splits > 1 ? static_cast<float*>(ws) : nullptr, rows, out_dim, mx_groups(in_dim), plan.splits, vec};
-        int rc;
-        if (plan.kind == MX_FEW) rc = fmt == GAN_MX_E4M3 ? launch_few<T, GAN_MX_E4M3>(p, st) : launch_few<T, GAN_MX_E2M1>(p, st);
-        else if (plan.kind == MX_TILE_LARGE)
-            rc = fmt == GAN_MX_E4M3 ? launch_tile<T, GAN_MX_E4M3, 256, 256, 2, 4>(p, st) : launch_tile<T, GAN_MX_E2M1, 256, 256, 2, 4>(p, st);
-        else
-            rc = fmt == GAN_MX_E4M3 ? launch_tile<T, GAN_MX_E4M3, 128, 128, 2, 2>(p, st) : launch_tile<T, GAN_MX_E2M1, 128, 128, 2, 2>(p, st);
-        if (rc) return rc;
-        if (plan.splits > 1) join_slabs(p.slabs, plan.splits, static_cast<T*>(y), (long)rows, out_dim, bias, 0, vec, st);
-        return check_launch("gan_mx_matmul");
-    });
+    return mx_product(dtype, fmt, rows, in_dim, out_dim, nullptr, 0, a_codes, a_scales, w_codes, w_scales, bias, y, ws,
+                      as_stream(stream), "gan_mx_matmul");
+}
+
+// Codes and scales of the rows in front of the product's own workspace.
+static size_t mx_codes_bytes(int fmt, int rows, int in_dim) { return (size_t)rows * mx_groups(in_dim) * (fmt == GAN_MX_E4M3 ? 128 : 64); }
+static size_t mx_scales_bytes(int rows, int in_dim) { return ((size_t)rows * mx_groups(in_dim) * 4 + 15) / 16 * 16; }
+
+size_t gan_mx_linear_workspace_bytes(int dtype, int fmt, int rows, int in_dim, int out_dim) {
+    if (rows < 1 || rows > GAN_MX_MAX_ROWS || in_dim < 1 || in_dim > GAN_MX_MAX_IN || out_dim < 1 || !dtype_ok(dtype) || !mx_fmt_ok(fmt))
+        return 0;
+    const size_t own = gan_mx_matmul_workspace_bytes(dtype, fmt, rows, in_dim, out_dim);
+    if (mx_fused(mx_plan(dtype, fmt, rows, in_dim, out_dim), rows, in_dim)) return own;
+    return own + mx_codes_bytes(fmt, rows, in_dim) + mx_scales_bytes(rows, in_dim);
+}
+
+int gan_mx_linear(int dtype, int fmt, int rows, int in_dim, int out_dim, const void* x, long ldx, const void* w_codes,
+                  const void* w_scales, const float* bias, void* y, void* ws, size_t ws_bytes, gan_stream_t stream) {
+    GAN_CHECK_ARG(dtype_ok(dtype) && mx_fmt_ok(fmt), "gan_mx_linear: unknown element type %d or format %d", dtype, fmt);
+    GAN_CHECK_ARG(rows >= 0 && rows <= GAN_MX_MAX_ROWS && in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1 && ldx >= in_dim,
+                  "gan_mx_linear: %d rows of stride %ld, %d inputs, %d outputs (up to %d rows and inputs are served)", rows, ldx, in_dim,
+                  out_dim, GAN_MX_MAX_IN);
+    if (rows == 0) return 0;
+    GAN_CHECK_ARG(x && w_codes && w_scales && y, "gan_mx_linear: null pointer");
+    GAN_CHECK_ARG(aligned16(w_codes) && (reinterpret_cast<size_t>(w_scales) & 3) == 0,
+                  "gan_mx_linear: codes have to be 16-byte and scales 4-byte aligned");
+    const size_t need = gan_mx_linear_workspace_bytes(dtype, fmt, rows, in_dim, out_dim);
+    GAN_CHECK_ARG(ws_bytes >= need && (need == 0 || (ws && aligned16(ws))),
+                  "gan_mx_linear: workspace of %zu bytes needed (16-byte aligned), %zu given", need, ws_bytes);
+    if (mx_fused(mx_plan(dtype, fmt, rows, in_dim, out_dim), rows, in_dim))
+        return mx_product(dtype, fmt, rows, in_dim, out_dim, x, ldx, nullptr, nullptr, w_codes, w_scales, bias, y, ws, as_stream(stream),
+                          "gan_mx_linear");
+    unsigned char* codes = static_cast<unsigned char*>(ws);
+    unsigned char* scales = codes + mx_codes_bytes(fmt, rows, in_dim);
+    if (const int rc = gan_mx_quantize(dtype, fmt, rows, in_dim, x, ldx, codes, scales, stream)) return rc;
+    return mx_product(dtype, fmt, rows, in_dim, out_dim, nullptr, 0, codes, scales, w_codes, w_scales, bias, y,
+                      scales + mx_scales_bytes(rows, in_dim), as_stream(stream), "gan_mx_linear");
 }
 
 }  // extern "C"

@@ -1037,6 +1037,18 @@ def _mx_product(q, w, bias):
     return y
 
 
+def _mx_linear(x, w, bias, fmt):
+    """The same from floats, in one call."""
+    _lib.here(x, w.codes, w.scales, bias)
+    code, f = _lib.dtype_code(x.dtype), _lib.MX_FORMATS[fmt]
+    y = torch.empty(tuple(x.shape[:-1]) + (w.out_dim,), dtype=x.dtype, device=x.device)
+    xs, rows, k, ld = _rows_of(x)
+    wp, wn, hold = _lib.scratch(lib.gan_mx_linear_workspace_bytes(code, f, rows, k, w.out_dim), x.device)
+    check(lib.gan_mx_linear(code, f, rows, k, w.out_dim, xs.data_ptr(), ld, w.codes.data_ptr(), w.scales.data_ptr(), ptr(bias),
+                            y.data_ptr(), wp, wn, stream()))
+    return y
+
+
 class _MxMatmulFn(torch.autograd.Function):
     """x: what carries the gradient -- the float input, or the stand-in of an MxTensor.  matrix / bias_var: the variables behind
     the packed weights (None: frozen)."""
@@ -1087,7 +1099,7 @@ def _mx_apply(x, w, bias, fmt, token=None, matrix=None, bias_var=None):
         raise ValueError("microscaled product: bias %s %s for %d outputs" % (tuple(bias.shape), bias.dtype, w.out_dim))
     if torch.is_grad_enabled() and (token is not None or (carrier is not None and carrier.requires_grad)):
         return _MxMatmulFn.apply(carrier, token, q, w, bias, matrix, bias_var, fmt)
-    return _mx_product(mx_quantize(x, fmt) if q is None else q, w, bias)
+    return _mx_linear(x, w, bias, fmt) if q is None else _mx_product(q, w, bias)
 
 
 def mx_matmul(x, w, bias=None, fmt='e4m3'):

@@ -370,6 +370,10 @@ size_t gan_mx_matmul_workspace_bytes(int dtype, int fmt, int rows, int in_dim, i
 int gan_mx_matmul(int dtype, int fmt, int rows, int in_dim, int out_dim, const void* a_codes, const void* a_scales,
                   const void* w_codes, const void* w_scales, const float* bias, void* y, void* ws, size_t ws_bytes,
                   gan_stream_t stream);
+/* the same from rows x of type dtype (row stride ldx), quantised to fmt on the way */
+size_t gan_mx_linear_workspace_bytes(int dtype, int fmt, int rows, int in_dim, int out_dim);
+int gan_mx_linear(int dtype, int fmt, int rows, int in_dim, int out_dim, const void* x, long ldx, const void* w_codes,
+                  const void* w_scales, const float* bias, void* y, void* ws, size_t ws_bytes, gan_stream_t stream);
 size_t gan_mx_matmul_dgrad_workspace_bytes(int dtype, int rows, int in_dim, int out_dim);
 int gan_mx_matmul_dgrad(int dtype, int rows, int in_dim, int out_dim, const void* dy, const void* w_codes,
                         const void* w_scales, void* dx, void* ws, size_t ws_bytes, gan_stream_t stream);
