@@ -171,8 +171,8 @@ int gan_mx_dequantize(int dtype, int fmt, long rows, int c, const void* codes, c
 int gan_mx_pack(int dtype, int in_dim, int out_dim, const void* matrix, long ld, void* codes, void* scales,
                 gan_stream_t stream) {
     GAN_CHECK_ARG(dtype_ok(dtype), "gan_mx_pack: unknown element type %d", dtype);
-    GAN_CHECK_ARG(in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1 && ld >= out_dim,
-                  "gan_mx_pack: matrix of %d x %d, row stride %ld (up to %d inputs are served)", in_dim, out_dim, ld, GAN_MX_MAX_IN);
+    GAN_CHECK_ARG(in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1 && out_dim <= GAN_MX_MAX_IN && ld >= out_dim,
+                  "gan_mx_pack: matrix of %d x %d, row stride %ld (up to %d of each are served)", in_dim, out_dim, ld, GAN_MX_MAX_IN);
     GAN_CHECK_ARG(matrix && codes && scales, "gan_mx_pack: null pointer");
     GAN_CHECK_ARG(aligned16(codes) && (reinterpret_cast<size_t>(scales) & 3) == 0,
                   "gan_mx_pack: codes have to be 16-byte and scales 4-byte aligned");
@@ -188,7 +188,7 @@ int gan_mx_pack(int dtype, int in_dim, int out_dim, const void* matrix, long ld,
 int gan_mx_unpack(int dtype, int in_dim, int out_dim, const void* codes, const void* scales, void* matrix,
                   gan_stream_t stream) {
     GAN_CHECK_ARG(dtype_ok(dtype), "gan_mx_unpack: unknown element type %d", dtype);
-    GAN_CHECK_ARG(in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1, "gan_mx_unpack: matrix of %d x %d", in_dim, out_dim);
+    GAN_CHECK_ARG(in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1 && out_dim <= GAN_MX_MAX_IN, "gan_mx_unpack: matrix of %d x %d", in_dim, out_dim);
     GAN_CHECK_ARG(matrix && codes && scales, "gan_mx_unpack: null pointer");
     GAN_CHECK_ARG(aligned16(codes) && (reinterpret_cast<size_t>(scales) & 3) == 0,
                   "gan_mx_unpack: codes have to be 16-byte and scales 4-byte aligned");

@@ -13,13 +13,19 @@
 namespace gan {
 
 // C[i][j] over a tile of BI x BJ, WI x WJ waves, 32x32x16 instructions with Q as their first operand (a lane ends with four
-// consecutive j of one i).  A step is 64 deep: rows of 128 bytes, their 16-byte chunks swapped by row so that a fragment read
-// hits all banks; two stages, filled by direct copies one step ahead.
-template <typename T, int BI, int BJ, int WI, int WJ>
+// consecutive j of one i).  A stage in LDS is 64 deep: 128 bytes of every row -- whole cache lines; 64 bytes a row and stage cost
+// twice the requests to the L2 --, their 16-byte chunks swapped by row so that a fragment read hits all banks.  STAGES stages form
+// a ring that direct copies keep filled.  The fragments of the next 16 are read while the matrix pipe works on these; the one
+// barrier of a stage stands before its last quarter, when all of it has been read: it asks for the next stage and frees this one.
+// Large tiles have two waves a SIMD with 128 x 64 outputs each: LDS then gives 96 bytes a clock of its 128; one wave of
+// 128 x 128 needs less of it, but nothing covers its waits (4096^3: 126 us against 115, the weights' image included).
+// 4096 x 4096 x 8192: 1.25 PF/s, a library product of that size 1.45.
+template <typename T, int BI, int BJ, int WI, int WJ, int STAGES>
 __global__ __launch_bounds__(64 * WI * WJ) void bf16_product_kernel(Bf16Product p, T* out, float* slabs, int splits, bool vec) {
-    constexpr int THREADS = 64 * WI * WJ, FI = BI / WI / 32, FJ = BJ / WJ / 32, STAGE = (BI + BJ) * 128;
+    constexpr int WAVES = WI * WJ, THREADS = 64 * WAVES, FI = BI / WI / 32, FJ = BJ / WJ / 32, STAGE = (BI + BJ) * 128;
+    constexpr int COPIES = STAGE / 16 / THREADS;        // of a wave for a stage
     extern __shared__ __align__(16) unsigned char lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wj = wave % WJ, wi = wave / WJ;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wj = wave % WJ, wi = wave / WJ;
     const int l32 = lane & 31, half = lane >> 5;
     int ti, tj;
     tile_of(blockIdx.x, (p.rows + BI - 1) / BI, (p.cols + BJ - 1) / BJ, ti, tj);
@@ -28,23 +34,51 @@ __global__ __launch_bounds__(64 * WI * WJ) void bf16_product_kernel(Bf16Product 
     const long steps = (long)per * p.parts;
     const int s0 = (int)(steps * blockIdx.y / splits), s1 = (int)(steps * (blockIdx.y + 1) / splits);
 
-    auto fill = [&](int s, int buf) {
-        unsigned char* base = lds + buf * STAGE;
-        const int part = s / per, c = (s - part * per) * 64;
-        const bf16_t* ps = p.p + part * p.pstep + c;
-        const bf16_t* qs = p.q + part * p.qstep + c;
+    // where this lane's copies begin, and the two operands' places in the part at hand (rows beyond the last: the last again)
+    constexpr int PC = BI * 8 / THREADS, QC = BJ * 8 / THREADS;
+    unsigned p_off[PC], q_off[QC];
 #pragma unroll
-        for (int i = 0; i < BI * 8 / THREADS; ++i) {
-            const int at = (i * WI * WJ + wave) * 64, row = (at + lane) >> 3, chunk = (lane & 7) ^ (row & 7);
-            copy_to_lds16(ps + (long)min(i0 + row, p.rows - 1) * p.ldp + chunk * 8, base + at * 16);
+    for (int i = 0; i < PC; ++i) {
+        const int row = ((i * WAVES + wave) * 64 + lane) >> 3, chunk = (lane & 7) ^ (row & 7);
+        p_off[i] = (unsigned)min(row, p.rows - 1 - i0) * (unsigned)(p.ldp * 2) + chunk * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < QC; ++i) {
+        const int row = ((i * WAVES + wave) * 64 + lane) >> 3, chunk = (lane & 7) ^ (row & 7);
+        q_off[i] = (unsigned)min(row, p.cols - 1 - j0) * (unsigned)(p.ldq * 2) + chunk * 16;
+    }
+    int filled = s0, in_part = s0 % per;
+    const unsigned char* pp = reinterpret_cast<const unsigned char*>(p.p + (long)i0 * p.ldp + (s0 / per) * p.pstep + in_part * 64L);
+    const unsigned char* qp = reinterpret_cast<const unsigned char*>(p.q + (long)j0 * p.ldq + (s0 / per) * p.qstep + in_part * 64L);
+    const long p_jump = (p.pstep - (per - 1) * 64L) * 2, q_jump = (p.qstep - (per - 1) * 64L) * 2;
+    // copies of the stage after the last one copied, into LDS from `to` on; past the end the last one again, which nobody reads
+    auto fill = [&](int to) {
+        unsigned char* base = lds + to;
+#pragma unroll
+        for (int i = 0; i < PC; ++i) copy_to_lds16(copy_source(pp), p_off[i], base + (i * WAVES + wave) * 1024);
+#pragma unroll
+        for (int i = 0; i < QC; ++i) copy_to_lds16(copy_source(qp), q_off[i], base + BI * 128 + (i * WAVES + wave) * 1024);
+        const bool more = ++filled < s1, jump = in_part == per - 1;
+        in_part = jump ? 0 : in_part + 1;
+        pp += more ? (jump ? p_jump : 128L) : 0L;
+        qp += more ? (jump ? q_jump : 128L) : 0L;
+    };
+    struct Fragments {
+        bf16x8 p[FI], q[FJ];
+    };
+    auto read = [&](int at, int k, Fragments& f) {
+        const unsigned char* base = lds + at;
+#pragma unroll
+        for (int j = 0; j < FJ; ++j) {
+            const int row = BI + (wj * FJ + j) * 32 + l32;
+            f.q[j] = *reinterpret_cast<const bf16x8*>(base + row * 128 + (((2 * k + half) ^ (row & 7)) * 16));
         }
 #pragma unroll
-        for (int i = 0; i < BJ * 8 / THREADS; ++i) {
-            const int at = (i * WI * WJ + wave) * 64, row = (at + lane) >> 3, chunk = (lane & 7) ^ (row & 7);
-            copy_to_lds16(qs + (long)min(j0 + row, p.cols - 1) * p.ldq + chunk * 8, base + BI * 128 + at * 16);
+        for (int i = 0; i < FI; ++i) {
+            const int row = (wi * FI + i) * 32 + l32;
+            f.p[i] = *reinterpret_cast<const bf16x8*>(base + row * 128 + (((2 * k + half) ^ (row & 7)) * 16));
         }
     };
-
     f32x16 acc[FJ][FI];
 #pragma unroll
     for (int j = 0; j < FJ; ++j)
@@ -52,49 +86,43 @@ __global__ __launch_bounds__(64 * WI * WJ) void bf16_product_kernel(Bf16Product 
         for (int i = 0; i < FI; ++i)
 #pragma unroll
             for (int k = 0; k < 16; ++k) acc[j][i][k] = 0.f;
-    if (s0 < s1) fill(s0, 0);
-    for (int s = s0; s < s1; ++s) {
-        const int buf = (s - s0) & 1;
-        copies_done_barrier();
-        if (s + 1 < s1) fill(s + 1, buf ^ 1);
-        const unsigned char* lp = lds + buf * STAGE;
-        const unsigned char* lq = lp + BI * 128;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            bf16x8 fp[FI], fq[FJ];
-#pragma unroll
-            for (int j = 0; j < FJ; ++j) {
-                const int row = (wj * FJ + j) * 32 + l32;
-                fq[j] = *reinterpret_cast<const bf16x8*>(lq + row * 128 + (((2 * k + half) ^ (row & 7)) * 16));
-            }
-#pragma unroll
-            for (int i = 0; i < FI; ++i) {
-                const int row = (wi * FI + i) * 32 + l32;
-                fp[i] = *reinterpret_cast<const bf16x8*>(lp + row * 128 + (((2 * k + half) ^ (row & 7)) * 16));
-            }
-#pragma unroll
-            for (int j = 0; j < FJ; ++j)
-#pragma unroll
-                for (int i = 0; i < FI; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fq[j], fp[i], acc[j][i], 0, 0, 0);
-        }
-    }
-    const int n4 = (p.cols + 3) / 4 * 4;
-#pragma unroll
-    for (int i = 0; i < FI; ++i) {
-        const int row = i0 + (wi * FI + i) * 32 + l32;
-        if (row >= p.rows) continue;
+    auto multiply = [&](const Fragments& f) {
 #pragma unroll
         for (int j = 0; j < FJ; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int col = j0 + (wj * FJ + j) * 32 + 8 * q + 4 * half;
-                const f32x4 v = {acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
-                if (slabs) {
-                    if (col < p.cols) *reinterpret_cast<f32x4*>(slabs + ((long)blockIdx.y * p.rows + row) * n4 + col) = v;
-                } else {
-                    store4(out + (long)row * p.cols, col, p.cols, vec, v, p.bias, p.accumulate);
-                }
-            }
+            for (int i = 0; i < FI; ++i) acc[j][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.q[j], f.p[i], acc[j][i], 0, 0, 0);
+    };
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s) fill(s * STAGE);
+    landed_barrier<(STAGES - 1) * COPIES>();
+    Fragments f[2];
+    read(0, 0, f[0]);
+    int at = 0;
+    for (int s = s0; s < s1; ++s) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            read(at, k + 1, f[(k + 1) % 2]);
+            multiply(f[k % 2]);
+            interleave<FI * FJ, FI + FJ, 0>();
+        }
+        landed_barrier<(STAGES - 2) * COPIES>();        // the next stage is there; STAGES - 2 more are on their way
+        const int freed = at;
+        at = at + STAGE == STAGES * STAGE ? 0 : at + STAGE;
+        read(at, 0, f[0]);
+        fill(freed);
+        multiply(f[1]);
+        interleave<FI * FJ, FI + FJ, COPIES>();
+    }
+    landed_barrier<0>();        // (no copy is in flight when the workgroup gives its LDS back)
+    float* stage = reinterpret_cast<float*>(lds) + wave * 32 * (32 * FJ + 4);
+    static_assert(WAVES * 32 * (32 * FJ + 4) * 4 <= STAGES * STAGE, "the results pass through the stages' LDS");
+    const int n4 = (p.cols + 3) / 4 * 4, col0 = j0 + wj * FJ * 32;
+#pragma unroll
+    for (int i = 0; i < FI; ++i) {
+        const int row0 = i0 + (wi * FI + i) * 32;
+        auto pick = [&](int j) -> const f32x16& { return acc[j][i]; };
+        if (slabs) store_rows<float, FJ>(pick, stage, row0, col0, p.rows, n4, slabs + (long)blockIdx.y * p.rows * n4, n4, nullptr, 0, true);
+        else store_rows<T, FJ>(pick, stage, row0, col0, p.rows, p.cols, out, p.cols, p.bias, p.accumulate, vec);
     }
 }
 
@@ -103,10 +131,13 @@ struct Bf16Plan {
     int splits;
 };
 static Bf16Plan bf16_plan(int rows, int cols, int parts, int depth) {
-    const long large = (long)((rows + 255) / 256) * ((cols + 255) / 256);
+    // 256 x 256 tiles where they fill the chip, alone (4096^3: 115 us against 132) or in parts of 32 stages or more
+    // (1024 x 1024 <- 32768: 98 us in 16 parts against 110 with small tiles in 6; 1024 x 4096 <- 4096, parts of 16: 58 against 53)
+    const long large = (long)((rows + 255) / 256) * ((cols + 255) / 256), all = (long)parts * (depth / 64);
+    const int steps = (int)(all < (1 << 30) ? all : 1 << 30);
     if (large >= 192) return {true, 1};
-    const long steps = (long)parts * (depth / 64);
-    return {false, contraction_splits((long)((rows + 127) / 128) * ((cols + 127) / 128), (int)(steps < (1 << 30) ? steps : 1 << 30), 8)};
+    if (steps / (256 / large) >= 32) return {true, (int)(256 / large)};
+    return {false, contraction_splits((long)((rows + 127) / 128) * ((cols + 127) / 128), 384, steps, 8)};
 }
 
 size_t bf16_product_workspace(int rows, int cols, int parts, int depth) {
@@ -115,8 +146,8 @@ size_t bf16_product_workspace(int rows, int cols, int parts, int depth) {
 
 template <typename T, int BI, int BJ, int WI, int WJ>
 static int launch_bf16(const Bf16Product& p, T* out, float* slabs, int splits, bool vec, hipStream_t st, const char* what) {
-    constexpr int LDS = 2 * (BI + BJ) * 128;
-    auto kernel = bf16_product_kernel<T, BI, BJ, WI, WJ>;
+    constexpr int STAGES = 2, LDS = STAGES * (BI + BJ) * 128;       // (small tiles: two workgroups a CU)
+    auto kernel = bf16_product_kernel<T, BI, BJ, WI, WJ, STAGES>;
     static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                       hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
     if (set != hipSuccess) return fail("%s: %d bytes of LDS refused: %s", what, LDS, hipGetErrorString(set));
@@ -128,12 +159,12 @@ static int launch_bf16(const Bf16Product& p, T* out, float* slabs, int splits, b
 template <typename T>
 int bf16_product(const Bf16Product& p, T* out, void* ws, hipStream_t st, const char* what) {
     const Bf16Plan plan = bf16_plan(p.rows, p.cols, p.parts, p.depth);
-    const bool vec = p.cols % 4 == 0 && (reinterpret_cast<size_t>(out) & (4 * sizeof(T) - 1)) == 0 && aligned16(p.bias);
+    const bool vec = p.cols * sizeof(T) % 16 == 0 && aligned16(out), vec4 = vec && aligned16(p.bias);
     float* slabs = plan.splits > 1 ? static_cast<float*>(ws) : nullptr;
-    const int rc = plan.large ? launch_bf16<T, 256, 256, 4, 2>(p, out, slabs, plan.splits, vec, st, what)
+    const int rc = plan.large ? launch_bf16<T, 256, 256, 2, 4>(p, out, slabs, plan.splits, vec, st, what)
                               : launch_bf16<T, 128, 128, 2, 2>(p, out, slabs, plan.splits, vec, st, what);
     if (rc) return rc;
-    if (slabs) join_slabs(slabs, plan.splits, out, (long)p.rows, p.cols, p.bias, p.accumulate, vec, st);
+    if (slabs) join_slabs(slabs, plan.splits, out, (long)p.rows, p.cols, p.bias, p.accumulate, vec4, st);
     return check_launch(what);
 }
 template int bf16_product<float>(const Bf16Product&, float*, void*, hipStream_t, const char*);
@@ -364,7 +395,7 @@ using namespace gan;
 extern "C" {
 
 size_t gan_mx_matmul_dgrad_workspace_bytes(int dtype, int rows, int in_dim, int out_dim) {
-    if (rows < 1 || rows > GAN_MX_MAX_ROWS || in_dim < 1 || in_dim > GAN_MX_MAX_IN || out_dim < 1 || !dtype_ok(dtype)) return 0;
+    if (rows < 1 || rows > GAN_MX_MAX_ROWS || in_dim < 1 || in_dim > GAN_MX_MAX_IN || out_dim < 1 || out_dim > GAN_MX_MAX_IN || !dtype_ok(dtype)) return 0;
     const size_t np = to64(out_dim), parts = parts_of(dtype);
     return in_dim * np * 2 + (dy_as_is(dtype, out_dim) ? 0 : parts * rows * np * 2) +
            bf16_product_workspace(rows, in_dim, (int)parts, (int)np);
@@ -373,8 +404,8 @@ size_t gan_mx_matmul_dgrad_workspace_bytes(int dtype, int rows, int in_dim, int 
 int gan_mx_matmul_dgrad(int dtype, int rows, int in_dim, int out_dim, const void* dy, const void* w_codes, const void* w_scales,
                         void* dx, void* ws, size_t ws_bytes, gan_stream_t stream) {
     GAN_CHECK_ARG(dtype_ok(dtype), "gan_mx_matmul_dgrad: unknown element type %d", dtype);
-    GAN_CHECK_ARG(rows >= 0 && rows <= GAN_MX_MAX_ROWS && in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1,
-                  "gan_mx_matmul_dgrad: %d rows, %d inputs, %d outputs (up to %d rows and inputs are served)", rows, in_dim, out_dim, GAN_MX_MAX_IN);
+    GAN_CHECK_ARG(rows >= 0 && rows <= GAN_MX_MAX_ROWS && in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1 && out_dim <= GAN_MX_MAX_IN,
+                  "gan_mx_matmul_dgrad: %d rows, %d inputs, %d outputs (up to %d of each are served)", rows, in_dim, out_dim, GAN_MX_MAX_IN);
     if (rows == 0) return 0;
     GAN_CHECK_ARG(dy && w_codes && w_scales && dx, "gan_mx_matmul_dgrad: null pointer");
     GAN_CHECK_ARG(aligned16(dy) && aligned16(w_codes) && (reinterpret_cast<size_t>(w_scales) & 3) == 0,
@@ -405,7 +436,7 @@ int gan_mx_matmul_dgrad(int dtype, int rows, int in_dim, int out_dim, const void
 }
 
 size_t gan_mx_matmul_wgrad_workspace_bytes(int dtype, int rows, int in_dim, int out_dim) {
-    if (rows < 1 || rows > GAN_MX_MAX_ROWS || in_dim < 1 || in_dim > GAN_MX_MAX_IN || out_dim < 1 || !dtype_ok(dtype)) return 0;
+    if (rows < 1 || rows > GAN_MX_MAX_ROWS || in_dim < 1 || in_dim > GAN_MX_MAX_IN || out_dim < 1 || out_dim > GAN_MX_MAX_IN || !dtype_ok(dtype)) return 0;
     const size_t rp = to64(rows), parts = parts_of(dtype);
     return (in_dim + parts * out_dim) * rp * 2 + (rp / 64 * out_dim * 4 + 15) / 16 * 16 +
            bf16_product_workspace(in_dim, out_dim, (int)parts, (int)rp);
@@ -415,8 +446,8 @@ int gan_mx_matmul_wgrad(int dtype, int fmt, int rows, int in_dim, int out_dim, c
                         const void* dy, float* dmatrix, float* dbias, int accumulate, void* ws, size_t ws_bytes,
                         gan_stream_t stream) {
     GAN_CHECK_ARG(dtype_ok(dtype) && mx_fmt_ok(fmt), "gan_mx_matmul_wgrad: unknown element type %d or format %d", dtype, fmt);
-    GAN_CHECK_ARG(rows >= 1 && rows <= GAN_MX_MAX_ROWS && in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1,
-                  "gan_mx_matmul_wgrad: %d rows, %d inputs, %d outputs (up to %d rows and inputs are served)", rows, in_dim, out_dim, GAN_MX_MAX_IN);
+    GAN_CHECK_ARG(rows >= 1 && rows <= GAN_MX_MAX_ROWS && in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1 && out_dim <= GAN_MX_MAX_IN,
+                  "gan_mx_matmul_wgrad: %d rows, %d inputs, %d outputs (up to %d of each are served)", rows, in_dim, out_dim, GAN_MX_MAX_IN);
     GAN_CHECK_ARG(dy && a_codes && a_scales && dmatrix, "gan_mx_matmul_wgrad: null pointer");
     GAN_CHECK_ARG(aligned16(dy) && aligned16(a_codes), "gan_mx_matmul_wgrad: dy and codes have to be 16-byte aligned");
     const size_t need = gan_mx_matmul_wgrad_workspace_bytes(dtype, rows, in_dim, out_dim);

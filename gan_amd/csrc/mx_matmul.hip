@@ -18,7 +18,7 @@ struct MxProduct {
     void* y;
     float* slabs;                   // split contraction: [splits][rows][n rounded up to 4]
     int rows, n, groups, splits;
-    bool vec;
+    bool vec, vec16;                // rows of y take 4 values, 16 bytes at a time
     const void* x;                  // floats, quantised on the way: [rows][in_dim], row stride ldx
     long ldx;
     int in_dim;
@@ -27,17 +27,26 @@ struct MxProduct {
 
 // ------------------------------------------------------------------------------------------------ many rows
 // Tile of BN outputs x BR rows, WN x WR waves; the weights are the first operand of the 32x32x64 instruction, so that a lane ends
-// with four consecutive outputs of one row.  A step is one group (128 deep): weights 4 blocks x BN x 16 bytes, contiguous as
-// packed and as read back (a lane's fragment is one block); rows 128 (64) bytes each, their 16-byte chunks swapped by row so
-// that the 32 rows of a fragment read hit all banks.  Two stages in LDS, filled by direct copies one step ahead; the scale
-// dwords go to registers one step ahead.
-template <typename T, int FMT, int BN, int BR, int WN, int WR>
+// with four consecutive outputs of one row.  A stage in LDS is 128 bytes of every row -- whole cache lines; 64 bytes a row and
+// stage cost twice the requests to the L2 -- which is one group of 128 e4m3 or two of e2m1 values: weights 4 blocks a group x BN x
+// 16 bytes, contiguous as packed and as read back (a lane's fragment is one block); rows with their 16-byte chunks swapped by row
+// so that the 32 rows of a fragment read hit all banks; a scale dword a group, output and row.  STAGES stages form a ring that
+// direct copies keep filled.  The fragments of the next 64 are read while the matrix pipe works on these; the one barrier of a stage
+// stands before its last multiplication, when all of it has been read: it asks for the next stage and frees this one.  Large
+// tiles have two waves a SIMD with 128 x 64 outputs each, LDS then gives 64 (e4m3) or 96 bytes a clock of its 128; one wave of
+// 128 x 128 needs less of it, but nothing covers its waits (4096^3: e4m3 63 us against 56, e2m1 48 against 42).
+// 4096 x 8192 x 8192: 195 us = 2.8 PF/s e4m3, 139 us = 4.0 PF/s e2m1; a bf16 library product of that size runs at 1.45 PF/s on
+// this card.  Without the copies of the loop it would be 166 and 115 us, without its cache misses no faster: the copies' way
+// through the L1 into LDS, and the barrier around them, is what is left.
+template <typename T, int FMT, int BN, int BR, int WN, int WR, int STAGES>
 __global__ __launch_bounds__(64 * WN * WR) void mx_tile_kernel(MxProduct p) {
-    constexpr int THREADS = 64 * WN * WR, FN = BN / WN / 32, FR = BR / WR / 32;
-    constexpr int ROW = FMT == GAN_MX_E4M3 ? 128 : 64, CH = ROW / 16;
-    constexpr int W_BYTES = BN * 64, STAGE = W_BYTES + BR * ROW;
+    constexpr int WAVES = WN * WR, THREADS = 64 * WAVES, FN = BN / WN / 32, FR = BR / WR / 32;
+    constexpr int G = FMT == GAN_MX_E4M3 ? 1 : 2, ROW = 128 / G;        // groups a stage, bytes of a row and group
+    constexpr int A_AT = BN * 64 * G, S_AT = A_AT + BR * 128, STAGE = S_AT + (BN + BR) * 4 * G;
+    constexpr int W_COPIES = A_AT / 16 / THREADS, A_COPIES = BR * 8 / THREADS, SEGS = (BN + BR) / 64 * G;
+    constexpr int S_COPIES = (SEGS + WAVES - 1) / WAVES, COPIES = W_COPIES + A_COPIES + S_COPIES;      // of a wave for a stage
     extern __shared__ __align__(16) unsigned char lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wn = wave % WN, wr = wave / WN;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wr = wave / WN;
     const int l32 = lane & 31, half = lane >> 5;
     const int tr = (p.rows + BR - 1) / BR, tn = (p.n + BN - 1) / BN;
     int ir, in;
@@ -45,30 +54,110 @@ __global__ __launch_bounds__(64 * WN * WR) void mx_tile_kernel(MxProduct p) {
     const int r0 = ir * BR, n0 = in * BN;
     const int g0 = (int)((long)p.groups * blockIdx.y / p.splits), g1 = (int)((long)p.groups * (blockIdx.y + 1) / p.splits);
 
-    auto fill = [&](int g, int buf) {
-        unsigned char* base = lds + buf * STAGE;
+    // where this lane's copies of a group begin (rows and outputs beyond the last: the last again)
+    unsigned w_off[W_COPIES], a_off[A_COPIES], s_off[S_COPIES];
 #pragma unroll
-        for (int i = 0; i < W_BYTES / 16 / THREADS; ++i) {
-            const int at = (i * WN * WR + wave) * 64;            // 64 blocks, one kb
-            const int kb = at / BN, n = min(n0 + at % BN + lane, p.n - 1);
-            copy_to_lds16(p.w + (((long)g * 4 + kb) * p.n + n) * 16, base + at * 16);
+    for (int i = 0; i < W_COPIES; ++i) {
+        const int at = (i * WAVES + wave) * 64;                 // 64 blocks of one kb
+        w_off[i] = (unsigned)(at / BN % 4 * p.n + min(n0 + at % BN + lane, p.n - 1)) * 16u;
+    }
+#pragma unroll
+    for (int i = 0; i < A_COPIES; ++i) {
+        const int s = (i * WAVES + wave) * 64 + lane, row = s / 8, chunk = (s % 8) ^ (row & 7);
+        a_off[i] = (unsigned)min(row, p.rows - 1 - r0) * (unsigned)(p.groups * ROW) + chunk * 16;
+    }
+    const unsigned of_second = ((lane & 7) ^ (lane >> 3)) & 4 ? 64u : 0u;       // (this lane's chunks are of a second group)
+    // (waves in excess copy a segment of the scales again)
+#pragma unroll
+    for (int i = 0; i < S_COPIES; ++i) {
+        const int seg = (i * WAVES + wave) % SEGS / G, at = seg * 64 + lane;
+        s_off[i] = seg < BN / 64 ? (unsigned)min(n0 + at, p.n - 1) * 4u : (unsigned)min(at - BN, p.rows - 1 - r0) * (unsigned)(p.groups * 4);
+    }
+    // copies of the stage after the last one copied, into LDS from `to` on; past the end the last one again, which nobody reads.
+    // Of an odd number of groups the last stage has one twice; shift_scales() gives the second no weight.
+    int next = g0;
+    const unsigned char* wg = p.w + (long)g0 * p.n * 64;
+    const unsigned char* ag = p.a + ((long)r0 * p.groups + g0) * ROW;
+    const unsigned char* sg[S_COPIES];
+    long s_step[S_COPIES];
+#pragma unroll
+    for (int i = 0; i < S_COPIES; ++i) {
+        const bool of_w = (i * WAVES + wave) % SEGS / G < BN / 64;
+        sg[i] = of_w ? p.ws + (long)g0 * p.n * 4 : p.as + ((long)r0 * p.groups + g0) * 4;
+        s_step[i] = of_w ? p.n * 4L : 4L;
+    }
+    auto fill = [&](int to) {
+        unsigned char* base = lds + to;
+        const int second = next + 1 < g1 ? 1 : 0;
+#pragma unroll
+        for (int i = 0; i < W_COPIES; ++i) {
+            const int g = G == 1 ? 0 : (i * WAVES + wave) * 64 / BN / 4 * second;
+            copy_to_lds16(copy_source(wg + g * (p.n * 64L)), w_off[i], base + (i * WAVES + wave) * 1024);
         }
 #pragma unroll
-        for (int i = 0; i < BR * CH / THREADS; ++i) {
-            const int at = (i * WN * WR + wave) * 64, s = at + lane, row = s / CH;
-            const int chunk = (s % CH) ^ (CH == 8 ? row & 7 : (row >> 2) & 3);
-            const int r = min(r0 + row, p.rows - 1);
-            copy_to_lds16(p.a + ((long)r * p.groups + g) * ROW + chunk * 16, base + W_BYTES + at * 16);
+        for (int i = 0; i < A_COPIES; ++i)
+            copy_to_lds16(copy_source(ag), G == 1 || second ? a_off[i] : a_off[i] - of_second, base + A_AT + (i * WAVES + wave) * 1024);
+#pragma unroll
+        for (int i = 0; i < S_COPIES; ++i) {
+            const int seg = (i * WAVES + wave) % SEGS;
+            copy_to_lds4(copy_source(sg[i] + (G == 1 ? 0 : seg % G * second) * s_step[i]), s_off[i], base + S_AT + seg * 256);
+        }
+        const long on = next + G < g1 ? G : 0;
+        next += (int)on;
+        wg += on * (p.n * 64L);
+        ag += on * ROW;
+#pragma unroll
+        for (int i = 0; i < S_COPIES; ++i) sg[i] += on * s_step[i];
+    };
+    struct Fragments {
+        i32x4 w[FN], a[FR], b[FR];
+    };
+    auto read = [&](int at, int s, Fragments& f) {      // the s-th 64 of a stage
+        const unsigned char* base = lds + at;
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+            f.w[i] = *reinterpret_cast<const i32x4*>(base + ((2 * s + half) * BN + (wn * FN + i) * 32 + l32) * 16);
+#pragma unroll
+        for (int i = 0; i < FR; ++i) {
+            const int row = (wr * FR + i) * 32 + l32;
+            const unsigned char* rp = base + A_AT + row * 128;
+            if constexpr (FMT == GAN_MX_E4M3) {
+                // the 8-bit operand holds 16 values of each 32-deep quarter: chunks h and 2 + h of the half group
+                f.a[i] = *reinterpret_cast<const i32x4*>(rp + (((4 * s + half) ^ (row & 7)) * 16));
+                f.b[i] = *reinterpret_cast<const i32x4*>(rp + (((4 * s + 2 + half) ^ (row & 7)) * 16));
+            } else {
+                f.a[i] = *reinterpret_cast<const i32x4*>(rp + (((2 * s + half) ^ (row & 7)) * 16));
+            }
         }
     };
-    int sw[FN], sa[FR], nw[FN], na[FR];
-    auto scales = [&](int g, int (&w)[FN], int (&a)[FR]) {
+    unsigned sw[G][FN], sa[G][FR], nw[G][FN], na[G][FR];
+    auto read_scales = [&](int at) {
+        const unsigned* base = reinterpret_cast<const unsigned*>(lds + at + S_AT);
 #pragma unroll
-        for (int f = 0; f < FN; ++f)
-            w[f] = reinterpret_cast<const int*>(p.ws)[(long)g * p.n + min(n0 + (wn * FN + f) * 32 + l32, p.n - 1)];
+        for (int k = 0; k < G; ++k) {
 #pragma unroll
-        for (int f = 0; f < FR; ++f)
-            a[f] = reinterpret_cast<const int*>(p.as)[(long)min(r0 + (wr * FR + f) * 32 + l32, p.rows - 1) * p.groups + g];
+            for (int i = 0; i < FN; ++i) {
+                const int n = (wn * FN + i) * 32 + l32;
+                nw[k][i] = base[(n / 64 * G + k) * 64 + n % 64];
+            }
+#pragma unroll
+            for (int i = 0; i < FR; ++i) {
+                const int r = BN + (wr * FR + i) * 32 + l32;
+                na[k][i] = base[(r / 64 * G + k) * 64 + r % 64];
+            }
+        }
+    };
+    // bytes 0 and 2 become this half's blocks of the two halves of a group.  A group past the end gets scales of 2^-127 on both
+    // sides: no product of 4-bit codes under 2^-254 is above zero.
+    auto shift_scales = [&](int g) {
+#pragma unroll
+        for (int k = 0; k < G; ++k) {
+            const unsigned keep = k == 0 || g + k < g1 ? ~0u : 0u;
+#pragma unroll
+            for (int i = 0; i < FN; ++i) sw[k][i] = (nw[k][i] & keep) >> (8 * half);
+#pragma unroll
+            for (int i = 0; i < FR; ++i) sa[k][i] = (na[k][i] & keep) >> (8 * half);
+        }
     };
 
     f32x16 acc[FN][FR];
@@ -78,75 +167,62 @@ __global__ __launch_bounds__(64 * WN * WR) void mx_tile_kernel(MxProduct p) {
         for (int j = 0; j < FR; ++j)
 #pragma unroll
             for (int k = 0; k < 16; ++k) acc[i][j][k] = 0.f;
-
-    if (g0 < g1) {
-        fill(g0, 0);
-        scales(g0, nw, na);
-    }
-    for (int g = g0; g < g1; ++g) {
-        const int buf = (g - g0) & 1;
-        copies_done_barrier();
-        // bytes 0 and 2 become this half's blocks of the two 64-deep halves of the step
-#pragma unroll
-        for (int f = 0; f < FN; ++f) sw[f] = (int)((unsigned)nw[f] >> (8 * half));
-#pragma unroll
-        for (int f = 0; f < FR; ++f) sa[f] = (int)((unsigned)na[f] >> (8 * half));
-        if (g + 1 < g1) {
-            fill(g + 1, buf ^ 1);
-            scales(g + 1, nw, na);
-        }
-        const unsigned char* lw = lds + buf * STAGE;
-        const unsigned char* la = lw + W_BYTES;
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            i32x8 fw[FN], fa[FR];
-#pragma unroll
-            for (int f = 0; f < FN; ++f) {
-                const i32x4 t = *reinterpret_cast<const i32x4*>(lw + ((2 * s + half) * BN + (wn * FN + f) * 32 + l32) * 16);
-                fw[f] = i32x8{t[0], t[1], t[2], t[3], 0, 0, 0, 0};
-            }
-#pragma unroll
-            for (int f = 0; f < FR; ++f) {
-                const int row = (wr * FR + f) * 32 + l32;
-                const unsigned char* rp = la + row * ROW;
-                if constexpr (FMT == GAN_MX_E4M3) {
-                    // the 8-bit operand holds 16 values of each 32-deep quarter: chunks h and 2 + h of the half step
-                    const i32x4 t = *reinterpret_cast<const i32x4*>(rp + (((4 * s + half) ^ (row & 7)) * 16));
-                    const i32x4 u = *reinterpret_cast<const i32x4*>(rp + (((4 * s + 2 + half) ^ (row & 7)) * 16));
-                    fa[f] = i32x8{t[0], t[1], t[2], t[3], u[0], u[1], u[2], u[3]};
-                } else {
-                    const i32x4 t = *reinterpret_cast<const i32x4*>(rp + (((2 * s + half) ^ ((row >> 2) & 3)) * 16));
-                    fa[f] = i32x8{t[0], t[1], t[2], t[3], 0, 0, 0, 0};
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < FN; ++i)
-#pragma unroll
-                for (int j = 0; j < FR; ++j) {
-                    constexpr int kB = FMT == GAN_MX_E4M3 ? 0 : 4;
-                    acc[i][j] = s == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[i], fa[j], acc[i][j], 4, kB, 0, sw[i], 0, sa[j])
-                                       : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[i], fa[j], acc[i][j], 4, kB, 2, sw[i], 2, sa[j]);
-                }
-        }
-        // (the barrier at the top of the next step is also what lets its copies overwrite the stage read here one step later)
-    }
-    const int n4 = (p.n + 3) / 4 * 4;
-#pragma unroll
-    for (int j = 0; j < FR; ++j) {
-        const int r = r0 + (wr * FR + j) * 32 + l32;
-        if (r >= p.rows) continue;
+    auto multiply = [&](auto part, const Fragments& f) {
+        constexpr int kB = FMT == GAN_MX_E4M3 ? 0 : 4, kSel = decltype(part)::value % 2 * 2, k = decltype(part)::value / 2;
 #pragma unroll
         for (int i = 0; i < FN; ++i)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int n = n0 + (wn * FN + i) * 32 + 8 * q + 4 * half;
-                const f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                if (p.slabs) {
-                    if (n < p.n) *reinterpret_cast<f32x4*>(p.slabs + ((long)blockIdx.y * p.rows + r) * n4 + n) = v;
-                } else {
-                    store4(static_cast<T*>(p.y) + (long)r * p.n, n, p.n, p.vec, v, p.bias, 0);
-                }
+            for (int j = 0; j < FR; ++j) {
+                // (a 4-bit operand is the first four registers)
+                const i32x8 w = __builtin_shufflevector(f.w[i], f.w[i], 0, 1, 2, 3, -1, -1, -1, -1);
+                i32x8 a;
+                if constexpr (FMT == GAN_MX_E4M3) a = __builtin_shufflevector(f.a[j], f.b[j], 0, 1, 2, 3, 4, 5, 6, 7);
+                else a = __builtin_shufflevector(f.a[j], f.a[j], 0, 1, 2, 3, -1, -1, -1, -1);
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, a, acc[i][j], 4, kB, kSel, (int)sw[k][i], kSel, (int)sa[k][j]);
             }
+    };
+
+    constexpr int READS = FN + FR * (FMT == GAN_MX_E4M3 ? 2 : 1);
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s) fill(s * STAGE);
+    landed_barrier<(STAGES - 1) * COPIES>();
+    Fragments f[2];
+    read(0, 0, f[0]);
+    read_scales(0);
+    shift_scales(g0);
+    int at = 0;
+    for (int g = g0; g < g1; g += G) {
+        read(at, 1, f[1]);
+        multiply(std::integral_constant<int, 0>(), f[0]);
+        interleave<FN * FR, READS, 0>();
+        if constexpr (G == 2) {
+            read(at, 2, f[0]);
+            multiply(std::integral_constant<int, 1>(), f[1]);
+            interleave<FN * FR, READS, 0>();
+            read(at, 3, f[1]);
+            multiply(std::integral_constant<int, 2>(), f[0]);
+            interleave<FN * FR, READS, 0>();
+        }
+        landed_barrier<(STAGES - 2) * COPIES>();        // the next stage is there; STAGES - 2 more are on their way
+        const int freed = at;
+        at = at + STAGE == STAGES * STAGE ? 0 : at + STAGE;
+        read(at, 0, f[0]);
+        read_scales(at);
+        fill(freed);
+        multiply(std::integral_constant<int, 2 * G - 1>(), f[1]);
+        shift_scales(g + G);
+        interleave<FN * FR, READS + G * (FN + FR), COPIES>();
+    }
+    landed_barrier<0>();        // (no copy is in flight when the workgroup gives its LDS back)
+    float* stage = reinterpret_cast<float*>(lds) + wave * 32 * (32 * FN + 4);
+    static_assert(WAVES * 32 * (32 * FN + 4) * 4 <= STAGES * STAGE, "the results pass through the stages' LDS");
+    const int n4 = (p.n + 3) / 4 * 4, col0 = n0 + wn * FN * 32;
+#pragma unroll
+    for (int j = 0; j < FR; ++j) {
+        const int row0 = r0 + (wr * FR + j) * 32;
+        auto pick = [&](int i) -> const f32x16& { return acc[i][j]; };
+        if (p.slabs) store_rows<float, FN>(pick, stage, row0, col0, p.rows, n4, p.slabs + (long)blockIdx.y * p.rows * n4, n4, nullptr, 0, true);
+        else store_rows<T, FN>(pick, stage, row0, col0, p.rows, p.n, static_cast<T*>(p.y), p.n, p.bias, 0, p.vec16);
     }
 }
 
@@ -284,15 +360,20 @@ static MxPlan mx_plan(int dtype, int fmt, int rows, int in_dim, int out_dim) {
         return {MX_FEW, s < 1 ? 1 : (int)s};
     }
     if (fmt == GAN_MX_E4M3 && dtype == GAN_F32) return {MX_VIA_BF16, 1};
+    // 256 x 256 tiles where they fill the chip (4096^3 e4m3: 54 us against 69 with 128 x 128; 1024 x 4096 x 4096, 64 tiles: 42
+    // against 22).  A split contraction pays for its slabs only where few small tiles have long contractions (128 x 8192 x 8192:
+    // 32 us whole, 21 in three; 512 x 4096 x 4096, 128 tiles: 20 whole, 23 in two).
     const long large = (long)((rows + 255) / 256) * ((out_dim + 255) / 256);
     if (large >= 192) return {MX_TILE_LARGE, 1};
-    return {MX_TILE_SMALL, contraction_splits((long)((rows + 127) / 128) * ((out_dim + 127) / 128), groups, 4)};
+    return {MX_TILE_SMALL, contraction_splits((long)((rows + 127) / 128) * ((out_dim + 127) / 128), 192, groups, 8)};
 }
 
 template <typename T, int FMT, int BN, int BR, int WN, int WR>
 static int launch_tile(const MxProduct& p, hipStream_t st) {
-    constexpr int LDS = 2 * (BN * 64 + BR * (FMT == GAN_MX_E4M3 ? 128 : 64));
-    auto kernel = mx_tile_kernel<T, FMT, BN, BR, WN, WR>;
+    constexpr int G = FMT == GAN_MX_E4M3 ? 1 : 2, STAGE = BN * 64 * G + BR * 128 + (BN + BR) * 4 * G;
+    // small tiles: two workgroups a CU
+    constexpr int STAGES = STAGE * 3 <= (BN == 256 ? 160 : 80) * 1024 ? 3 : 2, LDS = STAGES * STAGE;
+    auto kernel = mx_tile_kernel<T, FMT, BN, BR, WN, WR, STAGES>;
     static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                       hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
     if (set != hipSuccess) return fail("gan_mx_matmul: %d bytes of LDS refused: %s", LDS, hipGetErrorString(set));
@@ -332,7 +413,7 @@ using namespace gan;
 extern "C" {
 
 size_t gan_mx_matmul_workspace_bytes(int dtype, int fmt, int rows, int in_dim, int out_dim) {
-    if (rows < 1 || rows > GAN_MX_MAX_ROWS || in_dim < 1 || in_dim > GAN_MX_MAX_IN || out_dim < 1 || !dtype_ok(dtype) || !mx_fmt_ok(fmt)) return 0;
+    if (rows < 1 || rows > GAN_MX_MAX_ROWS || in_dim < 1 || in_dim > GAN_MX_MAX_IN || out_dim < 1 || out_dim > GAN_MX_MAX_IN || !dtype_ok(dtype) || !mx_fmt_ok(fmt)) return 0;
     const MxPlan plan = mx_plan(dtype, fmt, rows, in_dim, out_dim);
     if (plan.kind == MX_VIA_BF16)
         return mx_bf16_bytes(rows, in_dim) + mx_bf16_bytes(out_dim, in_dim) +
@@ -359,7 +440,7 @@ static int mx_product(int dtype, int fmt, int rows, int in_dim, int out_dim, con
         MxProduct p{static_cast<const unsigned char*>(a_codes), static_cast<const unsigned char*>(a_scales),
                     static_cast<const unsigned char*>(w_codes), static_cast<const unsigned char*>(w_scales),
                     bias, y, plan.splits > 1 ? static_cast<float*>(ws) : nullptr, rows, out_dim, mx_groups(in_dim), plan.splits, vec,
-                    x, ldx, in_dim, aligned16(x) && ldx * sizeof(T) % 16 == 0};
+                    out_dim * sizeof(T) % 16 == 0 && aligned16(y), x, ldx, in_dim, aligned16(x) && ldx * sizeof(T) % 16 == 0};
         int rc;
         if (plan.kind == MX_FEW) rc = fmt == GAN_MX_E4M3 ? launch_few<T, GAN_MX_E4M3>(p, st) : launch_few<T, GAN_MX_E2M1>(p, st);
         else if (plan.kind == MX_TILE_LARGE)
@@ -376,8 +457,8 @@ int gan_mx_matmul(int dtype, int fmt, int rows, int in_dim, int out_dim, const v
                   const void* w_codes, const void* w_scales, const float* bias, void* y, void* ws, size_t ws_bytes,
                   gan_stream_t stream) {
     GAN_CHECK_ARG(dtype_ok(dtype) && mx_fmt_ok(fmt), "gan_mx_matmul: unknown element type %d or format %d", dtype, fmt);
-    GAN_CHECK_ARG(rows >= 0 && rows <= GAN_MX_MAX_ROWS && in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1,
-                  "gan_mx_matmul: %d rows, %d inputs, %d outputs (up to %d rows and inputs are served)", rows, in_dim, out_dim, GAN_MX_MAX_IN);
+    GAN_CHECK_ARG(rows >= 0 && rows <= GAN_MX_MAX_ROWS && in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1 && out_dim <= GAN_MX_MAX_IN,
+                  "gan_mx_matmul: %d rows, %d inputs, %d outputs (up to %d of each are served)", rows, in_dim, out_dim, GAN_MX_MAX_IN);
     if (rows == 0) return 0;
     GAN_CHECK_ARG(a_codes && a_scales && w_codes && w_scales && y, "gan_mx_matmul: null pointer");
     GAN_CHECK_ARG(aligned16(a_codes) && aligned16(w_codes) && ((reinterpret_cast<size_t>(a_scales) | reinterpret_cast<size_t>(w_scales)) & 3) == 0,
@@ -394,7 +475,7 @@ static size_t mx_codes_bytes(int fmt, int rows, int in_dim) { return (size_t)row
 static size_t mx_scales_bytes(int rows, int in_dim) { return ((size_t)rows * mx_groups(in_dim) * 4 + 15) / 16 * 16; }
 
 size_t gan_mx_linear_workspace_bytes(int dtype, int fmt, int rows, int in_dim, int out_dim) {
-    if (rows < 1 || rows > GAN_MX_MAX_ROWS || in_dim < 1 || in_dim > GAN_MX_MAX_IN || out_dim < 1 || !dtype_ok(dtype) || !mx_fmt_ok(fmt))
+    if (rows < 1 || rows > GAN_MX_MAX_ROWS || in_dim < 1 || in_dim > GAN_MX_MAX_IN || out_dim < 1 || out_dim > GAN_MX_MAX_IN || !dtype_ok(dtype) || !mx_fmt_ok(fmt))
         return 0;
     const size_t own = gan_mx_matmul_workspace_bytes(dtype, fmt, rows, in_dim, out_dim);
     if (mx_fused(mx_plan(dtype, fmt, rows, in_dim, out_dim), rows, in_dim)) return own;
@@ -404,8 +485,8 @@ size_t gan_mx_linear_workspace_bytes(int dtype, int fmt, int rows, int in_dim, i
 int gan_mx_linear(int dtype, int fmt, int rows, int in_dim, int out_dim, const void* x, long ldx, const void* w_codes,
                   const void* w_scales, const float* bias, void* y, void* ws, size_t ws_bytes, gan_stream_t stream) {
     GAN_CHECK_ARG(dtype_ok(dtype) && mx_fmt_ok(fmt), "gan_mx_linear: unknown element type %d or format %d", dtype, fmt);
-    GAN_CHECK_ARG(rows >= 0 && rows <= GAN_MX_MAX_ROWS && in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1 && ldx >= in_dim,
-                  "gan_mx_linear: %d rows of stride %ld, %d inputs, %d outputs (up to %d rows and inputs are served)", rows, ldx, in_dim,
+    GAN_CHECK_ARG(rows >= 0 && rows <= GAN_MX_MAX_ROWS && in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1 && out_dim <= GAN_MX_MAX_IN && ldx >= in_dim,
+                  "gan_mx_linear: %d rows of stride %ld, %d inputs, %d outputs (up to %d of each are served)", rows, ldx, in_dim,
                   out_dim, GAN_MX_MAX_IN);
     if (rows == 0) return 0;
     GAN_CHECK_ARG(x && w_codes && w_scales && y, "gan_mx_linear: null pointer");
