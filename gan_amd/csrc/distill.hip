@@ -10,8 +10,7 @@
 // threads hold the row in 16-byte chunks of the tensor's type; maximum and sum of exponentials come from two passes over the
 // registers, joined over the workgroup in one exchange; a third pass writes the gradient.
 // q_r is never 1 - sum q_i, which cancels: a bit per class marks the list, and sums over the marked and the unmarked classes
-// are taken apart.  The same bits tell whether a class is listed twice (its probabilities add up), and which values the chunks
-// leave to the first wave, which writes the listed classes: nobody waits for another's stores.
+// are taken apart.  The same bits tell whether a class is listed twice (its probabilities add up).
 // Statistics are fp32 in an order fixed by the thread number, so results are deterministic.
 #include "mx.h"
 
@@ -35,17 +34,6 @@ __device__ __forceinline__ float teacher_at(const Distill& p, long i) {
     if (p.teacher_dtype == GAN_F32) return static_cast<const float*>(p.teacher)[i];
     if (p.teacher_dtype == GAN_BF16) return (float)static_cast<const bf16_t*>(p.teacher)[i];
     return (float)static_cast<const f16_t*>(p.teacher)[i];
-}
-
-__device__ __forceinline__ float wave_all_sum(float v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-    return v;
-}
-__device__ __forceinline__ float wave_all_max(float v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
-    return v;
 }
 
 // e^((x - m) / tau) as 2^((x - m) c2), c2 = log2(e) / tau, with -inf as the maximum of nothing: of -inf and -inf it is 0 here.
@@ -85,11 +73,16 @@ __device__ __forceinline__ void unpack(const i32x4& r, float (&v)[8], f16_t) {
 template <typename T>
 __device__ __forceinline__ void strike(i32x4& r, unsigned marked) {
     constexpr int n = Chunk<T>::n;
+    if constexpr (n == 4) {
 #pragma unroll
-    for (int j = 0; j < n; ++j) {
-        if (!(marked >> j & 1)) continue;
-        if (n == 4) r[j] = 0xff800000;
-        else r[j / 2] = (r[j / 2] & (j & 1 ? 0x0000ffff : 0xffff0000)) | (std::is_same<T, bf16_t>::value ? 0xff80u : 0xfc00u) << (16 * (j & 1));
+        for (int j = 0; j < 4; ++j) r[j] = marked >> j & 1 ? 0xff800000 : r[j];
+    } else {
+        constexpr unsigned low = std::is_same<T, bf16_t>::value ? 0xff80u : 0xfc00u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const unsigned m = (marked >> (2 * j) & 1) * 0xffffu | (marked >> (2 * j + 1) & 1) * 0xffff0000u;
+            r[j] = (int)(((unsigned)r[j] & ~m) | (low * 0x10001u & m));
+        }
     }
 }
 
@@ -104,14 +97,16 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
     return v;
 }
 
-// NV chunks a thread in registers; NV = 0: the row does not fit and is read twice.
+// NV chunks a thread in registers; what a row has beyond them is read twice.
 template <typename T, int NT, int NV, bool REST>
 __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
     constexpr int N = Chunk<T>::n;
+    constexpr bool kKeep = sizeof(T) == 4;      // a power takes the place of its value, and is not computed twice
     extern __shared__ __align__(16) unsigned char lds[];
     __shared__ float red[2 * NT / 64];
-    // of the list: any, P, p_r, maximum, sum of powers, repeated classes; sum of the weights
-    __shared__ float told[7];
+    // of the list: any, P, p_r, maximum, sum of powers, repeated classes
+    __shared__ float told[6];
+    __shared__ float wsum[NT / 64];
     const int tid = threadIdx.x, lane = tid & 63, classes = p.classes;
     const long row = blockIdx.x;
     const T* x = static_cast<const T*>(p.logits) + row * p.ld;
@@ -132,9 +127,9 @@ __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
         const int at = chunk * N + 8;
         return bits[at >> 5] >> (at & 31) & ((1u << N) - 1);
     };
-    auto store = [&](int chunk, unsigned skip, const float (&g)[N]) {
+    auto store = [&](int chunk, const float (&g)[N]) {
         T* to = gr + head + chunk * N;
-        if (gvec && skip == 0) {
+        if (gvec) {
             typedef T vec __attribute__((ext_vector_type(N)));
             vec r;
 #pragma unroll
@@ -142,8 +137,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
             *reinterpret_cast<vec*>(to) = r;
         } else {
 #pragma unroll
-            for (int j = 0; j < N; ++j)
-                if (!(skip >> j & 1)) to[j] = (T)g[j];
+            for (int j = 0; j < N; ++j) to[j] = (T)g[j];
         }
     };
 
@@ -215,7 +209,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
             told[5] = twice ? 1.f : 0.f;
         }
     }
-    i32x4 raw[NV > 0 ? NV : 1];
+    i32x4 raw[NV];
     float lone = -INFINITY;         // the thread's loose value
     if (w != 0.f) {
 #pragma unroll
@@ -230,34 +224,43 @@ __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
         }
         if (loose >= 0) lone = (float)x[loose];
     }
-    if (p.weight && tid >= 64 && tid < 128) {
+    if (p.weight && !p.total) {
         float s = 0.f;
-        if (p.total) s = p.total[0];
-        else {
-            for (long i = lane; i < p.rows; i += 64) s += p.weight[i];
-            s = wave_all_sum(s);
-        }
-        if (lane == 0) told[6] = s;
+#pragma unroll 4
+        for (int i = tid; i < (int)p.rows; i += NT) s += p.weight[i];
+        s = wave_all_sum(s);
+        if (lane == 0) wsum[tid >> 6] = s;
     }
     __syncthreads();
     if (w == 0.f || told[0] == 0.f) {       // nothing to learn in this row
         if (p.grad) {
             const float zero[N] = {};
-            for (int c = tid; c < chunks; c += NT) store(c, 0, zero);
+            for (int c = tid; c < chunks; c += NT) store(c, zero);
             if (loose >= 0) gr[loose] = (T)0.f;
         }
         if (tid == 0) p.row_loss[row] = 0.f;
         return;
     }
-    const float total = p.weight ? told[6] : (float)p.rows;
+    float total = (float)p.rows;
+    if (p.weight) {
+        if (p.total) {
+            total = p.total[0];
+        } else {
+            total = 0.f;
+#pragma unroll
+            for (int i = 0; i < NT / 64; ++i) total += wsum[i];
+        }
+    }
     const bool lone_listed = loose >= 0 && (bits[(loose - head + 8) >> 5] >> ((loose - head + 8) & 31) & 1);
     if (REST && lone_listed) lone = -INFINITY;
 
     // maximum and sum of powers of the unlisted classes (REST) or of all
-    float m = lone, s = 0.f;
-    if (NV > 0) {
+    const int wave0 = __builtin_amdgcn_readfirstlane(tid & ~63);     // (chunks past the end of the row are skipped by whole waves)
+    float m = lone, s = 0.f, own;
+    {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
+            if (i * NT + wave0 >= chunks) continue;
             if (REST && i * NT + tid < chunks) {
                 const unsigned marked = marks(i * NT + tid);
                 if (marked) strike<T>(raw[i], marked);
@@ -268,18 +271,22 @@ __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
             for (int j = 0; j < N; ++j) m = fmaxf(m, v[j]);
         }
         const float off = m == -INFINITY ? 0.f : m;
+        own = off;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
+            if (i * NT + wave0 >= chunks) continue;
             asm volatile("" : "+v"(raw[i]));        // unpack again here: keeping every pass's values costs more registers than there are
             float v[N];
             unpack(raw[i], v, T());
 #pragma unroll
-            for (int j = 0; j < N; ++j) s += __builtin_amdgcn_exp2f((v[j] - off) * c2);
+            for (int j = 0; j < N; ++j) {
+                v[j] = __builtin_amdgcn_exp2f((v[j] - off) * c2);
+                s += v[j];
+                if constexpr (kKeep) raw[i][j] = __float_as_int(v[j]);
+            }
         }
         s += __builtin_amdgcn_exp2f((lone - off) * c2);
-    } else {
-        s = power(lone, lone, c2);
-        for (int c = tid; c < chunks; c += NT) {
+        for (int c = NV * NT + tid; c < chunks; c += NT) {
             i32x4 r = *reinterpret_cast<const i32x4*>(x + head + c * N);
             if (REST) {
                 const unsigned marked = marks(c);
@@ -303,9 +310,10 @@ __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
             red[2 * (tid >> 6) + 1] = s;
         }
         __syncthreads();
-        m = red[0];
-        s = red[1];
-        for (int i = 1; i < NT / 64; ++i) join_stats(m, s, red[2 * i], red[2 * i + 1], c2);
+        const float mi = lane < NT / 64 ? red[2 * (lane & (NT / 64 - 1))] : -INFINITY;
+        const float si = lane < NT / 64 ? red[2 * (lane & (NT / 64 - 1)) + 1] : 0.f;
+        m = wave_all_max(mi);
+        s = wave_all_sum(si * power(mi, m, c2));
     }
     const float P = told[1], rest = told[2];
     float mall = m, sall = s;
@@ -317,23 +325,33 @@ __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
         // e^((x - m) / tau) times one factor for every class that is not listed
         const float f = gs * (REST ? P * power(m, mall, c2) / sall - (there ? rest / s : 0.f) : P / s);
         const float off = m == -INFINITY ? 0.f : m;
+        const float f_own = f * power(own, m, c2);      // (of a kept power, which goes by the thread's own maximum)
         auto gradient = [&](int chunk, const i32x4& r) {
             float v[N];
             unpack(r, v, T());
 #pragma unroll
             for (int j = 0; j < N; ++j) v[j] = __builtin_amdgcn_exp2f((v[j] - off) * c2) * f;
-            store(chunk, marks(chunk), v);
+            store(chunk, v);
         };
-        if (NV > 0) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                asm volatile("" : "+v"(raw[i]));
-                if (i * NT + tid < chunks) gradient(i * NT + tid, raw[i]);
+        for (int i = 0; i < NV; ++i) {
+            if (i * NT + wave0 >= chunks) continue;
+            asm volatile("" : "+v"(raw[i]));
+            const int chunk = i * NT + tid;
+            if (chunk >= chunks) continue;
+            if constexpr (kKeep) {
+                float v[N];
+                unpack(raw[i], v, T());
+#pragma unroll
+                for (int j = 0; j < N; ++j) v[j] *= f_own;
+                store(chunk, v);
+            } else {
+                gradient(chunk, raw[i]);
             }
-        } else {
-            for (int c = tid; c < chunks; c += NT) gradient(c, *reinterpret_cast<const i32x4*>(x + head + c * N));
         }
-        if (loose >= 0 && !lone_listed) gr[loose] = (T)(__builtin_amdgcn_exp2f((lone - off) * c2) * f);
+        for (int c = NV * NT + tid; c < chunks; c += NT) gradient(c, *reinterpret_cast<const i32x4*>(x + head + c * N));
+        if (loose >= 0) gr[loose] = (T)(__builtin_amdgcn_exp2f((lone - off) * c2) * f);
+        __syncthreads();        // (waits for the stores: the listed classes are written once more)
     }
     if (tid < 64) {
         const bool twice = told[5] != 0.f;
@@ -431,14 +449,16 @@ int gan_distill_topk_mean(int dtype, long rows, int classes, const void* logits,
     const int rc = with_dtype(dtype, [&](auto* tag) {
         typedef typename std::remove_pointer<decltype(tag)>::type T;
         const int chunks = classes / Chunk<T>::n;
+        // What is in flight on a CU counts, not only that nothing is read twice: of 131072 bf16 classes (16384 chunks) 2048 rows
+        // take 249 us with half of a row in registers and 262 with all of it, of 32000 (4000 chunks) 4096 rows 124 us with 512
+        // threads, 143 with 1024, 134 with 256 x 16 chunks.  Few rows want every thread: 256 rows of 131072 41 us against 46.
         if (chunks <= 256) return launch_distill<T, 256, 1>(p, st);
         if (chunks <= 512) return launch_distill<T, 256, 2>(p, st);
         if (chunks <= 1024) return launch_distill<T, 256, 4>(p, st);
-        if (chunks <= 2048) return launch_distill<T, 512, 4>(p, st);
-        if (chunks <= 4096) return launch_distill<T, 1024, 4>(p, st);
-        if (chunks <= 8192) return launch_distill<T, 1024, 8>(p, st);
-        if (chunks <= 16384) return launch_distill<T, 1024, 16>(p, st);     // 64 of the 128 registers a thread has
-        return launch_distill<T, 1024, 0>(p, st);
+        if (chunks <= 2048) return launch_distill<T, 256, 8>(p, st);
+        if (chunks <= 4096) return launch_distill<T, 512, 8>(p, st);
+        if (chunks <= 8192 || (chunks <= 16384 && rows > 512)) return launch_distill<T, 1024, 8>(p, st);
+        return launch_distill<T, 1024, 16>(p, st);
     });
     if (rc) return rc;
     hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(1024), 0, st, row_loss, row_weight, rows, weight * temperature * temperature,

@@ -66,6 +66,43 @@ __device__ __forceinline__ void store8(T* __restrict__ row, int i0, int c, bool 
     }
 }
 
+// Reductions over the 64 lanes of a wave, the result in all of them: four steps inside the rows of 16 lanes as operand swizzles
+// (neighbour, pair, mirrored half row, mirrored row), then the four rows by scalar reads.  No trip through LDS.
+template <int CTRL>
+__device__ __forceinline__ float row_swizzle(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <int CTRL>
+__device__ __forceinline__ double row_swizzle(double v) {
+    const long u = __builtin_bit_cast(long, v);
+    const unsigned lo = (unsigned)__builtin_amdgcn_mov_dpp((int)u, CTRL, 0xf, 0xf, true);
+    const unsigned hi = (unsigned)__builtin_amdgcn_mov_dpp((int)(u >> 32), CTRL, 0xf, 0xf, true);
+    return __builtin_bit_cast(double, (unsigned long)hi << 32 | lo);
+}
+__device__ __forceinline__ float from_lane(float v, int lane) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+__device__ __forceinline__ double from_lane(double v, int lane) {
+    const long u = __builtin_bit_cast(long, v);
+    const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)u, lane), hi = (unsigned)__builtin_amdgcn_readlane((int)(u >> 32), lane);
+    return __builtin_bit_cast(double, (unsigned long)hi << 32 | lo);
+}
+template <typename S>
+__device__ __forceinline__ S wave_all_sum(S v) {
+    v += row_swizzle<0xb1>(v);
+    v += row_swizzle<0x4e>(v);
+    v += row_swizzle<0x141>(v);
+    v += row_swizzle<0x140>(v);
+    return (from_lane(v, 0) + from_lane(v, 16)) + (from_lane(v, 32) + from_lane(v, 48));
+}
+__device__ __forceinline__ float wave_all_max(float v) {
+    v = fmaxf(v, row_swizzle<0xb1>(v));
+    v = fmaxf(v, row_swizzle<0x4e>(v));
+    v = fmaxf(v, row_swizzle<0x141>(v));
+    v = fmaxf(v, row_swizzle<0x140>(v));
+    return fmaxf(fmaxf(from_lane(v, 0), from_lane(v, 16)), fmaxf(from_lane(v, 32), from_lane(v, 48)));
+}
+
 // |x| as an ordered integer: NaN > infinity > every number, so the maximum over a block tells all three apart.
 __device__ __forceinline__ unsigned mag_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
@@ -134,8 +171,8 @@ __device__ __forceinline__ unsigned mx_quantize_lane8(const float (&v)[8], unsig
     unsigned a = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) a = max(a, mag_bits(v[j]));
-    a = max(a, (unsigned)__shfl_xor((int)a, 1, 64));
-    a = max(a, (unsigned)__shfl_xor((int)a, 2, 64));
+    a = max(a, (unsigned)__builtin_amdgcn_mov_dpp((int)a, 0xb1, 0xf, 0xf, true));
+    a = max(a, (unsigned)__builtin_amdgcn_mov_dpp((int)a, 0x4e, 0xf, 0xf, true));
     const unsigned byte = mx_scale_byte<FMT>(a);
     const float inv = mx_inverse_scale(byte);
     float s[8];

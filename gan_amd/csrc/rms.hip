@@ -16,8 +16,7 @@ namespace gan {
 
 template <typename S>
 __device__ __forceinline__ S team_sum(S v, int tpr, S* red) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    v = wave_all_sum(v);
     if (tpr > 64) {
         const int wave = threadIdx.x >> 6, waves = tpr >> 6;
         __syncthreads();
