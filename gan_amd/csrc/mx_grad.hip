@@ -126,18 +126,20 @@ __global__ __launch_bounds__(64 * WI * WJ) void bf16_product_kernel(Bf16Product 
     }
 }
 
+enum { BF16_128, BF16_256_128, BF16_256 };      // tiles
 struct Bf16Plan {
-    bool large;
-    int splits;
+    int tile, splits;
 };
 static Bf16Plan bf16_plan(int rows, int cols, int parts, int depth) {
     // 256 x 256 tiles where they fill the chip, alone (4096^3: 115 us against 132) or in parts of 32 stages or more
     // (1024 x 1024 <- 32768: 98 us in 16 parts against 110 with small tiles in 6; 1024 x 4096 <- 4096, parts of 16: 58 against 53)
     const long large = (long)((rows + 255) / 256) * ((cols + 255) / 256), all = (long)parts * (depth / 64);
     const int steps = (int)(all < (1 << 30) ? all : 1 << 30);
-    if (large >= 192) return {true, 1};
-    if (steps / (256 / large) >= 32) return {true, (int)(256 / large)};
-    return {false, contraction_splits((long)((rows + 127) / 128) * ((cols + 127) / 128), 384, steps, 8)};
+    if (large >= 192) return {BF16_256, 1};
+    // (4096 x 2048 <- 8192: 125 us, 133 in two parts of 256 x 256 tiles)
+    if ((long)((rows + 255) / 256) * ((cols + 127) / 128) >= 192) return {BF16_256_128, 1};
+    if (steps / (256 / large) >= 32) return {BF16_256, (int)(256 / large)};
+    return {BF16_128, contraction_splits((long)((rows + 127) / 128) * ((cols + 127) / 128), 384, steps, 8)};
 }
 
 size_t bf16_product_workspace(int rows, int cols, int parts, int depth) {
@@ -146,7 +148,8 @@ size_t bf16_product_workspace(int rows, int cols, int parts, int depth) {
 
 template <typename T, int BI, int BJ, int WI, int WJ>
 static int launch_bf16(const Bf16Product& p, T* out, float* slabs, int splits, bool vec, hipStream_t st, const char* what) {
-    constexpr int STAGES = 2, LDS = STAGES * (BI + BJ) * 128;       // (small tiles: two workgroups a CU)
+    // 128 x 128: two workgroups a CU
+    constexpr int STAGES = BI + BJ == 384 ? 3 : 2, LDS = STAGES * (BI + BJ) * 128;
     auto kernel = bf16_product_kernel<T, BI, BJ, WI, WJ, STAGES>;
     static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                       hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
@@ -161,8 +164,9 @@ int bf16_product(const Bf16Product& p, T* out, void* ws, hipStream_t st, const c
     const Bf16Plan plan = bf16_plan(p.rows, p.cols, p.parts, p.depth);
     const bool vec = p.cols * sizeof(T) % 16 == 0 && aligned16(out), vec4 = vec && aligned16(p.bias);
     float* slabs = plan.splits > 1 ? static_cast<float*>(ws) : nullptr;
-    const int rc = plan.large ? launch_bf16<T, 256, 256, 2, 4>(p, out, slabs, plan.splits, vec, st, what)
-                              : launch_bf16<T, 128, 128, 2, 2>(p, out, slabs, plan.splits, vec, st, what);
+    const int rc = plan.tile == BF16_256       ? launch_bf16<T, 256, 256, 2, 4>(p, out, slabs, plan.splits, vec, st, what)
+                   : plan.tile == BF16_256_128 ? launch_bf16<T, 256, 128, 4, 2>(p, out, slabs, plan.splits, vec, st, what)
+                                               : launch_bf16<T, 128, 128, 2, 2>(p, out, slabs, plan.splits, vec, st, what);
     if (rc) return rc;
     if (slabs) join_slabs(slabs, plan.splits, out, (long)p.rows, p.cols, p.bias, p.accumulate, vec4, st);
     return check_launch(what);

@@ -818,6 +818,31 @@ def _dense16(t):
     return t.clone() if t.data_ptr() & 15 else t
 
 
+def _plain(t):
+    """t dense and outside of autograd."""
+    if t is None or (not t.requires_grad and t.is_contiguous()):
+        return t
+    return t.detach().contiguous()
+
+
+def _variable(st, scope, leaf, shape, initializer):
+    """The variable `scope`/`leaf` under the current scope; one that is there already without entering the scope."""
+    var = st.vars.get('/'.join(st._scope + [scope, leaf]))
+    if var is not None and var.shape == shape:
+        return var
+    with st.variable_scope(scope):
+        return st.get_variable(leaf, shape, initializer)
+
+
+def _size(query, *args):
+    """A workspace query of the library, asked once per shape."""
+    key = (query.__name__,) + args
+    n = _ws_cache.get(key)
+    if n is None:
+        n = _ws_cache[key] = int(query(*args))
+    return n
+
+
 def _rms_fwd(x, residual, gamma, eps, mx, want_rstd):
     """(y or MxTensor, h or None, rstd or None, the stream's tensor and row stride)"""
     code = _lib.dtype_code(x.dtype)
@@ -826,9 +851,9 @@ def _rms_fwd(x, residual, gamma, eps, mx, want_rstd):
     rs, ldr, h = None, 0, None
     if residual is not None:
         rs, _, _, ldr = _rows_of(residual)
-        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        h = x.new_empty(x.shape)
     rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if want_rstd else None
-    out = _mx_empty(x.shape, 'e4m3', x.dtype, x.device) if mx else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = _mx_empty(x.shape, 'e4m3', x.dtype, x.device) if mx else x.new_empty(x.shape)
     check(lib.gan_rms_norm_fwd(code, rows, c, xs.data_ptr(), ldx, None if rs is None else rs.data_ptr(), ldr, ptr(gamma.data), eps,
                                None if h is None else h.data_ptr(), None if mx else out.data_ptr(),
                                out.codes.data_ptr() if mx else None, out.scales.data_ptr() if mx else None, ptr(rstd), stream()))
@@ -860,11 +885,11 @@ class _RmsNormFn(torch.autograd.Function):
             rows = rstd.numel()
             dy = dy.contiguous()
             dh = None if dh is None or not want else dh.contiguous()
-            dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device) if want else None
+            dx = dy.new_empty(dy.shape) if want else None
             dg, acc, wp, wn, hold = None, 0, None, 0, None
             if gamma.wants_grad:
                 dg, acc = gamma.grad_target()
-                wp, wn, hold = _lib.scratch(lib.gan_rms_norm_workspace_bytes(rows, c), dy.device)
+                wp, wn, hold = _lib.scratch(_size(lib.gan_rms_norm_workspace_bytes, rows, c), dy.device)
             if dx is not None or dg is not None:
                 check(lib.gan_rms_norm_bwd(_lib.dtype_code(dy.dtype), rows, c, kept.data_ptr(), ctx.ld, ptr(gamma.data), ptr(rstd),
                                            dy.data_ptr(), None if dh is None else dh.data_ptr(),
@@ -885,8 +910,7 @@ def rms_norm(x, name="rms_norm", epsilon=1e-6, residual=None, mx=False):
     _lib.dtype_code(x.dtype)
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError("rms_norm: residual %s %s does not match x %s %s" % (tuple(residual.shape), residual.dtype, tuple(x.shape), x.dtype))
-    with st.variable_scope(name):
-        gamma = st.get_variable('gamma', [x.shape[-1]], V.constant_initializer(1.0))
+    gamma = _variable(st, name, 'gamma', (x.shape[-1],), V.constant_initializer(1.0))
     eps, mx = float(epsilon), bool(mx)
     token = _grad_token(x.device, gamma) if torch.is_grad_enabled() else None
     if token is None and not (torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad))):
@@ -1031,7 +1055,7 @@ def _mx_product(q, w, bias):
     lead = tuple(q.codes.shape[:-1])
     y = torch.empty(lead + (w.out_dim,), dtype=q.dtype, device=q.codes.device)
     rows = y.numel() // w.out_dim
-    wp, wn, hold = _lib.scratch(lib.gan_mx_matmul_workspace_bytes(code, fmt, rows, w.in_dim, w.out_dim), y.device)
+    wp, wn, hold = _lib.scratch(_size(lib.gan_mx_matmul_workspace_bytes, code, fmt, rows, w.in_dim, w.out_dim), y.device)
     check(lib.gan_mx_matmul(code, fmt, rows, w.in_dim, w.out_dim, q.codes.data_ptr(), q.scales.data_ptr(), w.codes.data_ptr(),
                             w.scales.data_ptr(), ptr(bias), y.data_ptr(), wp, wn, stream()))
     return y
@@ -1041,9 +1065,9 @@ def _mx_linear(x, w, bias, fmt):
     """The same from floats, in one call."""
     _lib.here(x, w.codes, w.scales, bias)
     code, f = _lib.dtype_code(x.dtype), _lib.MX_FORMATS[fmt]
-    y = torch.empty(tuple(x.shape[:-1]) + (w.out_dim,), dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape[:-1] + (w.out_dim,))
     xs, rows, k, ld = _rows_of(x)
-    wp, wn, hold = _lib.scratch(lib.gan_mx_linear_workspace_bytes(code, f, rows, k, w.out_dim), x.device)
+    wp, wn, hold = _lib.scratch(_size(lib.gan_mx_linear_workspace_bytes, code, f, rows, k, w.out_dim), x.device)
     check(lib.gan_mx_linear(code, f, rows, k, w.out_dim, xs.data_ptr(), ld, w.codes.data_ptr(), w.scales.data_ptr(), ptr(bias),
                             y.data_ptr(), wp, wn, stream()))
     return y
@@ -1073,13 +1097,13 @@ class _MxMatmulFn(torch.autograd.Function):
             dm, acc = ctx.matrix.grad_target()
             db, accb = ctx.bias.grad_target()
             assert acc == accb
-            wp, wn, hold = _lib.scratch(lib.gan_mx_matmul_wgrad_workspace_bytes(code, rows, in_dim, out_dim), dy.device)
+            wp, wn, hold = _lib.scratch(_size(lib.gan_mx_matmul_wgrad_workspace_bytes, code, rows, in_dim, out_dim), dy.device)
             check(lib.gan_mx_matmul_wgrad(code, _lib.MX_FORMATS[ctx.q[0]], rows, in_dim, out_dim, ac.data_ptr(), asc.data_ptr(),
                                           dy.data_ptr(), ptr(dm), ptr(db), acc, wp, wn, stream()))
         dx = None
         if ctx.needs_input_grad[0]:
             dx = torch.empty(tuple(dy.shape[:-1]) + (in_dim,), dtype=dy.dtype, device=dy.device)
-            wp, wn, hold = _lib.scratch(lib.gan_mx_matmul_dgrad_workspace_bytes(code, rows, in_dim, out_dim), dy.device)
+            wp, wn, hold = _lib.scratch(_size(lib.gan_mx_matmul_dgrad_workspace_bytes, code, rows, in_dim, out_dim), dy.device)
             check(lib.gan_mx_matmul_dgrad(code, rows, in_dim, out_dim, dy.data_ptr(), wc.data_ptr(), wsc.data_ptr(), dx.data_ptr(),
                                           wp, wn, stream()))
         return (dx,) + (None,) * 7
@@ -1402,8 +1426,8 @@ class _DistillFn(torch.autograd.Function):
         x, rows, classes, ld = _rows_of(logits)
         dev = x.device
         loss = torch.empty(1, dtype=torch.float32, device=dev)
-        grad = torch.empty(logits.shape, dtype=x.dtype, device=dev) if ctx.needs_input_grad[0] else None
-        wp, wn, hold = _lib.scratch(lib.gan_distill_topk_workspace_bytes(rows), dev)
+        grad = x.new_empty(logits.shape) if ctx.needs_input_grad[0] else None
+        wp, wn, hold = _lib.scratch(_size(lib.gan_distill_topk_workspace_bytes, rows), dev)
         check(lib.gan_distill_topk_mean(_lib.dtype_code(x.dtype), rows, classes, x.data_ptr(), ld, _lib.dtype_code(teacher.dtype),
                                         teacher.data_ptr(), index.data_ptr(), index.element_size(), teacher.shape[-1], ptr(lse),
                                         ptr(row_weight), tau, weight, 0, ptr(loss), None if grad is None else grad.data_ptr(), wp, wn,
@@ -1443,8 +1467,7 @@ def distill_topk_mean(logits, teacher_logits, teacher_index, temperature=1.0, we
             raise ValueError("distill_topk_mean: %s %s %s for rows %s (float32 expected)" % (what, tuple(t.shape), t.dtype, lead))
     if not 0.0 < float(temperature) < float('inf'):
         raise ValueError("distill_topk_mean: temperature %r" % (temperature,))
-    dense = lambda t: None if t is None else t.detach().contiguous()
-    return _DistillFn.apply(logits, dense(teacher_logits), dense(teacher_index), dense(teacher_lse), dense(row_weight),
+    return _DistillFn.apply(logits, _plain(teacher_logits), _plain(teacher_index), _plain(teacher_lse), _plain(row_weight),
                             float(temperature), float(weight))
 
 
