@@ -171,7 +171,6 @@ def ptr(t):
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # GAN_F32 / GAN_BF16 / GAN_F16
 MX_FORMATS = {'e4m3': 0, 'e2m1': 1}                                   # GAN_MX_E4M3 / GAN_MX_E2M1
-MX_MAX_IN = 1 << 22
 
 
 def dtype_code(dtype):

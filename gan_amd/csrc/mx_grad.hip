@@ -409,7 +409,7 @@ int gan_mx_matmul_dgrad(int dtype, int rows, int in_dim, int out_dim, const void
                         void* dx, void* ws, size_t ws_bytes, gan_stream_t stream) {
     GAN_CHECK_ARG(dtype_ok(dtype), "gan_mx_matmul_dgrad: unknown element type %d", dtype);
     GAN_CHECK_ARG(rows >= 0 && rows <= GAN_MX_MAX_ROWS && in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1 && out_dim <= GAN_MX_MAX_IN,
-                  "gan_mx_matmul_dgrad: %d rows, %d inputs, %d outputs (up to %d of each are served)", rows, in_dim, out_dim, GAN_MX_MAX_IN);
+                  "gan_mx_matmul_dgrad: %d rows, %d inputs, %d outputs (up to %d rows and %d of the others are served)", rows, in_dim, out_dim, GAN_MX_MAX_ROWS, GAN_MX_MAX_IN);
     if (rows == 0) return 0;
     GAN_CHECK_ARG(dy && w_codes && w_scales && dx, "gan_mx_matmul_dgrad: null pointer");
     GAN_CHECK_ARG(aligned16(dy) && aligned16(w_codes) && (reinterpret_cast<size_t>(w_scales) & 3) == 0,
@@ -451,7 +451,7 @@ int gan_mx_matmul_wgrad(int dtype, int fmt, int rows, int in_dim, int out_dim, c
                         gan_stream_t stream) {
     GAN_CHECK_ARG(dtype_ok(dtype) && mx_fmt_ok(fmt), "gan_mx_matmul_wgrad: unknown element type %d or format %d", dtype, fmt);
     GAN_CHECK_ARG(rows >= 1 && rows <= GAN_MX_MAX_ROWS && in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1 && out_dim <= GAN_MX_MAX_IN,
-                  "gan_mx_matmul_wgrad: %d rows, %d inputs, %d outputs (up to %d of each are served)", rows, in_dim, out_dim, GAN_MX_MAX_IN);
+                  "gan_mx_matmul_wgrad: %d rows, %d inputs, %d outputs (up to %d rows and %d of the others are served)", rows, in_dim, out_dim, GAN_MX_MAX_ROWS, GAN_MX_MAX_IN);
     GAN_CHECK_ARG(dy && a_codes && a_scales && dmatrix, "gan_mx_matmul_wgrad: null pointer");
     GAN_CHECK_ARG(aligned16(dy) && aligned16(a_codes), "gan_mx_matmul_wgrad: dy and codes have to be 16-byte aligned");
     const size_t need = gan_mx_matmul_wgrad_workspace_bytes(dtype, rows, in_dim, out_dim);

@@ -348,24 +348,33 @@ struct MxPlan {
     int kind, splits;
 };
 
-constexpr int kFewRows = 64;
-
 static MxPlan mx_plan(int dtype, int fmt, int rows, int in_dim, int out_dim) {
     const int groups = mx_groups(in_dim);
-    if (rows <= kFewRows) {
-        const long wgs = (long)((out_dim + 15) / 16) * ((rows + 31) / 32);
+    // The few-row kernel while its workgroups (16 outputs; 16 rows, or 32 of more) come to two a CU, or one of the heavier kind.
+    // bf16 e4m3, few rows against tiles: 16 x 4096 x 4096 6.6 us against 11, 32 x 4096 x 4096 8.9 against 12, 128 x 4096 x 1024
+    // 9.0 against 12; beyond: 16 x 1024 x 16384 14.7 against 7.3, 64 x 4096 x 4096 16.4 against 12.3.  Up to 8 rows bring so few
+    // activations along that long contractions stay with it: 1 x 16384 x 16384 25 us against 31, 8 x 4096 x 16384 12.3 against 13.3
+    // (1 x 1024 x 65536 22 against 10).
+    const long wgs = (long)((out_dim + 15) / 16) * (rows <= 16 ? 1 : (rows + 31) / 32);
+    const bool f32 = fmt == GAN_MX_E4M3 && dtype == GAN_F32;
+    // (fp32 results: against the images and the bf16 product, both as measured: 64 x 8192 x 8192 53 us against 76, 96 rows 78
+    // against 78, 64 x 1024 x 16384 52 against 35)
+    const bool few = wgs <= (rows <= 16 ? 512 : 256) || (rows <= 8 && groups >= 32) ||
+                     (f32 && rows <= 128 && wgs * (0.021 + 0.000475 * groups) <= 18 + 0.85e-6 * in_dim * out_dim);
+    if (few) {
         // (a workgroup takes 64 groups, 8 a wave, in the time that a second launch for the joining costs)
         long s = wgs >= 256 ? 1 : 256 / wgs;
         if (s > groups / 64) s = groups / 64;
         return {MX_FEW, s < 1 ? 1 : (int)s};
     }
-    if (fmt == GAN_MX_E4M3 && dtype == GAN_F32) return {MX_VIA_BF16, 1};
+    if (f32) return {MX_VIA_BF16, 1};
     // 256 x 256 tiles where they fill the chip (4096^3 e4m3: 54 us against 69 with 128 x 128; 1024 x 4096 x 4096, 64 tiles: 42
-    // against 22).  A split contraction pays for its slabs only where few small tiles have long contractions (128 x 8192 x 8192:
-    // 32 us whole, 21 in three; 512 x 4096 x 4096, 128 tiles: 20 whole, 23 in two).
+    // against 22).  A split contraction pays for its slabs where few small tiles have long contractions (64 x 8192 x 8192: 29 us
+    // whole, 16.5 in four; 256 x 8192 x 8192, 128 tiles: 33 whole, 28 in two; 512 x 4096 x 4096, 128 tiles: 20 whole, 23 in two).
     const long large = (long)((rows + 255) / 256) * ((out_dim + 255) / 256);
     if (large >= 192) return {MX_TILE_LARGE, 1};
-    return {MX_TILE_SMALL, contraction_splits((long)((rows + 127) / 128) * ((out_dim + 127) / 128), 192, groups, 8)};
+    const long tiles = (long)((rows + 127) / 128) * ((out_dim + 127) / 128);
+    return {MX_TILE_SMALL, contraction_splits(tiles, 256, groups, tiles >= 128 ? 32 : 8)};
 }
 
 template <typename T, int FMT, int BN, int BR, int WN, int WR>
@@ -458,7 +467,7 @@ int gan_mx_matmul(int dtype, int fmt, int rows, int in_dim, int out_dim, const v
                   gan_stream_t stream) {
     GAN_CHECK_ARG(dtype_ok(dtype) && mx_fmt_ok(fmt), "gan_mx_matmul: unknown element type %d or format %d", dtype, fmt);
     GAN_CHECK_ARG(rows >= 0 && rows <= GAN_MX_MAX_ROWS && in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1 && out_dim <= GAN_MX_MAX_IN,
-                  "gan_mx_matmul: %d rows, %d inputs, %d outputs (up to %d of each are served)", rows, in_dim, out_dim, GAN_MX_MAX_IN);
+                  "gan_mx_matmul: %d rows, %d inputs, %d outputs (up to %d rows and %d of the others are served)", rows, in_dim, out_dim, GAN_MX_MAX_ROWS, GAN_MX_MAX_IN);
     if (rows == 0) return 0;
     GAN_CHECK_ARG(a_codes && a_scales && w_codes && w_scales && y, "gan_mx_matmul: null pointer");
     GAN_CHECK_ARG(aligned16(a_codes) && aligned16(w_codes) && ((reinterpret_cast<size_t>(a_scales) | reinterpret_cast<size_t>(w_scales)) & 3) == 0,
@@ -486,8 +495,8 @@ int gan_mx_linear(int dtype, int fmt, int rows, int in_dim, int out_dim, const v
                   const void* w_scales, const float* bias, void* y, void* ws, size_t ws_bytes, gan_stream_t stream) {
     GAN_CHECK_ARG(dtype_ok(dtype) && mx_fmt_ok(fmt), "gan_mx_linear: unknown element type %d or format %d", dtype, fmt);
     GAN_CHECK_ARG(rows >= 0 && rows <= GAN_MX_MAX_ROWS && in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1 && out_dim <= GAN_MX_MAX_IN && ldx >= in_dim,
-                  "gan_mx_linear: %d rows of stride %ld, %d inputs, %d outputs (up to %d of each are served)", rows, ldx, in_dim,
-                  out_dim, GAN_MX_MAX_IN);
+                  "gan_mx_linear: %d rows of stride %ld, %d inputs, %d outputs (up to %d rows, %d of the others)", rows, ldx, in_dim,
+                  out_dim, GAN_MX_MAX_ROWS, GAN_MX_MAX_IN);
     if (rows == 0) return 0;
     GAN_CHECK_ARG(x && w_codes && w_scales && y, "gan_mx_linear: null pointer");
     GAN_CHECK_ARG(aligned16(w_codes) && (reinterpret_cast<size_t>(w_scales) & 3) == 0,

@@ -887,10 +887,10 @@ class _RmsNormFn(torch.autograd.Function):
             dh = None if dh is None or not want else dh.contiguous()
             dx = dy.new_empty(dy.shape) if want else None
             dg, acc, wp, wn, hold = None, 0, None, 0, None
-            if gamma.wants_grad:
+            if gamma.wants_grad and rows:
                 dg, acc = gamma.grad_target()
                 wp, wn, hold = _lib.scratch(_size(lib.gan_rms_norm_workspace_bytes, rows, c), dy.device)
-            if dx is not None or dg is not None:
+            if rows and (dx is not None or dg is not None):
                 check(lib.gan_rms_norm_bwd(_lib.dtype_code(dy.dtype), rows, c, kept.data_ptr(), ctx.ld, ptr(gamma.data), ptr(rstd),
                                            dy.data_ptr(), None if dh is None else dh.data_ptr(),
                                            None if dx is None else dx.data_ptr(), ptr(dg), acc, wp, wn, stream()))

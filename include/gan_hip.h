@@ -331,7 +331,7 @@ enum { GAN_F32 = 0, GAN_BF16 = 1, GAN_F16 = 2 };
  * 128 inputs.  Magnitudes within a rounding step of the largest float may stand for infinity. */
 enum { GAN_MX_E4M3 = 0, GAN_MX_E2M1 = 1 };
 #define GAN_MX_MAX_IN (1 << 22)   /* most inputs and outputs of a product */
-#define GAN_MX_MAX_ROWS (1 << 22)
+#define GAN_MX_MAX_ROWS 4000000
 
 /* ---- root-mean-square norm with the residual's addition (extension: the reference norms with batch_norm only, ops.py:30-44)
  *   h = T(x + residual), s = 1 / sqrt(mean(h^2) + eps) over the c values of a row, y = h s gamma

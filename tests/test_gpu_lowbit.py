@@ -611,3 +611,47 @@ def test_distillation_with_everything_outside_the_list_masked(dtype):
     logits.fill_(torch.finfo(dtype).min)
     logits.scatter_(1, index, keep)
     _check_distill(logits, teacher, index, 2.0, 1.0, None, torch.logsumexp(teacher / 2, 1) + 0.3)
+
+
+def test_empty_batches_give_empty_gradients():
+    from gan_amd import ops
+    x = torch.zeros(0, 64, device='cuda', requires_grad=True)
+    with layer(rms_norm__gamma=torch.ones(64), Linear__Matrix=torch.ones(64, 8), Linear__bias=torch.ones(8)) as l:
+        y = ops.linear_mx(ops.rms_norm(x), 8)
+        assert tuple(y.shape) == (0, 8)
+        dx, = torch.autograd.grad((y,), (x,), (torch.zeros(0, 8, device='cuda'),))
+        assert tuple(dx.shape) == (0, 64)
+    assert all(float(l.grad(n).abs().max()) == 0 for n in ('rms_norm/gamma', 'Linear/Matrix', 'Linear/bias'))
+    dx, = torch.autograd.grad((ops.mx_matmul(x, ops.mx_pack(torch.ones(64, 8, device='cuda'))),), (x,), (torch.zeros(0, 8, device='cuda'),))
+    assert tuple(dx.shape) == (0, 64)
+
+
+@pytest.mark.parametrize("fmt", ['e4m3', 'e2m1'])
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("rows,k,n", [(16, 700, 9000), (24, 1024, 16384), (40, 8200, 600), (128, 300, 1000), (70, 8192, 128), (200, 4224, 2100)])
+def test_product_at_the_choices_of_kernel(rows, k, n, dtype, fmt):
+    _product(rows, k, n, dtype, fmt, seed=5)
+
+
+def test_distillation_of_the_largest_vocabulary_and_list():
+    g = gen(41)
+    classes, top = 1 << 20, 1024
+    logits = normal(g, 1, classes)
+    index, teacher = _lists(g, 1, classes, top, torch.float32)
+    for t in (torch.float32, torch.bfloat16):
+        _check_distill(logits.to(t), teacher, index, 1.0, 1.0, None, torch.logsumexp(teacher, 1) + 0.2)
+
+
+def test_a_loss_backward_twice_and_gradients_of_shared_logits():
+    """A retained loss gives its gradient again; two losses on the same logits add theirs."""
+    from gan_amd import ops
+    g = gen(42)
+    x = normal(g, 5, 300).requires_grad_(True)
+    index, teacher = _lists(g, 5, 300, 4, torch.float32)
+    loss = ops.distill_topk_mean(x, teacher, index)
+    first, = torch.autograd.grad(loss, x, retain_graph=True)
+    first = first.clone()
+    again, = torch.autograd.grad(loss, x)
+    assert torch.equal(first, again)
+    ops.backward([ops.distill_topk_mean(x, teacher, index), ops.distill_topk_mean(x, teacher, index, weight=0.5)])
+    within(x.grad, 1.5 * first.double(), 2.0 ** -23 * 1.5 * first.double().abs() + 1e-12, "sum")

@@ -77,9 +77,9 @@ def test_library_refuses_before_any_launch():
     _refused(lib.gan_mx_pack(0, 64, 4, p, 3, p, p, None), b"row stride")
     _refused(lib.gan_mx_matmul(1, 0, -1, 64, 64, p, p, p, p, None, p, None, 0, None), b"-1 rows")
     _refused(lib.gan_mx_matmul(1, 0, 4, 64, 64, p, p, odd, p, None, p, None, 0, None), b"aligned")
-    need = lib.gan_mx_matmul_workspace_bytes(0, 0, 100, 64, 64)
+    need = lib.gan_mx_matmul_workspace_bytes(0, 0, 1000, 64, 2000)
     assert need > 0
-    _refused(lib.gan_mx_matmul(0, 0, 100, 64, 64, p, p, p, p, None, p, p, need - 1, None), b"workspace")
+    _refused(lib.gan_mx_matmul(0, 0, 1000, 64, 2000, p, p, p, p, None, p, p, need - 1, None), b"workspace")
     need = lib.gan_mx_linear_workspace_bytes(1, 0, 100, 64, 64)
     assert need > 0 and lib.gan_mx_linear_workspace_bytes(1, 0, 1, 64, 64) == 0      # (one token: nothing to keep between launches)
     _refused(lib.gan_mx_linear(1, 0, 100, 64, 64, p, 64, p, p, None, p, p, need - 1, None), b"workspace")
