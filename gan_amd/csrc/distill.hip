@@ -1,6 +1,7 @@
 // Distillation from a teacher's top logits: mean over rows of a Kullback-Leibler divergence, fused with its gradient.
 //
-//   z = s / tau, t' = t / tau; list entries whose class is outside [0, classes) or whose logit is -inf are left out
+//   z = s / tau, t' = t / tau; list entries whose class is outside [0, classes) or whose logit is -inf are left out.  Maxima and
+//   differences are taken before the division, which could carry a mask of the type's lowest value to -inf
 //   p_i = softmax of t' over the list, or exp(t'_i - lse) where the teacher's log-sum-exp is given
 //   l = sum_i p_i (log p_i - log q_i)  [+ p_r (log p_r - log q_r)],   q = softmax z
 //   p_r = max(0, 1 - sum p), q_r = sum of q over the classes not listed (with lse only)
@@ -151,7 +152,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
         for (int i = lane; i < p.top; i += 64) {
             const long at = row * p.top + i;
             const long id64 = p.index64 ? static_cast<const long*>(p.index)[at] : static_cast<const int*>(p.index)[at];
-            const float t = teacher_at(p, at) * p.inv_tau;
+            const float t = teacher_at(p, at);
             const bool in = id64 >= 0 && id64 < classes && t != -INFINITY;
             const int id = in ? (int)id64 : -1;
             l_id[i] = id;
@@ -171,16 +172,17 @@ __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
         float norm = 0.f;
         if (REST) {
             norm = p.lse[row];
+            m = 0.f;
         } else {
             m = wave_all_max(m);
             float s = 0.f;
             for (int i = lane; i < p.top; i += 64)
-                if (l_id[i] >= 0) s += expf(l_lp[i] - m);
-            norm = m + logf(wave_all_sum(s));
+                if (l_id[i] >= 0) s += expf((l_lp[i] - m) * p.inv_tau);
+            norm = logf(wave_all_sum(s));
         }
         float mass = 0.f;
         for (int i = lane; i < p.top; i += 64) {
-            const float lp = l_lp[i] - norm, pr = l_id[i] >= 0 ? expf(lp) : 0.f;
+            const float lp = (l_lp[i] - m) * p.inv_tau - norm, pr = l_id[i] >= 0 ? expf(lp) : 0.f;
             l_lp[i] = lp;
             l_p[i] = pr;
             mass += pr;
@@ -406,8 +408,8 @@ static int launch_distill(const Distill& p, hipStream_t st) {
     auto go = [&](auto kernel) {
         // the list's bits of the largest vocabulary and the longest list
         constexpr int most = kMaxClasses / 8 + 64 + kMaxTop * 16;
-        const hipError_t set = lds > 65536 ? hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                                                 hipFuncAttributeMaxDynamicSharedMemorySize, most) : hipSuccess;
+        static std::atomic<unsigned long> devices{0};
+        const hipError_t set = lds > 65536 ? allow_lds(reinterpret_cast<const void*>(kernel), most, devices) : hipSuccess;
         if (set != hipSuccess) return fail("gan_distill_topk_mean: %zu bytes of LDS refused: %s", lds, hipGetErrorString(set));
         hipLaunchKernelGGL(kernel, dim3((unsigned)p.rows), dim3(NT), lds, st, p);
         return 0;
@@ -428,11 +430,12 @@ int gan_distill_topk_mean(int dtype, long rows, int classes, const void* logits,
                           float temperature, float weight, int accumulate, float* loss_out, void* dlogits, void* ws,
                           size_t ws_bytes, gan_stream_t stream) {
     GAN_CHECK_ARG(dtype_ok(dtype) && dtype_ok(teacher_dtype), "gan_distill_topk_mean: unknown element type %d or %d", dtype, teacher_dtype);
-    GAN_CHECK_ARG(rows >= 1 && rows < (1L << 31), "gan_distill_topk_mean: %ld rows", rows);
+    GAN_CHECK_ARG(rows >= 1 && rows <= GAN_MX_MAX_ROWS, "gan_distill_topk_mean: %ld rows (1..%d are served)", rows, GAN_MX_MAX_ROWS);
     GAN_CHECK_ARG(classes >= 1 && classes <= kMaxClasses, "gan_distill_topk_mean: %d classes (1..%d are served)", classes, kMaxClasses);
     GAN_CHECK_ARG(top >= 1 && top <= kMaxTop, "gan_distill_topk_mean: lists of %d (1..%d are served)", top, kMaxTop);
     GAN_CHECK_ARG(index_bytes == 4 || index_bytes == 8, "gan_distill_topk_mean: indices of %d bytes", index_bytes);
-    GAN_CHECK_ARG(temperature > 0.f && temperature < INFINITY, "gan_distill_topk_mean: temperature %g", (double)temperature);
+    GAN_CHECK_ARG(temperature >= 0x1p-40f && temperature <= 0x1p40f, "gan_distill_topk_mean: temperature %g (2^-40..2^40 are served)",
+                  (double)temperature);
     GAN_CHECK_ARG(logits && teacher && index && loss_out, "gan_distill_topk_mean: null pointer");
     GAN_CHECK_ARG(ld >= classes, "gan_distill_topk_mean: row stride %ld smaller than the row", ld);
     GAN_CHECK_ARG(ws && ws_bytes >= gan_distill_topk_workspace_bytes(rows), "gan_distill_topk_mean: workspace of %zu bytes needed, %zu given",

@@ -6,6 +6,7 @@
 // quantiser can be passed straight through without a mask.  A block that holds an infinity or a NaN has scale byte 255 and
 // stands for NaN in all its values.  An all-zero block has scale byte 1.
 #pragma once
+#include <atomic>
 #include <type_traits>
 
 #include "common.h"
@@ -186,6 +187,16 @@ __device__ __forceinline__ unsigned mx_quantize_lane8(const float (&v)[8], unsig
         code[1] = 0;
     }
     return byte;
+}
+
+// A kernel's launches may use up to `bytes` of dynamic LDS.  Asked for once a device; `devices` remembers where.
+inline hipError_t allow_lds(const void* kernel, int bytes, std::atomic<unsigned long>& devices) {
+    int device = 0;
+    hipError_t rc = hipGetDevice(&device);
+    if (rc != hipSuccess || (device < 64 && devices.load(std::memory_order_relaxed) >> device & 1)) return rc;
+    rc = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (rc == hipSuccess && device < 64) devices.fetch_or(1ul << device, std::memory_order_relaxed);
+    return rc;
 }
 
 // Calls f with a null pointer of the element type `dtype` names.

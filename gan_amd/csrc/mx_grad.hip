@@ -151,8 +151,8 @@ static int launch_bf16(const Bf16Product& p, T* out, float* slabs, int splits, b
     // 128 x 128: two workgroups a CU
     constexpr int STAGES = BI + BJ == 384 ? 3 : 2, LDS = STAGES * (BI + BJ) * 128;
     auto kernel = bf16_product_kernel<T, BI, BJ, WI, WJ, STAGES>;
-    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                                      hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    static std::atomic<unsigned long> devices{0};
+    const hipError_t set = allow_lds(reinterpret_cast<const void*>(kernel), LDS, devices);
     if (set != hipSuccess) return fail("%s: %d bytes of LDS refused: %s", what, LDS, hipGetErrorString(set));
     const long tiles = (long)((p.rows + BI - 1) / BI) * ((p.cols + BJ - 1) / BJ);
     hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, splits), dim3(64 * WI * WJ), LDS, st, p, out, slabs, splits, vec);

@@ -383,8 +383,8 @@ static int launch_tile(const MxProduct& p, hipStream_t st) {
     // small tiles: two workgroups a CU
     constexpr int STAGES = STAGE * 3 <= (BN == 256 ? 160 : 80) * 1024 ? 3 : 2, LDS = STAGES * STAGE;
     auto kernel = mx_tile_kernel<T, FMT, BN, BR, WN, WR, STAGES>;
-    static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                                      hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    static std::atomic<unsigned long> devices{0};
+    const hipError_t set = allow_lds(reinterpret_cast<const void*>(kernel), LDS, devices);
     if (set != hipSuccess) return fail("gan_mx_matmul: %d bytes of LDS refused: %s", LDS, hipGetErrorString(set));
     const long tiles = (long)((p.rows + BR - 1) / BR) * ((p.n + BN - 1) / BN);
     hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, p.splits), dim3(64 * WN * WR), LDS, st, p);

@@ -4,9 +4,10 @@
 //   g = dy gamma   n = h s   dx = dr = s (g - n mean(g n)) + dh   dgamma = sum over rows of dy n
 //
 // h is rounded to the tensors' type before it is normalised: it is the residual stream that is stored and that the backward
-// pass reads again, so forward and backward see one h.  Sums are fp32; in front of the 8-bit output they, and y, are fp64:
-// the row is one division away from a grid with steps of 1/8, and with y rounded once from 64 bits a value next to a border
-// falls on its own side (fp64 runs at the fp32 rate here, and the kernel waits for memory: no cost was measurable).
+// pass reads again, so forward and backward see one h.  The sum of squares is fp64, so that no finite row overflows it; the
+// backward's sums are fp32.  In front of the 8-bit output y is fp64 too: the row is one division away from a grid with steps of
+// 1/8, and with y rounded once from 64 bits a value next to a border falls on its own side (fp64 runs at the fp32 rate here, and
+// the kernel waits for memory: no cost was measurable).
 //
 // Memory-bound.  A team of 64 to 1024 threads keeps a whole row in registers, eight values a chunk, so every tensor is
 // read and written once.
@@ -46,17 +47,15 @@ struct RmsFwd {
 template <typename T, int TPR, int NV, bool MX>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(RmsFwd p) {
     constexpr int TEAMS = TPR < 256 ? 256 / TPR : 1;
-    __shared__ double red_d[TPR / 64];
-    __shared__ float red_f[TPR / 64];
+    __shared__ double red[TPR / 64];
     const int t = threadIdx.x % TPR, team = threadIdx.x / TPR;
     const int c = p.c, chunks = MX ? mx_groups(c) * 16 : (c + 7) / 8;
-    const long row = (long)blockIdx.x * TEAMS + team;
+    const long row = ((long)blockIdx.y * gridDim.x + blockIdx.x) * TEAMS + team;
     const bool live = row < p.rows;
     const T* xr = static_cast<const T*>(p.x) + (live ? row : 0) * p.ldx;
     const T* rr = p.res ? static_cast<const T*>(p.res) + (live ? row : 0) * p.ldr : nullptr;
     float v[NV][8], g[NV][8];
-    double sd = 0;
-    float sf = 0;
+    double s = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int i0 = (i * TPR + t) * 8;
@@ -73,19 +72,10 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(RmsFwd p
         }
         load8(p.gamma, i0, i0 < c ? c : 0, p.vec_g, g[i]);      // (on its way while the row is summed)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (MX) sd = fma((double)v[i][j], (double)v[i][j], sd);
-            else sf = fmaf(v[i][j], v[i][j], sf);
-        }
+        for (int j = 0; j < 8; ++j) s = fma((double)v[i][j], (double)v[i][j], s);
     }
-    float rstd;
-    double inv = 0;
-    if (MX) {
-        inv = 1.0 / sqrt(team_sum(sd, TPR, red_d) / c + (double)p.eps);
-        rstd = (float)inv;
-    } else {
-        rstd = 1.f / sqrtf(team_sum(sf, TPR, red_f) / c + p.eps);
-    }
+    const double inv = 1.0 / sqrt(team_sum(s, TPR, red) / c + (double)p.eps);
+    const float rstd = (float)inv;
     if (!live) return;
     if (p.rstd && t == 0) p.rstd[row] = rstd;
 #pragma unroll
@@ -244,6 +234,7 @@ int gan_rms_norm_fwd(int dtype, long rows, int c, const void* x, long ldx, const
     GAN_CHECK_ARG(gamma && (rows == 0 || (x && (mx ? mx_scales && !y : y != nullptr) && (residual != nullptr) == (h != nullptr))),
                   "gan_rms_norm_fwd: null pointer (x, gamma, one of y or mx_codes with mx_scales; h exactly with a residual)");
     GAN_CHECK_ARG(ldx >= c && (!residual || ldr >= c), "gan_rms_norm_fwd: row stride smaller than the row");
+    GAN_CHECK_ARG(eps >= 0.f, "gan_rms_norm_fwd: epsilon %g", (double)eps);
     GAN_CHECK_ARG(!mx || ((reinterpret_cast<size_t>(mx_codes) & 7) == 0), "gan_rms_norm_fwd: mx_codes is not 8-byte aligned");
     if (rows == 0) return 0;
     return with_dtype(dtype, [&](auto* tag) {
@@ -254,7 +245,9 @@ int gan_rms_norm_fwd(int dtype, long rows, int c, const void* x, long ldx, const
                  c * sizeof(T) % 16 == 0 && aligned16(h) && aligned16(y), aligned16(gamma)};
         with_shape(mx ? mx_groups(c) * 16 : (c + 7) / 8, [&](auto tpr, auto nv) {
             constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, TEAMS = TPR < 256 ? 256 / TPR : 1;
-            const dim3 grid((unsigned)((rows + TEAMS - 1) / TEAMS)), block(TPR < 256 ? 256 : TPR);
+            // (fewer than 2^32 threads along x)
+            const long blocks = (rows + TEAMS - 1) / TEAMS, along = blocks < (1L << 21) ? blocks : 1L << 21;
+            const dim3 grid((unsigned)along, (unsigned)((blocks + along - 1) / along)), block(TPR < 256 ? 256 : TPR);
             if (mx) hipLaunchKernelGGL((rms_fwd_kernel<T, TPR, NV, true>), grid, block, 0, as_stream(stream), p);
             else hipLaunchKernelGGL((rms_fwd_kernel<T, TPR, NV, false>), grid, block, 0, as_stream(stream), p);
         });

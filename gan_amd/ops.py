@@ -53,6 +53,13 @@ class taping(object):
         _force_tape[0] = self.previous
 
 
+def _token_key(device, early):
+    """A pass under capture has leaves of its own: autograd joins the stream a leaf was first used on, which would drag the
+    stream of an eager pass that is still alive into the capture and end it."""
+    capturing = torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
+    return device, early, stream() if capturing else None
+
+
 def _grad_token(device, var=None):
     """A leaf that requires grad, threaded through a layer so that its backward runs (and can emit
     weight gradients) even when its data input needs no gradient.  Layers whose weights are frozen
@@ -60,7 +67,7 @@ def _grad_token(device, var=None):
     (tf.gradients prunes the same sub-graph, e.g. G_B2A(real_B) in cyclegan.py's g_loss_a2b)."""
     if var is not None and not var.wants_grad and not _force_tape[0]:
         return None
-    key = (device, bool(var is not None and var.early))
+    key = _token_key(device, bool(var is not None and var.early))
     t = _token.get(key)
     if t is None:
         t = torch.zeros(1, device=device, requires_grad=True)
@@ -802,10 +809,15 @@ def instance_norm(x, name="instance_norm", epsilon=1e-5, act=None, act_param=0.2
 # --------------------------------------------------------------------------------------------
 # root-mean-square norm (extension): fp32 / bf16 / fp16, with the residual's addition and an 8-bit output
 # --------------------------------------------------------------------------------------------
+_MOST = (1 << 31) - 1
+
+
 def _rows_of(t):
     """(tensor, rows, columns, row stride) of t seen as rows along its last axis: a rank-2 view with its columns side by side
     is taken as it is, everything else made dense."""
     c = t.shape[-1]
+    if c > _MOST or t.numel() > c * _MOST:
+        raise ValueError("shape %s is beyond 32-bit counts of rows and columns" % (tuple(t.shape),))
     if t.dim() == 2 and t.shape[0] > 1 and t.stride(1) == 1 and t.stride(0) >= c:
         return t, t.shape[0], c, t.stride(0)
     t = t.contiguous()
@@ -900,7 +912,7 @@ class _RmsNormFn(torch.autograd.Function):
 def rms_norm(x, name="rms_norm", epsilon=1e-6, residual=None, mx=False):
     """Extension: y = h / sqrt(mean(h^2) + epsilon) * gamma over the last axis, h = x + residual rounded to x's type; gamma
     (fp32, ones at first) is created under the caller's scope + name.  x and residual: fp32, bf16 or fp16, one shape and
-    type, up to 32768 values on the last axis.
+    type, up to 32768 values on the last axis; epsilon >= 0.
 
     Returns y, or (y, h) with a residual: h is the next residual.  mx=True returns y as an e4m3 `MxTensor`, the form
     `linear_mx` and `mx_matmul` multiply; gradients pass straight through its rounding."""
@@ -910,8 +922,10 @@ def rms_norm(x, name="rms_norm", epsilon=1e-6, residual=None, mx=False):
     _lib.dtype_code(x.dtype)
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError("rms_norm: residual %s %s does not match x %s %s" % (tuple(residual.shape), residual.dtype, tuple(x.shape), x.dtype))
-    gamma = _variable(st, name, 'gamma', (x.shape[-1],), V.constant_initializer(1.0))
     eps, mx = float(epsilon), bool(mx)
+    if not 0.0 <= eps < float('inf'):
+        raise ValueError("rms_norm: epsilon %r" % (epsilon,))
+    gamma = _variable(st, name, 'gamma', (x.shape[-1],), V.constant_initializer(1.0))
     token = _grad_token(x.device, gamma) if torch.is_grad_enabled() else None
     if token is None and not (torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad))):
         out, h, _, _ = _rms_fwd(x, residual, gamma, eps, mx, False)
@@ -1031,7 +1045,8 @@ def mx_pack(matrix):
 
 
 def mx_dequantize(q, dtype=None):
-    """The values an `MxTensor` (in its own type unless `dtype` is given) or an `MxMatrix` (fp32) stands for, dense."""
+    """The values an `MxTensor` (in its own type unless `dtype` is given) or an `MxMatrix` (fp32) stands for, dense and outside
+    of autograd."""
     if isinstance(q, MxMatrix):
         dtype = torch.float32 if dtype is None else dtype
         code = _lib.dtype_code(dtype)
@@ -1444,7 +1459,7 @@ class _DistillFn(torch.autograd.Function):
 
 def distill_topk_mean(logits, teacher_logits, teacher_index, temperature=1.0, weight=1.0, row_weight=None, teacher_lse=None):
     """Extension: mean divergence of the student's softmax from a teacher known by its top logits, times weight * temperature^2;
-    a root for `backward` like the losses above.
+    a root for `backward` like the losses above.  temperature: 2^-40 to 2^40.
 
     logits [..., classes] (fp32, bf16, fp16); teacher_logits (any of the three types) and teacher_index (int32 / int64) [..., top]:
     the teacher's highest logits and their classes, in any order.  Entries with an index outside [0, classes) (-1 fills a short
@@ -1465,7 +1480,7 @@ def distill_topk_mean(logits, teacher_logits, teacher_index, temperature=1.0, we
     for what, t in (("row_weight", row_weight), ("teacher_lse", teacher_lse)):
         if t is not None and (tuple(t.shape) != lead or t.dtype != torch.float32):
             raise ValueError("distill_topk_mean: %s %s %s for rows %s (float32 expected)" % (what, tuple(t.shape), t.dtype, lead))
-    if not 0.0 < float(temperature) < float('inf'):
+    if not 2.0 ** -40 <= float(temperature) <= 2.0 ** 40:
         raise ValueError("distill_topk_mean: temperature %r" % (temperature,))
     return _DistillFn.apply(logits, _plain(teacher_logits), _plain(teacher_index), _plain(teacher_lse), _plain(row_weight),
                             float(temperature), float(weight))
@@ -1495,7 +1510,7 @@ def backward(losses, boundary=None, at_boundary=None):
         for t in boundary:
             if not t.requires_grad:
                 raise ValueError("backward: a boundary activation does not take part in the backward pass")
-        early_token = _token.get((dev, True))
+        early_token = _token.get(_token_key(dev, True))
         wanted = boundary + ([early_token] if early_token is not None else [])
         grads = torch.autograd.grad(roots, wanted, seeds, allow_unused=True)[:len(boundary)]
         if any(g is None for g in grads):

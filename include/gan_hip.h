@@ -331,13 +331,13 @@ enum { GAN_F32 = 0, GAN_BF16 = 1, GAN_F16 = 2 };
  * 128 inputs.  Magnitudes within a rounding step of the largest float may stand for infinity. */
 enum { GAN_MX_E4M3 = 0, GAN_MX_E2M1 = 1 };
 #define GAN_MX_MAX_IN (1 << 22)   /* most inputs and outputs of a product */
-#define GAN_MX_MAX_ROWS 4000000
+#define GAN_MX_MAX_ROWS 4000000   /* most rows of a product or a distillation */
 
 /* ---- root-mean-square norm with the residual's addition (extension: the reference norms with batch_norm only, ops.py:30-44)
  *   h = T(x + residual), s = 1 / sqrt(mean(h^2) + eps) over the c values of a row, y = h s gamma
  * x and residual have row strides ldx, ldr (in values); h and y are dense, all of type dtype; gamma fp32.  h is written exactly
  * when a residual is given.  Output either y, or mx_codes / mx_scales: y in e4m3 (the product's operand; y is then computed
- * in 64 bits, and nothing is stored in T).  rstd (fp32 [rows], may be NULL) receives s for the backward.  c <= 32768.
+ * in 64 bits, and nothing is stored in T).  rstd (fp32 [rows], may be NULL) receives s for the backward.  c <= 32768, eps >= 0.
  * Backward, from the stored stream h (x itself without a residual), with g = dy gamma, n = h s:
  *   dx = s (g - n mean(g n)) + dh      dgamma (+)= sum over rows of dy n
  * dh (the gradient that reaches h from elsewhere), dx and dgamma may be NULL. */
@@ -392,7 +392,7 @@ int gan_mx_matmul_wgrad(int dtype, int fmt, int rows, int in_dim, int out_dim, c
  *   loss_out[0] = (accumulate ? loss_out[0] : 0) + weight temperature^2 sum_r w_r l_r / sum_r w_r
  * dlogits (dense, type dtype, may be NULL) = its gradient.  row_weight NULL: all 1.  A row of weight 0 or without a list entry
  * has loss 0 and gradient 0 whatever its logits hold; weights that add up to 0 give loss 0 and gradient 0.
- * classes <= 2^20, top <= 1024. */
+ * classes <= 2^20, top <= 1024, 2^-40 <= temperature <= 2^40. */
 size_t gan_distill_topk_workspace_bytes(long rows);
 int gan_distill_topk_mean(int dtype, long rows, int classes, const void* logits, long ld, int teacher_dtype,
                           const void* teacher, const void* index, int index_bytes, int top, const float* teacher_lse,

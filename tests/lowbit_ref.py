@@ -71,7 +71,8 @@ def distill(logits, teacher, index, tau=1.0, weight=1.0, row_weight=None, lse=No
         logq = z - torch.logsumexp(z, 0)
         q = torch.exp(logq)
         t = torch.tensor([v for _, v in at], dtype=torch.float64)
-        logp = t - (torch.logsumexp(t, 0) if lse is None else float(lse[r]))
+        # (differences first: beside the type's lowest value there is no room for the log of a number of entries)
+        logp = torch.log_softmax(t - t.max(), 0) if lse is None else t - float(lse[r])
         p = torch.exp(logp)
         rest = 0.0 if lse is None else max(0.0, 1.0 - float(p.sum()))
         mass = (float(p.sum()) if lse is not None else 1.0) + rest

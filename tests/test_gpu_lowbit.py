@@ -655,3 +655,76 @@ def test_a_loss_backward_twice_and_gradients_of_shared_logits():
     assert torch.equal(first, again)
     ops.backward([ops.distill_topk_mean(x, teacher, index), ops.distill_topk_mean(x, teacher, index, weight=0.5)])
     within(x.grad, 1.5 * first.double(), 2.0 ** -23 * 1.5 * first.double().abs() + 1e-12, "sum")
+
+
+@pytest.mark.parametrize("dtype,size", [(torch.float32, 1e30), (torch.float32, 1e-25), (torch.bfloat16, 1e38), (torch.bfloat16, 1e-30)])
+def test_norm_of_values_whose_squares_leave_fp32(dtype, size):
+    from gan_amd import ops
+    g = gen(51)
+    x = (normal(g, 3, 700).clamp(-3, 3) * size).to(dtype)
+    gamma = 1 + 0.1 * normal(g, 700)
+    with layer(rms_norm__gamma=gamma), torch.no_grad():
+        want = R.rms(x, gamma, 0.0)
+        # (1 / 1e38 is subnormal in fp32: 2^-23 relative, two E, on top)
+        within(ops.rms_norm(x, epsilon=0.0), want, (half_step(dtype) + 52 * E) * want.abs(), "y")
+        _mx_equal(ops.rms_norm(x, epsilon=0.0, mx=True), want.float(), "codes")
+
+
+def test_norm_of_more_rows_than_one_axis_of_a_grid_holds():
+    """70 million rows of one value each: y = gamma x / sqrt(x^2 + eps)."""
+    from gan_amd import ops
+    g = gen(52)
+    x = normal(g, 70000000, 1).bfloat16()
+    with layer(rms_norm__gamma=torch.full((1,), 1.5)), torch.no_grad():
+        y = ops.rms_norm(x)
+    for part in (slice(0, 1000), slice(34000000, 34001000), slice(-1000, None)):
+        want = R.rms(x[part], torch.full((1,), 1.5, device='cuda'), 1e-6)
+        within(y[part], want, (half_step(torch.bfloat16) + 50 * E) * want.abs(), "rows")
+    assert bool((y.sign() == x.sign()).all())
+
+
+def test_distillation_from_a_teacher_whose_list_is_all_masked():
+    """Logits of the type's lowest value divided by a temperature below 1 are still logits: p is uniform over them."""
+    g = gen(53)
+    logits = normal(g, 3, 200)
+    index, teacher = _lists(g, 3, 200, 5, torch.float32)
+    teacher[0] = torch.finfo(torch.float32).min
+    teacher[1, 2:] = torch.finfo(torch.float32).min
+    _check_distill(logits, teacher, index, 0.5)
+    _check_distill(logits, teacher.bfloat16().clamp(min=torch.finfo(torch.bfloat16).min), index, 0.5)
+
+
+def test_a_pass_is_captured_while_an_eager_one_lives():
+    from gan_amd import ops
+    g = gen(54)
+    l, x, r, _, (index, teacher, lse) = _student(g)
+    names = ('rms_norm/gamma', 'head/Matrix', 'head/bias')
+
+    def loss():
+        q, _ = ops.rms_norm(x, residual=r, mx=True)
+        return ops.distill_topk_mean(ops.linear_mx(q, teacher_classes(l), 'head'), teacher, index, teacher_lse=lse)
+
+    def step():
+        with l:
+            ops.backward(loss())
+    with l:
+        alive = loss()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+        grads = [l.grad(n).clone() for n in names]
+    with l:
+        ops.backward(alive)
+    want = [l.grad(n).clone() for n in names]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(grads, want):
+            assert torch.equal(a, b)
+        step()

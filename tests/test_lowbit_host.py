@@ -145,3 +145,38 @@ def test_python_layer_refuses_what_does_not_go_together():
         ops.distill_topk_mean(x, t, i.float())
     with pytest.raises(ValueError):
         ops.distill_topk_mean(x[:0], t[:0], i[:0])
+
+
+def test_ranges_beyond_the_documented_ones_are_refused():
+    from gan_amd import _lib as L
+    from gan_amd import ops
+    from gan_amd import variables as V
+    lib, p, x = L.lib, FAKE, torch.zeros(4, 64)
+    _refused(lib.gan_rms_norm_fwd(0, 4, 64, p, 64, None, 0, p, -1e-6, None, p, None, None, None, None), b"epsilon")
+    _refused(lib.gan_distill_topk_mean(0, 4000001, 9, p, 9, 0, p, p, 4, 3, None, None, 1.0, 1.0, 0, p, p, p, 1 << 30, None), b"4000001 rows")
+    _refused(lib.gan_distill_topk_mean(0, 4, 9, p, 9, 0, p, p, 4, 3, None, None, 1e-20, 1.0, 0, p, p, p, 1 << 30, None), b"temperature")
+    with V.use_store(V.VariableStore(device='cpu')):
+        for eps in (-1e-6, float('nan'), float('inf')):
+            with pytest.raises(ValueError):
+                ops.rms_norm(x, epsilon=eps)
+    t, i = torch.zeros(4, 3), torch.zeros(4, 3, dtype=torch.int64)
+    for tau in (1e-20, 1e20, float('nan')):
+        with pytest.raises(ValueError):
+            ops.distill_topk_mean(x, t, i, temperature=tau)
+    # counts that a 32-bit argument would wrap around (expanded: nothing of that size is allocated)
+    for shape in ((1 << 32, 64), (2, (1 << 32) + 64)):
+        with pytest.raises(ValueError):
+            ops._rows_of(torch.zeros(1, 1).expand(shape))
+
+
+def test_a_capture_has_leaves_of_its_own(monkeypatch):
+    from gan_amd import ops
+    device = torch.device('cuda', 0)
+    eager = ops._token_key(device, True)
+    assert eager == ops._token_key(device, True) != ops._token_key(device, False)
+    monkeypatch.setattr(torch.cuda, 'is_initialized', lambda: True)
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+    monkeypatch.setattr(ops, 'stream', lambda: 7)
+    first = ops._token_key(device, True)
+    monkeypatch.setattr(ops, 'stream', lambda: 8)
+    assert len({eager, first, ops._token_key(device, True)}) == 3
