@@ -117,6 +117,8 @@ SIGNATURES = {
     "gan_mx_matmul_dgrad": (I, [I, I, I, I, P, P, P, P, P, Z, P]),
     "gan_mx_matmul_wgrad_workspace_bytes": (Z, [I, I, I, I]),
     "gan_mx_matmul_wgrad": (I, [I, I, I, I, I, P, P, P, P, P, I, P, Z, P]),
+    "gan_mx_matmul_bwd_workspace_bytes": (Z, [I, I, I, I]),
+    "gan_mx_matmul_bwd": (I, [I, I, I, I, I, P, P, P, P, P, P, P, P, I, P, Z, P]),
     "gan_distill_topk_workspace_bytes": (Z, [L]),
     "gan_distill_topk_mean": (I, [I, L, I, P, L, I, P, P, I, I, P, P, F, F, I, P, P, P, Z, P]),
     "gan_adam_tf_step": (I, [P, P, P, P, L, F, F, F, F, F, P, P, P]),

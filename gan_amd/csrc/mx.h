@@ -25,7 +25,7 @@ typedef float f32x8 __attribute__((ext_vector_type(8), aligned(16)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef short i16x2 __attribute__((ext_vector_type(2)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
 
 template <typename T> struct Vec8;
 template <> struct Vec8<float> { typedef f32x8 type; };

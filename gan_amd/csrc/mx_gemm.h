@@ -167,22 +167,22 @@ inline int contraction_splits(long tiles, int workgroups, int steps, int least) 
     return s < 1 ? 1 : (int)s;
 }
 
-// The bf16-pipe product of mx_grad.hip: C[i][j] (+)= bias[j] + sum over parts and c of P[i][c] Q[j][c].
+// The bf16-pipe product of mx_grad.hip: C[i][j] (+)= bias[j] + sum over parts and c of P[i][c] Q[j][c], or (TRANS) P[c][i] Q[c][j].
 struct Bf16Product {
     const bf16_t* p;
     const bf16_t* q;
     long ldp, ldq, pstep, qstep;    // row strides; step from one part to the next
-    int parts, depth;               // depth of one part: a multiple of 64, rows filled up with zeros to it
+    int parts, depth;               // depth of one part: a multiple of 64, operands filled up with zeros to it
     int rows, cols;                 // of C, dense
     const float* bias;
     int accumulate;
 };
 size_t bf16_product_workspace(int rows, int cols, int parts, int depth);
-template <typename T>
+template <bool TRANS, typename T>
 int bf16_product(const Bf16Product& p, T* out, void* ws, hipStream_t st, const char* what);
 
-// [rows][groups * 128] bf16 and [out][groups * 128] bf16 of microscaled operands (forward with fp32 results).
-void mx_rows_to_bf16(int fmt, const void* codes, const void* scales, bf16_t* out, long rows, int in_dim, hipStream_t st);
+// [filled][groups * 128] bf16 (rows and then zeros) and [out][groups * 128] bf16 of microscaled operands.
+void mx_rows_to_bf16(int fmt, const void* codes, const void* scales, bf16_t* out, long rows, long filled, int in_dim, hipStream_t st);
 void mx_weights_to_bf16(const void* codes, const void* scales, bf16_t* out, int in_dim, int out_dim, hipStream_t st);
 
 }  // namespace gan

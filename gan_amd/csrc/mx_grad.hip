@@ -6,11 +6,17 @@
 // bf16; dY is split exactly into one (bf16), two (fp16: 11 = 8 + 3 bits) or three (fp32: 24 = 8 + 8 + 8) bf16 parts, whose
 // products are summed in fp32.  So a gradient carries the error of an fp32 sum of exact products whatever the type.
 //
-// All three products contract over rows that are contiguous in memory: memory-bound passes turn the operands into bf16 images
-// with the contraction axis innermost and filled up with zeros to a multiple of 64, then one compute-bound kernel runs.
+// Memory-bound passes turn the operands into bf16 images whose contraction axis is filled up with zeros to a multiple of 64 -- one
+// image of dY for both products, none where dY is bf16 in whole 64s --, then one compute-bound kernel runs each product.  The forward
+// and dA contract over contiguous values, dW over rows (TRANS).
 #include "mx_gemm.h"
 
 namespace gan {
+
+// The LDS's transposing read.  (The restrict is for the compiler's waits: of an access that it knows nothing about it assumes that it
+// reads what a copy in flight writes, and waits for all of them.)
+typedef __attribute__((address_space(3))) i16x4* lds_i16x4;
+__device__ __forceinline__ i16x4 read_transposed(lds_i16x4 __restrict__ from) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16(from); }
 
 // C[i][j] over a tile of BI x BJ, WI x WJ waves, 32x32x16 instructions with Q as their first operand (a lane ends with four
 // consecutive j of one i).  A stage in LDS is 64 deep: 128 bytes of every row -- whole cache lines; 64 bytes a row and stage cost
@@ -20,7 +26,10 @@ namespace gan {
 // Large tiles have two waves a SIMD with 128 x 64 outputs each: LDS then gives 96 bytes a clock of its 128; one wave of
 // 128 x 128 needs less of it, but nothing covers its waits (4096^3: 126 us against 115, the weights' image included).
 // 4096 x 4096 x 8192: 1.25 PF/s, a library product of that size 1.45.
-template <typename T, int BI, int BJ, int WI, int WJ, int STAGES>
+// TRANS: the operands lie the other way round, [contraction][rows of C] and [contraction][columns of C], as a gradient of weights
+// has them.  A stage then is 64 rows of BI and of BJ values, its 64-byte pieces swapped by row; a fragment, eight consecutive of the
+// contraction for each of 32 values, is read by the LDS's transposing read: 16 lanes fetch 4 x 16 values, lane i keeps column i.
+template <typename T, int BI, int BJ, int WI, int WJ, int STAGES, bool TRANS>
 __global__ __launch_bounds__(64 * WI * WJ) void bf16_product_kernel(Bf16Product p, T* out, float* slabs, int splits, bool vec) {
     constexpr int WAVES = WI * WJ, THREADS = 64 * WAVES, FI = BI / WI / 32, FJ = BJ / WJ / 32, STAGE = (BI + BJ) * 128;
     constexpr int COPIES = STAGE / 16 / THREADS;        // of a wave for a stage
@@ -37,20 +46,29 @@ __global__ __launch_bounds__(64 * WI * WJ) void bf16_product_kernel(Bf16Product 
     // where this lane's copies begin, and the two operands' places in the part at hand (rows beyond the last: the last again)
     constexpr int PC = BI * 8 / THREADS, QC = BJ * 8 / THREADS;
     unsigned p_off[PC], q_off[QC];
+    auto offset = [&](int at, auto width, int first, int last, long ld) -> unsigned {
+        constexpr int kChunks = decltype(width)::value / 8;
+        if constexpr (TRANS) {      // (chunks beyond the row: its last again)
+            const int k = at / kChunks, chunk = at % kChunks ^ (k & 3) << 2;
+            return (unsigned)k * (unsigned)(ld * 2) + (unsigned)min(first + chunk * 8, (int)ld - 8) * 2u;
+        } else {
+            const int row = at >> 3, chunk = (at & 7) ^ (row & 7);
+            return (unsigned)min(row, last - first) * (unsigned)(ld * 2) + chunk * 16;
+        }
+    };
 #pragma unroll
-    for (int i = 0; i < PC; ++i) {
-        const int row = ((i * WAVES + wave) * 64 + lane) >> 3, chunk = (lane & 7) ^ (row & 7);
-        p_off[i] = (unsigned)min(row, p.rows - 1 - i0) * (unsigned)(p.ldp * 2) + chunk * 16;
-    }
+    for (int i = 0; i < PC; ++i)
+        p_off[i] = offset((i * WAVES + wave) * 64 + lane, std::integral_constant<int, BI>(), i0, p.rows - 1, p.ldp);
 #pragma unroll
-    for (int i = 0; i < QC; ++i) {
-        const int row = ((i * WAVES + wave) * 64 + lane) >> 3, chunk = (lane & 7) ^ (row & 7);
-        q_off[i] = (unsigned)min(row, p.cols - 1 - j0) * (unsigned)(p.ldq * 2) + chunk * 16;
-    }
+    for (int i = 0; i < QC; ++i)
+        q_off[i] = offset((i * WAVES + wave) * 64 + lane, std::integral_constant<int, BJ>(), j0, p.cols - 1, p.ldq);
     int filled = s0, in_part = s0 % per;
-    const unsigned char* pp = reinterpret_cast<const unsigned char*>(p.p + (long)i0 * p.ldp + (s0 / per) * p.pstep + in_part * 64L);
-    const unsigned char* qp = reinterpret_cast<const unsigned char*>(p.q + (long)j0 * p.ldq + (s0 / per) * p.qstep + in_part * 64L);
-    const long p_jump = (p.pstep - (per - 1) * 64L) * 2, q_jump = (p.qstep - (per - 1) * 64L) * 2;
+    const long p_step = TRANS ? 64 * p.ldp : 64, q_step = TRANS ? 64 * p.ldq : 64;
+    const unsigned char* pp =
+        reinterpret_cast<const unsigned char*>(p.p + (TRANS ? 0 : i0 * p.ldp) + (s0 / per) * p.pstep + in_part * p_step);
+    const unsigned char* qp =
+        reinterpret_cast<const unsigned char*>(p.q + (TRANS ? 0 : j0 * p.ldq) + (s0 / per) * p.qstep + in_part * q_step);
+    const long p_jump = (p.pstep - (per - 1) * p_step) * 2, q_jump = (p.qstep - (per - 1) * q_step) * 2;
     // copies of the stage after the last one copied, into LDS from `to` on; past the end the last one again, which nobody reads
     auto fill = [&](int to) {
         unsigned char* base = lds + to;
@@ -60,25 +78,32 @@ __global__ __launch_bounds__(64 * WI * WJ) void bf16_product_kernel(Bf16Product 
         for (int i = 0; i < QC; ++i) copy_to_lds16(copy_source(qp), q_off[i], base + BI * 128 + (i * WAVES + wave) * 1024);
         const bool more = ++filled < s1, jump = in_part == per - 1;
         in_part = jump ? 0 : in_part + 1;
-        pp += more ? (jump ? p_jump : 128L) : 0L;
-        qp += more ? (jump ? q_jump : 128L) : 0L;
+        pp += more ? (jump ? p_jump : 2 * p_step) : 0L;
+        qp += more ? (jump ? q_jump : 2 * q_step) : 0L;
     };
     struct Fragments {
         bf16x8 p[FI], q[FJ];
     };
+    auto fragment = [&](const unsigned char* base, auto width, int f, int k) -> bf16x8 {     // the f-th 32 of an operand
+        if constexpr (TRANS) {
+            constexpr int kPitch = decltype(width)::value * 2;
+            const int row = k * 16 + half * 8 + (lane >> 2 & 3);        // (row + 4 has the same swap)
+            const unsigned char* at = base + row * kPitch + ((f ^ (row & 3)) * 64) + (lane >> 4 & 1) * 32 + (lane & 3) * 8;
+            const i16x4 a = read_transposed((lds_i16x4)at), b = read_transposed((lds_i16x4)(at + 4 * kPitch));
+            return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            const int row = f * 32 + l32;
+            return *reinterpret_cast<const bf16x8*>(base + row * 128 + (((2 * k + half) ^ (row & 7)) * 16));
+        }
+    };
     auto read = [&](int at, int k, Fragments& f) {
         const unsigned char* base = lds + at;
 #pragma unroll
-        for (int j = 0; j < FJ; ++j) {
-            const int row = BI + (wj * FJ + j) * 32 + l32;
-            f.q[j] = *reinterpret_cast<const bf16x8*>(base + row * 128 + (((2 * k + half) ^ (row & 7)) * 16));
-        }
+        for (int j = 0; j < FJ; ++j) f.q[j] = fragment(base + BI * 128, std::integral_constant<int, BJ>(), wj * FJ + j, k);
 #pragma unroll
-        for (int i = 0; i < FI; ++i) {
-            const int row = (wi * FI + i) * 32 + l32;
-            f.p[i] = *reinterpret_cast<const bf16x8*>(base + row * 128 + (((2 * k + half) ^ (row & 7)) * 16));
-        }
+        for (int i = 0; i < FI; ++i) f.p[i] = fragment(base, std::integral_constant<int, BI>(), wi * FI + i, k);
     };
+    constexpr int READS = (FI + FJ) * (TRANS ? 2 : 1);
     f32x16 acc[FJ][FI];
 #pragma unroll
     for (int j = 0; j < FJ; ++j)
@@ -103,7 +128,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void bf16_product_kernel(Bf16Product 
         for (int k = 0; k < 3; ++k) {
             read(at, k + 1, f[(k + 1) % 2]);
             multiply(f[k % 2]);
-            interleave<FI * FJ, FI + FJ, 0>();
+            interleave<FI * FJ, READS, 0>();
         }
         landed_barrier<(STAGES - 2) * COPIES>();        // the next stage is there; STAGES - 2 more are on their way
         const int freed = at;
@@ -111,7 +136,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void bf16_product_kernel(Bf16Product 
         read(at, 0, f[0]);
         fill(freed);
         multiply(f[1]);
-        interleave<FI * FJ, FI + FJ, COPIES>();
+        interleave<FI * FJ, READS, COPIES>();
     }
     landed_barrier<0>();        // (no copy is in flight when the workgroup gives its LDS back)
     float* stage = reinterpret_cast<float*>(lds) + wave * 32 * (32 * FJ + 4);
@@ -146,11 +171,11 @@ size_t bf16_product_workspace(int rows, int cols, int parts, int depth) {
     return slab_bytes(bf16_plan(rows, cols, parts, depth).splits, rows, cols);
 }
 
-template <typename T, int BI, int BJ, int WI, int WJ>
+template <bool TRANS, typename T, int BI, int BJ, int WI, int WJ>
 static int launch_bf16(const Bf16Product& p, T* out, float* slabs, int splits, bool vec, hipStream_t st, const char* what) {
     // 128 x 128: two workgroups a CU
     constexpr int STAGES = BI + BJ == 384 ? 3 : 2, LDS = STAGES * (BI + BJ) * 128;
-    auto kernel = bf16_product_kernel<T, BI, BJ, WI, WJ, STAGES>;
+    auto kernel = bf16_product_kernel<T, BI, BJ, WI, WJ, STAGES, TRANS>;
     static std::atomic<unsigned long> devices{0};
     const hipError_t set = allow_lds(reinterpret_cast<const void*>(kernel), LDS, devices);
     if (set != hipSuccess) return fail("%s: %d bytes of LDS refused: %s", what, LDS, hipGetErrorString(set));
@@ -159,19 +184,19 @@ static int launch_bf16(const Bf16Product& p, T* out, float* slabs, int splits, b
     return 0;
 }
 
-template <typename T>
+template <bool TRANS, typename T>
 int bf16_product(const Bf16Product& p, T* out, void* ws, hipStream_t st, const char* what) {
     const Bf16Plan plan = bf16_plan(p.rows, p.cols, p.parts, p.depth);
     const bool vec = p.cols * sizeof(T) % 16 == 0 && aligned16(out), vec4 = vec && aligned16(p.bias);
     float* slabs = plan.splits > 1 ? static_cast<float*>(ws) : nullptr;
-    const int rc = plan.tile == BF16_256       ? launch_bf16<T, 256, 256, 2, 4>(p, out, slabs, plan.splits, vec, st, what)
-                   : plan.tile == BF16_256_128 ? launch_bf16<T, 256, 128, 4, 2>(p, out, slabs, plan.splits, vec, st, what)
-                                               : launch_bf16<T, 128, 128, 2, 2>(p, out, slabs, plan.splits, vec, st, what);
+    const int rc = plan.tile == BF16_256       ? launch_bf16<TRANS, T, 256, 256, 2, 4>(p, out, slabs, plan.splits, vec, st, what)
+                   : plan.tile == BF16_256_128 ? launch_bf16<TRANS, T, 256, 128, 4, 2>(p, out, slabs, plan.splits, vec, st, what)
+                                               : launch_bf16<TRANS, T, 128, 128, 2, 2>(p, out, slabs, plan.splits, vec, st, what);
     if (rc) return rc;
     if (slabs) join_slabs(slabs, plan.splits, out, (long)p.rows, p.cols, p.bias, p.accumulate, vec4, st);
     return check_launch(what);
 }
-template int bf16_product<float>(const Bf16Product&, float*, void*, hipStream_t, const char*);
+template int bf16_product<false, float>(const Bf16Product&, float*, void*, hipStream_t, const char*);
 
 // ------------------------------------------------------------------------------------------------ operand images
 // Part `part` of the exact split of v into bf16 values, largest first.  By truncation: it cannot overflow, and what is left is
@@ -193,116 +218,56 @@ template <> struct Parts<float> { static constexpr int n = 3; };
 
 __host__ __device__ __forceinline__ long to64(long n) { return (n + 63) / 64 * 64; }
 
-// dY [rows][n] -> parts [rows][n filled up to 64] bf16.
+// dY [rows][n] -> parts [rows filled up to 64][n filled up to 64] bf16, and the sums of 64 rows of each column (for dbias); either may
+// be null.  A workgroup takes 64 rows x 256 columns, a thread 8 rows x 8 columns.
 template <typename T>
-__global__ __launch_bounds__(256) void split_rows_kernel(const T* __restrict__ y, bf16_t* __restrict__ out, long rows, int n,
-                                                         bool vec) {
-    const long np = to64(n), chunks = np / 8, total = rows * chunks;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
-        const long row = i / chunks;
-        const int i0 = (int)(i - row * chunks) * 8;
-        float v[8];
-        load8(y + row * n, i0, i0 < n ? n : 0, vec, v);
+__global__ __launch_bounds__(256) void split_kernel(const T* __restrict__ y, bf16_t* __restrict__ out, float* __restrict__ colsum,
+                                                    int rows, int n, bool vec) {
+    __shared__ float red[8][256];
+    const int rp = (int)to64(rows), np = (int)to64(n);
+    const int t = threadIdx.x % 32, group = threadIdx.x / 32, i0 = blockIdx.x * 256 + t * 8, r0 = blockIdx.y * 64 + group;
+    float s[8] = {}, v[8][8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const int row = r0 + 8 * k;
+        load8(y + (long)min(row, rows - 1) * n, i0, row < rows && i0 < n ? n : 0, vec, v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] += v[k][j];
+        if (!out || i0 >= np) continue;
 #pragma unroll
         for (int part = 0; part < Parts<T>::n; ++part) {
             bf16x8 b;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) b[j] = split_part(v[j], part);
-            *reinterpret_cast<bf16x8*>(out + (part * rows + row) * np + i0) = b;
+            for (int j = 0; j < 8; ++j) b[j] = split_part(v[k][j], part);
+            *reinterpret_cast<bf16x8*>(out + ((long)part * rp + r0 + 8 * k) * np + i0) = b;
         }
     }
-}
-
-// dY [rows][n] -> parts [n][rows filled up to 64] bf16, and the sums of 64 rows of each column (dbias).  64 x 64 tiles through
-// LDS.
-template <typename T>
-__global__ __launch_bounds__(256) void split_transpose_kernel(const T* __restrict__ y, bf16_t* __restrict__ out,
-                                                              float* __restrict__ colsum, int rows, int n, bool vec) {
-    __shared__ float tile[64][65];
-    const long rp = to64(rows);
-    const int n0 = blockIdx.x * 64, r0 = blockIdx.y * 64, t = threadIdx.x;
+    if (!colsum) return;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int row = h * 32 + t / 8, i0 = n0 + (t % 8) * 8;
-        float v[8];
-        load8(y + (long)min(r0 + row, rows - 1) * n, i0, r0 + row < rows && i0 < n ? n : 0, vec, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) tile[row][(t % 8) * 8 + j] = v[j];
-    }
+    for (int j = 0; j < 8; ++j) red[group][t * 8 + j] = s[j];
     __syncthreads();
+    const int col = blockIdx.x * 256 + threadIdx.x;
+    float total = 0.f;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int col = h * 32 + t / 8, r8 = (t % 8) * 8;
-        float v[8], s = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[j] = tile[r8 + j][col];
-            s += v[j];
-        }
-        if (n0 + col < n) {
-#pragma unroll
-            for (int part = 0; part < Parts<T>::n; ++part) {
-                bf16x8 b;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) b[j] = split_part(v[j], part);
-                *reinterpret_cast<bf16x8*>(out + ((long)part * n + n0 + col) * rp + r0 + r8) = b;
-            }
-        }
-        s += __shfl_xor(s, 1, 64);
-        s += __shfl_xor(s, 2, 64);
-        s += __shfl_xor(s, 4, 64);
-        if (colsum && (t & 7) == 0 && n0 + col < n) colsum[(long)blockIdx.y * n + n0 + col] = s;
-    }
+    for (int g = 0; g < 8; ++g) total += red[g][threadIdx.x];
+    if (col < n) colsum[(long)blockIdx.y * n + col] = total;
 }
 
-// A [rows][in] microscaled -> [in][rows filled up to 64] bf16, 64 rows x 64 values a workgroup.
-template <int FMT>
-__global__ __launch_bounds__(256) void mx_rows_transpose_kernel(const unsigned char* __restrict__ codes,
-                                                                const unsigned char* __restrict__ scales, bf16_t* __restrict__ out,
-                                                                int rows, int in_dim) {
-    __shared__ bf16_t tile[64][66];
-    const long rp = to64(rows), pitch = mx_groups(in_dim) * 16L;
-    const int k0 = blockIdx.x * 64, r0 = blockIdx.y * 64, t = threadIdx.x;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int row = h * 32 + t / 8;
-        bf16x8 b;
-        if (r0 + row < rows) {
-            const long at = (long)(r0 + row) * pitch + k0 / 8 + t % 8;
-            const float s = mx_scale(scales[at / 4]);
-            if constexpr (FMT == GAN_MX_E4M3) {
-                const uint2 u = *reinterpret_cast<const uint2*>(codes + at * 8);
-                b = e4m3_to_bf16(u.x, u.y, s);
-            } else {
-                b = e2m1_to_bf16(*reinterpret_cast<const unsigned*>(codes + at * 4), s);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) b[j] = (bf16_t)0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) tile[row][(t % 8) * 8 + j] = b[j];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int col = h * 32 + t / 8, r8 = (t % 8) * 8;
-        if (k0 + col >= in_dim) continue;
-        bf16x8 b;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) b[j] = tile[r8 + j][col];
-        *reinterpret_cast<bf16x8*>(out + (long)(k0 + col) * rp + r0 + r8) = b;
-    }
-}
-
+// A microscaled [rows][groups * 128] -> bf16, by eights: `live` of them, then zeros up to `total`.
 template <int FMT>
 __global__ __launch_bounds__(256) void mx_rows_bf16_kernel(const unsigned char* __restrict__ codes,
                                                            const unsigned char* __restrict__ scales, bf16_t* __restrict__ out,
-                                                           long total) {
+                                                           long live, long total) {
     for (long at = (long)blockIdx.x * 256 + threadIdx.x; at < total; at += (long)gridDim.x * 256) {
-        const float s = mx_scale(scales[at / 4]);
+        const float s = at < live ? mx_scale(scales[at / 4]) : 0.f;
         bf16x8 b;
-        if constexpr (FMT == GAN_MX_E4M3) {
+        if (at >= live) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) b[j] = (bf16_t)0.f;
+        } else if constexpr (FMT == GAN_MX_E4M3) {
             const uint2 u = *reinterpret_cast<const uint2*>(codes + at * 8);
             b = e4m3_to_bf16(u.x, u.y, s);
         } else {
@@ -373,12 +338,12 @@ static dim3 flat_grid(long items) {
     return dim3((unsigned)(blocks < 8192 ? (blocks < 1 ? 1 : blocks) : 8192));
 }
 
-void mx_rows_to_bf16(int fmt, const void* codes, const void* scales, bf16_t* out, long rows, int in_dim, hipStream_t st) {
-    const long total = rows * mx_groups(in_dim) * 16;
+void mx_rows_to_bf16(int fmt, const void* codes, const void* scales, bf16_t* out, long rows, long filled, int in_dim, hipStream_t st) {
+    const long live = rows * mx_groups(in_dim) * 16, total = filled * mx_groups(in_dim) * 16;
     const unsigned char* c = static_cast<const unsigned char*>(codes);
     const unsigned char* s = static_cast<const unsigned char*>(scales);
-    if (fmt == GAN_MX_E4M3) hipLaunchKernelGGL(mx_rows_bf16_kernel<GAN_MX_E4M3>, flat_grid(total), dim3(256), 0, st, c, s, out, total);
-    else hipLaunchKernelGGL(mx_rows_bf16_kernel<GAN_MX_E2M1>, flat_grid(total), dim3(256), 0, st, c, s, out, total);
+    if (fmt == GAN_MX_E4M3) hipLaunchKernelGGL(mx_rows_bf16_kernel<GAN_MX_E4M3>, flat_grid(total), dim3(256), 0, st, c, s, out, live, total);
+    else hipLaunchKernelGGL(mx_rows_bf16_kernel<GAN_MX_E2M1>, flat_grid(total), dim3(256), 0, st, c, s, out, live, total);
 }
 
 void mx_weights_to_bf16(const void* codes, const void* scales, bf16_t* out, int in_dim, int out_dim, hipStream_t st) {
@@ -389,8 +354,95 @@ void mx_weights_to_bf16(const void* codes, const void* scales, bf16_t* out, int 
 
 static int parts_of(int dtype) { return dtype == GAN_BF16 ? 1 : dtype == GAN_F16 ? 2 : 3; }
 
-// dY itself is the operand of dA when it is bf16 in whole 64s.
-static bool dy_as_is(int dtype, int out_dim) { return dtype == GAN_BF16 && out_dim % 64 == 0; }
+// The gradients of one product, dx and dmatrix both or either, with their images' places in the workspace.
+struct Gradients {
+    int dtype, fmt, rows, in_dim, out_dim;
+    const void *a_codes, *a_scales, *w_codes, *w_scales, *dy;
+    void* dx;
+    float *dmatrix, *dbias;
+    int accumulate;
+};
+struct GradientImages {
+    bool as_is;                     // dY itself is the operand: bf16, nothing to fill up
+    long ldy, rp, kp;               // row strides of dY's image and of A's; rows of both
+    size_t y, w, a, colsum, slabs, bytes;       // offsets
+};
+
+static GradientImages gradient_images(int dtype, int rows, int in_dim, int out_dim, bool dx, bool dmatrix) {
+    GradientImages g;
+    // (dx contracts over outputs, dmatrix over rows: steps of 64)
+    g.as_is = dtype == GAN_BF16 && (!dx || out_dim % 64 == 0) && (!dmatrix || (rows % 64 == 0 && out_dim % 8 == 0));
+    g.ldy = g.as_is ? out_dim : to64(out_dim);
+    g.rp = to64(rows);
+    g.kp = mx_groups(in_dim) * 128L;
+    const int parts = parts_of(dtype);
+    const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+    size_t slabs = 0;
+    if (dx) slabs = bf16_product_workspace(rows, in_dim, parts, (int)to64(out_dim));
+    if (dmatrix) {
+        const size_t more = bf16_product_workspace(in_dim, out_dim, parts, (int)g.rp);
+        slabs = more > slabs ? more : slabs;
+    }
+    g.y = 0;
+    g.w = g.y + (g.as_is ? 0 : up((size_t)parts * g.rp * g.ldy * 2));
+    g.a = g.w + (dx ? up((size_t)in_dim * to64(out_dim) * 2) : 0);
+    g.colsum = g.a + (dmatrix ? up((size_t)g.rp * g.kp * 2) : 0);
+    g.slabs = g.colsum + (dmatrix ? up((size_t)g.rp / 64 * out_dim * 4) : 0);
+    g.bytes = g.slabs + slabs;
+    return g;
+}
+
+static bool gradient_sizes_ok(int rows, int in_dim, int out_dim) {
+    return rows <= GAN_MX_MAX_ROWS && in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1 && out_dim <= GAN_MX_MAX_IN;
+}
+static size_t gradient_bytes(int dtype, int rows, int in_dim, int out_dim, bool dx, bool dmatrix) {
+    if (rows < 1 || !gradient_sizes_ok(rows, in_dim, out_dim) || !dtype_ok(dtype)) return 0;
+    return gradient_images(dtype, rows, in_dim, out_dim, dx, dmatrix).bytes;
+}
+
+static int gradients(const Gradients& g, void* ws, size_t ws_bytes, hipStream_t st, const char* what) {
+    const bool dm = g.dmatrix != nullptr, dx = g.dx != nullptr;
+    GAN_CHECK_ARG(dtype_ok(g.dtype) && mx_fmt_ok(g.fmt), "%s: unknown element type %d or format %d", what, g.dtype, g.fmt);
+    GAN_CHECK_ARG(g.rows >= (dm ? 1 : 0) && gradient_sizes_ok(g.rows, g.in_dim, g.out_dim),
+                  "%s: %d rows, %d inputs, %d outputs (up to %d rows and %d of the others are served)", what, g.rows, g.in_dim,
+                  g.out_dim, GAN_MX_MAX_ROWS, GAN_MX_MAX_IN);
+    if (g.rows == 0) return 0;
+    GAN_CHECK_ARG(g.dy && (dx || dm) && (!dx || (g.w_codes && g.w_scales)) && (!dm || (g.a_codes && g.a_scales)), "%s: null pointer", what);
+    GAN_CHECK_ARG(aligned16(g.dy) && aligned16(g.w_codes) && aligned16(g.a_codes) &&
+                  ((reinterpret_cast<size_t>(g.w_scales) | reinterpret_cast<size_t>(g.a_scales)) & 3) == 0,
+                  "%s: dy and codes have to be 16-byte and scales 4-byte aligned", what);
+    const GradientImages im = gradient_images(g.dtype, g.rows, g.in_dim, g.out_dim, dx, dm);
+    GAN_CHECK_ARG(im.bytes == 0 || (ws && aligned16(ws) && ws_bytes >= im.bytes),
+                  "%s: workspace of %zu bytes needed (16-byte aligned), %zu given", what, im.bytes, ws_bytes);
+    char* base = static_cast<char*>(ws);
+    float* colsum = dm && g.dbias ? reinterpret_cast<float*>(base + im.colsum) : nullptr;
+    bf16_t* w = reinterpret_cast<bf16_t*>(base + im.w);
+    bf16_t* a = reinterpret_cast<bf16_t*>(base + im.a);
+    bf16_t* image = im.as_is ? nullptr : reinterpret_cast<bf16_t*>(base + im.y);
+    const bf16_t* y = im.as_is ? static_cast<const bf16_t*>(g.dy) : image;
+    const int parts = parts_of(g.dtype), blocks = (int)(im.rp / 64);
+    const long np = to64(g.out_dim);
+    return with_dtype(g.dtype, [&](auto* tag) {
+        typedef typename std::remove_pointer<decltype(tag)>::type T;
+        if (image || colsum)
+            hipLaunchKernelGGL((split_kernel<T>), dim3((unsigned)((np + 255) / 256), blocks), dim3(256), 0, st, static_cast<const T*>(g.dy),
+                               image, colsum, g.rows, g.out_dim, g.out_dim * sizeof(T) % 16 == 0);
+        if (dm) {
+            if (g.dbias)
+                hipLaunchKernelGGL(mx_dbias_kernel, dim3((g.out_dim + 31) / 32), dim3(256), 0, st, colsum, g.dbias, blocks, g.out_dim,
+                                   g.accumulate);
+            mx_rows_to_bf16(g.fmt, g.a_codes, g.a_scales, a, g.rows, im.rp, g.in_dim, st);
+            const Bf16Product p{a, y, im.kp, im.ldy, 0, im.rp * im.ldy, parts, (int)im.rp, g.in_dim, g.out_dim, nullptr, g.accumulate};
+            if (const int rc = bf16_product<true>(p, g.dmatrix, base + im.slabs, st, what)) return rc;
+        }
+        if (!dx) return 0;
+        hipLaunchKernelGGL(mx_weights_transpose_kernel, dim3((unsigned)(np / 64), mx_groups(g.in_dim)), dim3(256), 0, st,
+                           static_cast<const unsigned char*>(g.w_codes), static_cast<const unsigned char*>(g.w_scales), w, g.in_dim,
+                           g.out_dim);
+        const Bf16Product p{y, w, im.ldy, np, im.rp * im.ldy, 0, parts, (int)np, g.rows, g.in_dim, nullptr, 0};
+        return bf16_product<false>(p, static_cast<T*>(g.dx), base + im.slabs, st, what);
+    });
+}
 
 }  // namespace gan
 
@@ -399,85 +451,38 @@ using namespace gan;
 extern "C" {
 
 size_t gan_mx_matmul_dgrad_workspace_bytes(int dtype, int rows, int in_dim, int out_dim) {
-    if (rows < 1 || rows > GAN_MX_MAX_ROWS || in_dim < 1 || in_dim > GAN_MX_MAX_IN || out_dim < 1 || out_dim > GAN_MX_MAX_IN || !dtype_ok(dtype)) return 0;
-    const size_t np = to64(out_dim), parts = parts_of(dtype);
-    return in_dim * np * 2 + (dy_as_is(dtype, out_dim) ? 0 : parts * rows * np * 2) +
-           bf16_product_workspace(rows, in_dim, (int)parts, (int)np);
+    return gradient_bytes(dtype, rows, in_dim, out_dim, true, false);
 }
 
 int gan_mx_matmul_dgrad(int dtype, int rows, int in_dim, int out_dim, const void* dy, const void* w_codes, const void* w_scales,
                         void* dx, void* ws, size_t ws_bytes, gan_stream_t stream) {
-    GAN_CHECK_ARG(dtype_ok(dtype), "gan_mx_matmul_dgrad: unknown element type %d", dtype);
-    GAN_CHECK_ARG(rows >= 0 && rows <= GAN_MX_MAX_ROWS && in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1 && out_dim <= GAN_MX_MAX_IN,
-                  "gan_mx_matmul_dgrad: %d rows, %d inputs, %d outputs (up to %d rows and %d of the others are served)", rows, in_dim, out_dim, GAN_MX_MAX_ROWS, GAN_MX_MAX_IN);
-    if (rows == 0) return 0;
-    GAN_CHECK_ARG(dy && w_codes && w_scales && dx, "gan_mx_matmul_dgrad: null pointer");
-    GAN_CHECK_ARG(aligned16(dy) && aligned16(w_codes) && (reinterpret_cast<size_t>(w_scales) & 3) == 0,
-                  "gan_mx_matmul_dgrad: dy and codes have to be 16-byte and scales 4-byte aligned");
-    const size_t need = gan_mx_matmul_dgrad_workspace_bytes(dtype, rows, in_dim, out_dim);
-    GAN_CHECK_ARG(ws && aligned16(ws) && ws_bytes >= need,
-                  "gan_mx_matmul_dgrad: workspace of %zu bytes needed (16-byte aligned), %zu given", need, ws_bytes);
-    const hipStream_t st = as_stream(stream);
-    const long np = to64(out_dim);
-    const int parts = parts_of(dtype);
-    bf16_t* w = static_cast<bf16_t*>(ws);
-    bf16_t* y = w + in_dim * np;
-    hipLaunchKernelGGL(mx_weights_transpose_kernel, dim3((unsigned)(np / 64), mx_groups(in_dim)), dim3(256), 0, st,
-                       static_cast<const unsigned char*>(w_codes), static_cast<const unsigned char*>(w_scales), w, in_dim, out_dim);
-    return with_dtype(dtype, [&](auto* tag) {
-        typedef typename std::remove_pointer<decltype(tag)>::type T;
-        const bf16_t* dyp = static_cast<const bf16_t*>(dy);
-        bf16_t* end = y;
-        if (!dy_as_is(dtype, out_dim)) {
-            hipLaunchKernelGGL((split_rows_kernel<T>), flat_grid(rows * np / 8), dim3(256), 0, st, static_cast<const T*>(dy), y,
-                               (long)rows, out_dim, out_dim * sizeof(T) % 16 == 0);
-            dyp = y;
-            end = y + (long)parts * rows * np;
-        }
-        const Bf16Product p{dyp, w, np, np, rows * np, 0, parts, (int)np, rows, in_dim, nullptr, 0};
-        return bf16_product(p, static_cast<T*>(dx), end, st, "gan_mx_matmul_dgrad");
-    });
+    GAN_CHECK_ARG(rows == 0 || dx, "gan_mx_matmul_dgrad: null pointer");
+    const Gradients g{dtype, GAN_MX_E4M3, rows, in_dim, out_dim, nullptr, nullptr, w_codes, w_scales, dy, dx, nullptr, nullptr, 0};
+    return gradients(g, ws, ws_bytes, as_stream(stream), "gan_mx_matmul_dgrad");
 }
 
 size_t gan_mx_matmul_wgrad_workspace_bytes(int dtype, int rows, int in_dim, int out_dim) {
-    if (rows < 1 || rows > GAN_MX_MAX_ROWS || in_dim < 1 || in_dim > GAN_MX_MAX_IN || out_dim < 1 || out_dim > GAN_MX_MAX_IN || !dtype_ok(dtype)) return 0;
-    const size_t rp = to64(rows), parts = parts_of(dtype);
-    return (in_dim + parts * out_dim) * rp * 2 + (rp / 64 * out_dim * 4 + 15) / 16 * 16 +
-           bf16_product_workspace(in_dim, out_dim, (int)parts, (int)rp);
+    return gradient_bytes(dtype, rows, in_dim, out_dim, false, true);
 }
 
 int gan_mx_matmul_wgrad(int dtype, int fmt, int rows, int in_dim, int out_dim, const void* a_codes, const void* a_scales,
                         const void* dy, float* dmatrix, float* dbias, int accumulate, void* ws, size_t ws_bytes,
                         gan_stream_t stream) {
-    GAN_CHECK_ARG(dtype_ok(dtype) && mx_fmt_ok(fmt), "gan_mx_matmul_wgrad: unknown element type %d or format %d", dtype, fmt);
-    GAN_CHECK_ARG(rows >= 1 && rows <= GAN_MX_MAX_ROWS && in_dim >= 1 && in_dim <= GAN_MX_MAX_IN && out_dim >= 1 && out_dim <= GAN_MX_MAX_IN,
-                  "gan_mx_matmul_wgrad: %d rows, %d inputs, %d outputs (up to %d rows and %d of the others are served)", rows, in_dim, out_dim, GAN_MX_MAX_ROWS, GAN_MX_MAX_IN);
-    GAN_CHECK_ARG(dy && a_codes && a_scales && dmatrix, "gan_mx_matmul_wgrad: null pointer");
-    GAN_CHECK_ARG(aligned16(dy) && aligned16(a_codes), "gan_mx_matmul_wgrad: dy and codes have to be 16-byte aligned");
-    const size_t need = gan_mx_matmul_wgrad_workspace_bytes(dtype, rows, in_dim, out_dim);
-    GAN_CHECK_ARG(ws && aligned16(ws) && ws_bytes >= need,
-                  "gan_mx_matmul_wgrad: workspace of %zu bytes needed (16-byte aligned), %zu given", need, ws_bytes);
-    const hipStream_t st = as_stream(stream);
-    const long rp = to64(rows);
-    const int parts = parts_of(dtype), blocks = (int)(rp / 64);
-    bf16_t* a = static_cast<bf16_t*>(ws);
-    bf16_t* y = a + in_dim * rp;
-    float* colsum = reinterpret_cast<float*>(y + (long)parts * out_dim * rp);
-    void* end = reinterpret_cast<char*>(colsum) + ((size_t)blocks * out_dim * 4 + 15) / 16 * 16;
-    const dim3 ga((in_dim + 63) / 64, blocks), gy((out_dim + 63) / 64, blocks);
-    const unsigned char* c = static_cast<const unsigned char*>(a_codes);
-    const unsigned char* s = static_cast<const unsigned char*>(a_scales);
-    if (fmt == GAN_MX_E4M3) hipLaunchKernelGGL(mx_rows_transpose_kernel<GAN_MX_E4M3>, ga, dim3(256), 0, st, c, s, a, rows, in_dim);
-    else hipLaunchKernelGGL(mx_rows_transpose_kernel<GAN_MX_E2M1>, ga, dim3(256), 0, st, c, s, a, rows, in_dim);
-    return with_dtype(dtype, [&](auto* tag) {
-        typedef typename std::remove_pointer<decltype(tag)>::type T;
-        hipLaunchKernelGGL((split_transpose_kernel<T>), gy, dim3(256), 0, st, static_cast<const T*>(dy), y,
-                           dbias ? colsum : nullptr, rows, out_dim, out_dim * sizeof(T) % 16 == 0);
-        if (dbias)
-            hipLaunchKernelGGL(mx_dbias_kernel, dim3((out_dim + 31) / 32), dim3(256), 0, st, colsum, dbias, blocks, out_dim, accumulate);
-        const Bf16Product p{a, y, rp, rp, 0, out_dim * rp, parts, (int)rp, in_dim, out_dim, nullptr, accumulate};
-        return bf16_product(p, dmatrix, end, st, "gan_mx_matmul_wgrad");
-    });
+    GAN_CHECK_ARG(dmatrix, "gan_mx_matmul_wgrad: null pointer");
+    const Gradients g{dtype, fmt, rows, in_dim, out_dim, a_codes, a_scales, nullptr, nullptr, dy, nullptr, dmatrix, dbias, accumulate};
+    return gradients(g, ws, ws_bytes, as_stream(stream), "gan_mx_matmul_wgrad");
+}
+
+size_t gan_mx_matmul_bwd_workspace_bytes(int dtype, int rows, int in_dim, int out_dim) {
+    return gradient_bytes(dtype, rows, in_dim, out_dim, true, true);
+}
+
+int gan_mx_matmul_bwd(int dtype, int fmt, int rows, int in_dim, int out_dim, const void* a_codes, const void* a_scales,
+                      const void* w_codes, const void* w_scales, const void* dy, void* dx, float* dmatrix, float* dbias,
+                      int accumulate, void* ws, size_t ws_bytes, gan_stream_t stream) {
+    GAN_CHECK_ARG(dx && dmatrix, "gan_mx_matmul_bwd: null pointer");
+    const Gradients g{dtype, fmt, rows, in_dim, out_dim, a_codes, a_scales, w_codes, w_scales, dy, dx, dmatrix, dbias, accumulate};
+    return gradients(g, ws, ws_bytes, as_stream(stream), "gan_mx_matmul_bwd");
 }
 
 }  // extern "C"

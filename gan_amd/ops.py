@@ -1108,19 +1108,25 @@ class _MxMatmulFn(torch.autograd.Function):
         dy = _dense16(dy)
         _lib.here(dy, ac)
         code, rows = _lib.dtype_code(dy.dtype), dy.numel() // out_dim
+        dx, sizes = None, (rows, in_dim, out_dim)
+        if ctx.needs_input_grad[0]:
+            dx = torch.empty(tuple(dy.shape[:-1]) + (in_dim,), dtype=dy.dtype, device=dy.device)
         if ctx.matrix is not None and ctx.matrix.wants_grad and rows:
             dm, acc = ctx.matrix.grad_target()
             db, accb = ctx.bias.grad_target()
             assert acc == accb
-            wp, wn, hold = _lib.scratch(_size(lib.gan_mx_matmul_wgrad_workspace_bytes, code, rows, in_dim, out_dim), dy.device)
-            check(lib.gan_mx_matmul_wgrad(code, _lib.MX_FORMATS[ctx.q[0]], rows, in_dim, out_dim, ac.data_ptr(), asc.data_ptr(),
-                                          dy.data_ptr(), ptr(dm), ptr(db), acc, wp, wn, stream()))
-        dx = None
-        if ctx.needs_input_grad[0]:
-            dx = torch.empty(tuple(dy.shape[:-1]) + (in_dim,), dtype=dy.dtype, device=dy.device)
-            wp, wn, hold = _lib.scratch(_size(lib.gan_mx_matmul_dgrad_workspace_bytes, code, rows, in_dim, out_dim), dy.device)
-            check(lib.gan_mx_matmul_dgrad(code, rows, in_dim, out_dim, dy.data_ptr(), wc.data_ptr(), wsc.data_ptr(), dx.data_ptr(),
-                                          wp, wn, stream()))
+            fmt = _lib.MX_FORMATS[ctx.q[0]]
+            if dx is None:
+                wp, wn, hold = _lib.scratch(_size(lib.gan_mx_matmul_wgrad_workspace_bytes, code, *sizes), dy.device)
+                check(lib.gan_mx_matmul_wgrad(code, fmt, *sizes, ac.data_ptr(), asc.data_ptr(), dy.data_ptr(), ptr(dm), ptr(db), acc,
+                                              wp, wn, stream()))
+            else:
+                wp, wn, hold = _lib.scratch(_size(lib.gan_mx_matmul_bwd_workspace_bytes, code, *sizes), dy.device)
+                check(lib.gan_mx_matmul_bwd(code, fmt, *sizes, ac.data_ptr(), asc.data_ptr(), wc.data_ptr(), wsc.data_ptr(),
+                                            dy.data_ptr(), dx.data_ptr(), ptr(dm), ptr(db), acc, wp, wn, stream()))
+        elif dx is not None:
+            wp, wn, hold = _lib.scratch(_size(lib.gan_mx_matmul_dgrad_workspace_bytes, code, *sizes), dy.device)
+            check(lib.gan_mx_matmul_dgrad(code, *sizes, dy.data_ptr(), wc.data_ptr(), wsc.data_ptr(), dx.data_ptr(), wp, wn, stream()))
         return (dx,) + (None,) * 7
 
 

@@ -381,6 +381,11 @@ size_t gan_mx_matmul_wgrad_workspace_bytes(int dtype, int rows, int in_dim, int 
 int gan_mx_matmul_wgrad(int dtype, int fmt, int rows, int in_dim, int out_dim, const void* a_codes,
                         const void* a_scales, const void* dy, float* dmatrix, float* dbias, int accumulate, void* ws,
                         size_t ws_bytes, gan_stream_t stream);
+/* both at once: dY is read and split one time */
+size_t gan_mx_matmul_bwd_workspace_bytes(int dtype, int rows, int in_dim, int out_dim);
+int gan_mx_matmul_bwd(int dtype, int fmt, int rows, int in_dim, int out_dim, const void* a_codes, const void* a_scales,
+                      const void* w_codes, const void* w_scales, const void* dy, void* dx, float* dmatrix, float* dbias,
+                      int accumulate, void* ws, size_t ws_bytes, gan_stream_t stream);
 
 /* ---- distillation from a teacher's top logits, fused with its gradient (extension; conventions of the losses above) ------
  * logits [rows][classes] of type dtype, row stride ld; teacher and index [rows][top], dense, index int32 or int64 by

@@ -728,3 +728,21 @@ def test_a_pass_is_captured_while_an_eager_one_lives():
         for a, b in zip(grads, want):
             assert torch.equal(a, b)
         step()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("rows,k,n", [(1, 40, 8), (63, 130, 24), (64, 100, 64), (128, 384, 72), (65, 30, 7), (192, 257, 320), (2048, 96, 512)])
+def test_gradients_apart_are_those_computed_together(rows, k, n, dtype):
+    """The three entry points agree to the bit: weights frozen, input without a gradient, both."""
+    from gan_amd import ops
+    g = gen(rows + k + n)
+    x, m, dy = normal(g, rows, k).to(dtype), normal(g, k, n), normal(g, rows, n).to(dtype)
+    with layer(Linear__Matrix=m, Linear__bias=torch.zeros(n, device='cuda')) as l:
+        xx = x.clone().requires_grad_(True)
+        dx, = torch.autograd.grad((ops.linear_mx(xx, n),), (xx,), (dy,))
+        both = [l.grad(v).clone() for v in ('Linear/Matrix', 'Linear/bias')]
+        l.group.begin_update()
+        torch.autograd.backward((ops.linear_mx(x, n),), (dy,))
+        alone = [l.grad(v).clone() for v in ('Linear/Matrix', 'Linear/bias')]
+    frozen, = torch.autograd.grad((ops.mx_matmul(xx, ops.mx_pack(m)),), (xx,), (dy,))
+    assert torch.equal(dx, frozen) and torch.equal(both[0], alone[0]) and torch.equal(both[1], alone[1])

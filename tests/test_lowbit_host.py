@@ -180,3 +180,17 @@ def test_a_capture_has_leaves_of_its_own(monkeypatch):
     first = ops._token_key(device, True)
     monkeypatch.setattr(ops, 'stream', lambda: 8)
     assert len({eager, first, ops._token_key(device, True)}) == 3
+
+
+def test_both_gradients_at_once_are_refused_without_their_parts():
+    from gan_amd import _lib as L
+    lib, p, odd = L.lib, FAKE, ctypes.c_void_p(4096 + 2)
+    need = lib.gan_mx_matmul_bwd_workspace_bytes(1, 64, 64, 64)
+    assert need > lib.gan_mx_matmul_dgrad_workspace_bytes(1, 64, 64, 64) > 0 and lib.gan_mx_matmul_bwd_workspace_bytes(1, 0, 64, 64) == 0
+    call = lambda rows=64, dy=p, dx=p, dm=p, a=p, n=need: lib.gan_mx_matmul_bwd(1, 0, rows, 64, 64, a, p, p, p, dy, dx, dm, None, 0, p, n, None)
+    _refused(call(rows=0), b"0 rows")
+    _refused(call(dx=None), b"null")
+    _refused(call(dm=None), b"null")
+    _refused(call(a=None), b"null")
+    _refused(call(dy=odd), b"aligned")
+    _refused(call(n=need - 1), b"workspace")
