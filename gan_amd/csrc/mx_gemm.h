@@ -167,7 +167,8 @@ inline int contraction_splits(long tiles, int workgroups, int steps, int least) 
     return s < 1 ? 1 : (int)s;
 }
 
-// The bf16-pipe product of mx_grad.hip: C[i][j] (+)= bias[j] + sum over parts and c of P[i][c] Q[j][c], or (TRANS) P[c][i] Q[c][j].
+// The bf16-pipe product of mx_grad.hip: C[i][j] (+)= bias[j] + sum over parts and c of P[i][c] Q[j][c], with PT of P[c][i],
+// with QT of Q[c][j].
 struct Bf16Product {
     const bf16_t* p;
     const bf16_t* q;
@@ -178,11 +179,11 @@ struct Bf16Product {
     int accumulate;
 };
 size_t bf16_product_workspace(int rows, int cols, int parts, int depth);
-template <bool TRANS, typename T>
+template <bool PT, bool QT, typename T>
 int bf16_product(const Bf16Product& p, T* out, void* ws, hipStream_t st, const char* what);
 
-// [filled][groups * 128] bf16 (rows and then zeros) and [out][groups * 128] bf16 of microscaled operands.
+// [filled][groups * 128] bf16 of microscaled operands: rows (outputs) and then zeros.
 void mx_rows_to_bf16(int fmt, const void* codes, const void* scales, bf16_t* out, long rows, long filled, int in_dim, hipStream_t st);
-void mx_weights_to_bf16(const void* codes, const void* scales, bf16_t* out, int in_dim, int out_dim, hipStream_t st);
+void mx_weights_to_bf16(const void* codes, const void* scales, bf16_t* out, int in_dim, int out_dim, int filled, hipStream_t st);
 
 }  // namespace gan

@@ -7,8 +7,8 @@
 // products are summed in fp32.  So a gradient carries the error of an fp32 sum of exact products whatever the type.
 //
 // Memory-bound passes turn the operands into bf16 images whose contraction axis is filled up with zeros to a multiple of 64 -- one
-// image of dY for both products, none where dY is bf16 in whole 64s --, then one compute-bound kernel runs each product.  The forward
-// and dA contract over contiguous values, dW over rows (TRANS).
+// image of dY for both products, none where dY is bf16 in whole 64s --, then one compute-bound kernel runs each product.  It takes
+// operands that contract over contiguous values (dY for dA) and over rows (W for dA, A and dY for dW) as they are.
 #include "mx_gemm.h"
 
 namespace gan {
@@ -26,10 +26,10 @@ __device__ __forceinline__ i16x4 read_transposed(lds_i16x4 __restrict__ from) { 
 // Large tiles have two waves a SIMD with 128 x 64 outputs each: LDS then gives 96 bytes a clock of its 128; one wave of
 // 128 x 128 needs less of it, but nothing covers its waits (4096^3: 126 us against 115, the weights' image included).
 // 4096 x 4096 x 8192: 1.25 PF/s, a library product of that size 1.45.
-// TRANS: the operands lie the other way round, [contraction][rows of C] and [contraction][columns of C], as a gradient of weights
-// has them.  A stage then is 64 rows of BI and of BJ values, its 64-byte pieces swapped by row; a fragment, eight consecutive of the
-// contraction for each of 32 values, is read by the LDS's transposing read: 16 lanes fetch 4 x 16 values, lane i keeps column i.
-template <typename T, int BI, int BJ, int WI, int WJ, int STAGES, bool TRANS>
+// PT, QT: an operand lies the other way round, [contraction][rows (columns) of C].  Its part of a stage then is 64 rows of BI (BJ)
+// values, their 64-byte pieces swapped by row; a fragment, eight consecutive of the contraction for each of 32 values, is read by the
+// LDS's transposing read: 16 lanes fetch 4 x 16 values, lane i keeps column i.
+template <typename T, int BI, int BJ, int WI, int WJ, int STAGES, bool PT, bool QT>
 __global__ __launch_bounds__(64 * WI * WJ) void bf16_product_kernel(Bf16Product p, T* out, float* slabs, int splits, bool vec) {
     constexpr int WAVES = WI * WJ, THREADS = 64 * WAVES, FI = BI / WI / 32, FJ = BJ / WJ / 32, STAGE = (BI + BJ) * 128;
     constexpr int COPIES = STAGE / 16 / THREADS;        // of a wave for a stage
@@ -46,9 +46,9 @@ __global__ __launch_bounds__(64 * WI * WJ) void bf16_product_kernel(Bf16Product 
     // where this lane's copies begin, and the two operands' places in the part at hand (rows beyond the last: the last again)
     constexpr int PC = BI * 8 / THREADS, QC = BJ * 8 / THREADS;
     unsigned p_off[PC], q_off[QC];
-    auto offset = [&](int at, auto width, int first, int last, long ld) -> unsigned {
+    auto offset = [&](auto trans, int at, auto width, int first, int last, long ld) -> unsigned {
         constexpr int kChunks = decltype(width)::value / 8;
-        if constexpr (TRANS) {      // (chunks beyond the row: its last again)
+        if constexpr (decltype(trans)::value) {      // (chunks beyond the row: its last again)
             const int k = at / kChunks, chunk = at % kChunks ^ (k & 3) << 2;
             return (unsigned)k * (unsigned)(ld * 2) + (unsigned)min(first + chunk * 8, (int)ld - 8) * 2u;
         } else {
@@ -58,16 +58,16 @@ __global__ __launch_bounds__(64 * WI * WJ) void bf16_product_kernel(Bf16Product 
     };
 #pragma unroll
     for (int i = 0; i < PC; ++i)
-        p_off[i] = offset((i * WAVES + wave) * 64 + lane, std::integral_constant<int, BI>(), i0, p.rows - 1, p.ldp);
+        p_off[i] = offset(std::bool_constant<PT>(), (i * WAVES + wave) * 64 + lane, std::integral_constant<int, BI>(), i0, p.rows - 1, p.ldp);
 #pragma unroll
     for (int i = 0; i < QC; ++i)
-        q_off[i] = offset((i * WAVES + wave) * 64 + lane, std::integral_constant<int, BJ>(), j0, p.cols - 1, p.ldq);
+        q_off[i] = offset(std::bool_constant<QT>(), (i * WAVES + wave) * 64 + lane, std::integral_constant<int, BJ>(), j0, p.cols - 1, p.ldq);
     int filled = s0, in_part = s0 % per;
-    const long p_step = TRANS ? 64 * p.ldp : 64, q_step = TRANS ? 64 * p.ldq : 64;
+    const long p_step = PT ? 64 * p.ldp : 64, q_step = QT ? 64 * p.ldq : 64;
     const unsigned char* pp =
-        reinterpret_cast<const unsigned char*>(p.p + (TRANS ? 0 : i0 * p.ldp) + (s0 / per) * p.pstep + in_part * p_step);
+        reinterpret_cast<const unsigned char*>(p.p + (PT ? 0 : i0 * p.ldp) + (s0 / per) * p.pstep + in_part * p_step);
     const unsigned char* qp =
-        reinterpret_cast<const unsigned char*>(p.q + (TRANS ? 0 : j0 * p.ldq) + (s0 / per) * p.qstep + in_part * q_step);
+        reinterpret_cast<const unsigned char*>(p.q + (QT ? 0 : j0 * p.ldq) + (s0 / per) * p.qstep + in_part * q_step);
     const long p_jump = (p.pstep - (per - 1) * p_step) * 2, q_jump = (p.qstep - (per - 1) * q_step) * 2;
     // copies of the stage after the last one copied, into LDS from `to` on; past the end the last one again, which nobody reads
     auto fill = [&](int to) {
@@ -84,8 +84,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void bf16_product_kernel(Bf16Product 
     struct Fragments {
         bf16x8 p[FI], q[FJ];
     };
-    auto fragment = [&](const unsigned char* base, auto width, int f, int k) -> bf16x8 {     // the f-th 32 of an operand
-        if constexpr (TRANS) {
+    auto fragment = [&](auto trans, const unsigned char* base, auto width, int f, int k) -> bf16x8 {     // the f-th 32 of an operand
+        if constexpr (decltype(trans)::value) {
             constexpr int kPitch = decltype(width)::value * 2;
             const int row = k * 16 + half * 8 + (lane >> 2 & 3);        // (row + 4 has the same swap)
             const unsigned char* at = base + row * kPitch + ((f ^ (row & 3)) * 64) + (lane >> 4 & 1) * 32 + (lane & 3) * 8;
@@ -99,11 +99,11 @@ __global__ __launch_bounds__(64 * WI * WJ) void bf16_product_kernel(Bf16Product 
     auto read = [&](int at, int k, Fragments& f) {
         const unsigned char* base = lds + at;
 #pragma unroll
-        for (int j = 0; j < FJ; ++j) f.q[j] = fragment(base + BI * 128, std::integral_constant<int, BJ>(), wj * FJ + j, k);
+        for (int j = 0; j < FJ; ++j) f.q[j] = fragment(std::bool_constant<QT>(), base + BI * 128, std::integral_constant<int, BJ>(), wj * FJ + j, k);
 #pragma unroll
-        for (int i = 0; i < FI; ++i) f.p[i] = fragment(base, std::integral_constant<int, BI>(), wi * FI + i, k);
+        for (int i = 0; i < FI; ++i) f.p[i] = fragment(std::bool_constant<PT>(), base, std::integral_constant<int, BI>(), wi * FI + i, k);
     };
-    constexpr int READS = (FI + FJ) * (TRANS ? 2 : 1);
+    constexpr int READS = FI * (PT ? 2 : 1) + FJ * (QT ? 2 : 1);
     f32x16 acc[FJ][FI];
 #pragma unroll
     for (int j = 0; j < FJ; ++j)
@@ -171,11 +171,11 @@ size_t bf16_product_workspace(int rows, int cols, int parts, int depth) {
     return slab_bytes(bf16_plan(rows, cols, parts, depth).splits, rows, cols);
 }
 
-template <bool TRANS, typename T, int BI, int BJ, int WI, int WJ>
+template <bool PT, bool QT, typename T, int BI, int BJ, int WI, int WJ>
 static int launch_bf16(const Bf16Product& p, T* out, float* slabs, int splits, bool vec, hipStream_t st, const char* what) {
     // 128 x 128: two workgroups a CU
     constexpr int STAGES = BI + BJ == 384 ? 3 : 2, LDS = STAGES * (BI + BJ) * 128;
-    auto kernel = bf16_product_kernel<T, BI, BJ, WI, WJ, STAGES, TRANS>;
+    auto kernel = bf16_product_kernel<T, BI, BJ, WI, WJ, STAGES, PT, QT>;
     static std::atomic<unsigned long> devices{0};
     const hipError_t set = allow_lds(reinterpret_cast<const void*>(kernel), LDS, devices);
     if (set != hipSuccess) return fail("%s: %d bytes of LDS refused: %s", what, LDS, hipGetErrorString(set));
@@ -184,19 +184,19 @@ static int launch_bf16(const Bf16Product& p, T* out, float* slabs, int splits, b
     return 0;
 }
 
-template <bool TRANS, typename T>
+template <bool PT, bool QT, typename T>
 int bf16_product(const Bf16Product& p, T* out, void* ws, hipStream_t st, const char* what) {
     const Bf16Plan plan = bf16_plan(p.rows, p.cols, p.parts, p.depth);
     const bool vec = p.cols * sizeof(T) % 16 == 0 && aligned16(out), vec4 = vec && aligned16(p.bias);
     float* slabs = plan.splits > 1 ? static_cast<float*>(ws) : nullptr;
-    const int rc = plan.tile == BF16_256       ? launch_bf16<TRANS, T, 256, 256, 2, 4>(p, out, slabs, plan.splits, vec, st, what)
-                   : plan.tile == BF16_256_128 ? launch_bf16<TRANS, T, 256, 128, 4, 2>(p, out, slabs, plan.splits, vec, st, what)
-                                               : launch_bf16<TRANS, T, 128, 128, 2, 2>(p, out, slabs, plan.splits, vec, st, what);
+    const int rc = plan.tile == BF16_256       ? launch_bf16<PT, QT, T, 256, 256, 2, 4>(p, out, slabs, plan.splits, vec, st, what)
+                   : plan.tile == BF16_256_128 ? launch_bf16<PT, QT, T, 256, 128, 4, 2>(p, out, slabs, plan.splits, vec, st, what)
+                                               : launch_bf16<PT, QT, T, 128, 128, 2, 2>(p, out, slabs, plan.splits, vec, st, what);
     if (rc) return rc;
     if (slabs) join_slabs(slabs, plan.splits, out, (long)p.rows, p.cols, p.bias, p.accumulate, vec4, st);
     return check_launch(what);
 }
-template int bf16_product<false, float>(const Bf16Product&, float*, void*, hipStream_t, const char*);
+template int bf16_product<false, false, float>(const Bf16Product&, float*, void*, hipStream_t, const char*);
 
 // ------------------------------------------------------------------------------------------------ operand images
 // Part `part` of the exact split of v into bf16 values, largest first.  By truncation: it cannot overflow, and what is left is
@@ -277,42 +277,20 @@ __global__ __launch_bounds__(256) void mx_rows_bf16_kernel(const unsigned char* 
     }
 }
 
-// Packed W -> [out][groups * 128] bf16: a lane writes one block, 64 bytes.
+// Packed W -> [filled][groups * 128] bf16, outputs and then zeros: a lane turns 8 codes of one output into 16 bytes, 16 lanes write
+// 256 bytes of a row.
 __global__ __launch_bounds__(256) void mx_weights_bf16_kernel(const unsigned char* __restrict__ codes,
                                                               const unsigned char* __restrict__ scales, bf16_t* __restrict__ out,
-                                                              int groups, int out_dim) {
-    // 4 blocks of 64 outputs; neighbouring lanes take the four blocks of one output, so that 256 bytes of a row are written
-    const int q = threadIdx.x & 3, n = blockIdx.x * 64 + threadIdx.x / 4, g = blockIdx.y;
-    if (n >= out_dim) return;
-    const uint4 u = reinterpret_cast<const uint4*>(codes)[((long)g * 4 + q) * out_dim + n];
-    const float s = mx_scale(scales[((long)g * out_dim + n) * 4 + q]);
-    bf16x8* o = reinterpret_cast<bf16x8*>(out + ((long)n * groups + g) * 128 + q * 32);
-    o[0] = e2m1_to_bf16(u.x, s);
-    o[1] = e2m1_to_bf16(u.y, s);
-    o[2] = e2m1_to_bf16(u.z, s);
-    o[3] = e2m1_to_bf16(u.w, s);
-}
-
-// Packed W -> [in][out filled up to 64] bf16: a lane takes one block of one output; the lanes of a wave are neighbouring
-// outputs, so each of the 32 stores is contiguous.
-__global__ __launch_bounds__(256) void mx_weights_transpose_kernel(const unsigned char* __restrict__ codes,
-                                                                   const unsigned char* __restrict__ scales,
-                                                                   bf16_t* __restrict__ out, int in_dim, int out_dim) {
-    const long np = to64(out_dim);
-    const int n = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6, k0 = blockIdx.y * 128 + q * 32;
-    uint4 u = make_uint4(0, 0, 0, 0);
-    float s = 1.f;
-    if (n < out_dim) {
-        u = reinterpret_cast<const uint4*>(codes)[((long)blockIdx.y * 4 + q) * out_dim + n];
-        s = mx_scale(scales[((long)blockIdx.y * out_dim + n) * 4 + q]);
-    }
-    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+                                                              int groups, int out_dim, int filled) {
+    const int c = threadIdx.x & 15, g = blockIdx.y;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const bf16x8 b = e2m1_to_bf16(w[i], s);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (k0 + i * 8 + j < in_dim) out[(long)(k0 + i * 8 + j) * np + n] = b[j];
+        const int n = blockIdx.x * 64 + i * 16 + threadIdx.x / 16;
+        if (n >= filled) continue;
+        const long at = min(n, out_dim - 1);
+        const unsigned u = reinterpret_cast<const unsigned*>(codes)[(((long)g * 4 + c / 4) * out_dim + at) * 4 + c % 4];
+        const float s = mx_scale(scales[((long)g * out_dim + at) * 4 + c / 4]);
+        *reinterpret_cast<bf16x8*>(out + ((long)n * groups + g) * 128 + c * 8) = e2m1_to_bf16(n < out_dim ? u : 0u, n < out_dim ? s : 1.f);
     }
 }
 
@@ -346,10 +324,10 @@ void mx_rows_to_bf16(int fmt, const void* codes, const void* scales, bf16_t* out
     else hipLaunchKernelGGL(mx_rows_bf16_kernel<GAN_MX_E2M1>, flat_grid(total), dim3(256), 0, st, c, s, out, live, total);
 }
 
-void mx_weights_to_bf16(const void* codes, const void* scales, bf16_t* out, int in_dim, int out_dim, hipStream_t st) {
-    hipLaunchKernelGGL(mx_weights_bf16_kernel, dim3((out_dim + 63) / 64, mx_groups(in_dim)), dim3(256), 0, st,
+void mx_weights_to_bf16(const void* codes, const void* scales, bf16_t* out, int in_dim, int out_dim, int filled, hipStream_t st) {
+    hipLaunchKernelGGL(mx_weights_bf16_kernel, dim3((filled + 63) / 64, mx_groups(in_dim)), dim3(256), 0, st,
                        static_cast<const unsigned char*>(codes), static_cast<const unsigned char*>(scales), out, mx_groups(in_dim),
-                       out_dim);
+                       out_dim, filled);
 }
 
 static int parts_of(int dtype) { return dtype == GAN_BF16 ? 1 : dtype == GAN_F16 ? 2 : 3; }
@@ -364,7 +342,7 @@ struct Gradients {
 };
 struct GradientImages {
     bool as_is;                     // dY itself is the operand: bf16, nothing to fill up
-    long ldy, rp, kp;               // row strides of dY's image and of A's; rows of both
+    long ldy, rp, kp;               // row strides of dY's image and of A's and W's; rows of the first two
     size_t y, w, a, colsum, slabs, bytes;       // offsets
 };
 
@@ -385,7 +363,7 @@ static GradientImages gradient_images(int dtype, int rows, int in_dim, int out_d
     }
     g.y = 0;
     g.w = g.y + (g.as_is ? 0 : up((size_t)parts * g.rp * g.ldy * 2));
-    g.a = g.w + (dx ? up((size_t)in_dim * to64(out_dim) * 2) : 0);
+    g.a = g.w + (dx ? up((size_t)to64(out_dim) * g.kp * 2) : 0);
     g.colsum = g.a + (dmatrix ? up((size_t)g.rp * g.kp * 2) : 0);
     g.slabs = g.colsum + (dmatrix ? up((size_t)g.rp / 64 * out_dim * 4) : 0);
     g.bytes = g.slabs + slabs;
@@ -433,14 +411,12 @@ static int gradients(const Gradients& g, void* ws, size_t ws_bytes, hipStream_t 
                                    g.accumulate);
             mx_rows_to_bf16(g.fmt, g.a_codes, g.a_scales, a, g.rows, im.rp, g.in_dim, st);
             const Bf16Product p{a, y, im.kp, im.ldy, 0, im.rp * im.ldy, parts, (int)im.rp, g.in_dim, g.out_dim, nullptr, g.accumulate};
-            if (const int rc = bf16_product<true>(p, g.dmatrix, base + im.slabs, st, what)) return rc;
+            if (const int rc = bf16_product<true, true>(p, g.dmatrix, base + im.slabs, st, what)) return rc;
         }
         if (!dx) return 0;
-        hipLaunchKernelGGL(mx_weights_transpose_kernel, dim3((unsigned)(np / 64), mx_groups(g.in_dim)), dim3(256), 0, st,
-                           static_cast<const unsigned char*>(g.w_codes), static_cast<const unsigned char*>(g.w_scales), w, g.in_dim,
-                           g.out_dim);
-        const Bf16Product p{y, w, im.ldy, np, im.rp * im.ldy, 0, parts, (int)np, g.rows, g.in_dim, nullptr, 0};
-        return bf16_product<false>(p, static_cast<T*>(g.dx), base + im.slabs, st, what);
+        mx_weights_to_bf16(g.w_codes, g.w_scales, w, g.in_dim, g.out_dim, (int)np, st);
+        const Bf16Product p{y, w, im.ldy, im.kp, im.rp * im.ldy, 0, parts, (int)np, g.rows, g.in_dim, nullptr, 0};
+        return bf16_product<false, true>(p, static_cast<T*>(g.dx), base + im.slabs, st, what);
     });
 }
 
