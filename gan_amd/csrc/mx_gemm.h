@@ -47,12 +47,14 @@ __device__ __forceinline__ void landed_barrier() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// Launch position -> tile.  Workgroups go to the 8 XCDs round robin, each with an L2 of its own: position p works on tile
-// (p % 8) * (tiles / 8) + p / 8, so that one XCD holds a contiguous run of tiles, and a run walks bands of 8 row tiles, so that
-// tiles in flight together share their operand rows and columns in that L2.
-__device__ __forceinline__ void tile_of(int p, int ti, int tj, int& i, int& j) {
-    const int total = ti * tj, per = total / 8, extra = total % 8, x = p % 8, q = p / 8;
-    const int t = x * per + min(x, extra) + q;
+// Launch position -> tile and part of the contraction.  Workgroups go to the 8 XCDs round robin, each with an L2 of its own: position
+// p works on item (p % 8) * (items / 8) + p / 8, so that one XCD holds a contiguous run, of whole parts first, and within a part the
+// run walks bands of 8 row tiles: workgroups in flight together share their operand rows and columns in that L2.
+__device__ __forceinline__ void tile_of(int p, int ti, int tj, int splits, int& i, int& j, int& split) {
+    const int total = ti * tj * splits, per = total / 8, extra = total % 8, x = p % 8, q = p / 8;
+    int t = x * per + min(x, extra) + q;
+    split = t / (ti * tj);
+    t -= split * ti * tj;
     const int band = t / (8 * tj), in = t - band * 8 * tj, high = min(8, ti - band * 8);
     i = band * 8 + in % high;
     j = in / high;

@@ -36,12 +36,12 @@ __global__ __launch_bounds__(64 * WI * WJ) void bf16_product_kernel(Bf16Product 
     extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wj = wave % WJ, wi = wave / WJ;
     const int l32 = lane & 31, half = lane >> 5;
-    int ti, tj;
-    tile_of(blockIdx.x, (p.rows + BI - 1) / BI, (p.cols + BJ - 1) / BJ, ti, tj);
+    int ti, tj, split;
+    tile_of(blockIdx.x, (p.rows + BI - 1) / BI, (p.cols + BJ - 1) / BJ, splits, ti, tj, split);
     const int i0 = ti * BI, j0 = tj * BJ;
-    const int per = p.depth / 64;
-    const long steps = (long)per * p.parts;
-    const int s0 = (int)(steps * blockIdx.y / splits), s1 = (int)(steps * (blockIdx.y + 1) / splits);
+    // the parts of one 64 follow each other: the operand they share then comes from the L2
+    const long steps = (long)(p.depth / 64) * p.parts;
+    const int s0 = (int)(steps * split / splits), s1 = (int)(steps * (split + 1) / splits);
 
     // where this lane's copies begin, and the two operands' places in the part at hand (rows beyond the last: the last again)
     constexpr int PC = BI * 8 / THREADS, QC = BJ * 8 / THREADS;
@@ -62,13 +62,13 @@ __global__ __launch_bounds__(64 * WI * WJ) void bf16_product_kernel(Bf16Product 
 #pragma unroll
     for (int i = 0; i < QC; ++i)
         q_off[i] = offset(std::bool_constant<QT>(), (i * WAVES + wave) * 64 + lane, std::integral_constant<int, BJ>(), j0, p.cols - 1, p.ldq);
-    int filled = s0, in_part = s0 % per;
+    int filled = s0, part = s0 % p.parts;
     const long p_step = PT ? 64 * p.ldp : 64, q_step = QT ? 64 * p.ldq : 64;
     const unsigned char* pp =
-        reinterpret_cast<const unsigned char*>(p.p + (PT ? 0 : i0 * p.ldp) + (s0 / per) * p.pstep + in_part * p_step);
+        reinterpret_cast<const unsigned char*>(p.p + (PT ? 0 : i0 * p.ldp) + s0 / p.parts * p_step + part * p.pstep);
     const unsigned char* qp =
-        reinterpret_cast<const unsigned char*>(p.q + (QT ? 0 : j0 * p.ldq) + (s0 / per) * p.qstep + in_part * q_step);
-    const long p_jump = (p.pstep - (per - 1) * p_step) * 2, q_jump = (p.qstep - (per - 1) * q_step) * 2;
+        reinterpret_cast<const unsigned char*>(p.q + (QT ? 0 : j0 * p.ldq) + s0 / p.parts * q_step + part * p.qstep);
+    const long p_jump = (p_step - (p.parts - 1) * p.pstep) * 2, q_jump = (q_step - (p.parts - 1) * p.qstep) * 2;
     // copies of the stage after the last one copied, into LDS from `to` on; past the end the last one again, which nobody reads
     auto fill = [&](int to) {
         unsigned char* base = lds + to;
@@ -76,10 +76,10 @@ __global__ __launch_bounds__(64 * WI * WJ) void bf16_product_kernel(Bf16Product 
         for (int i = 0; i < PC; ++i) copy_to_lds16(copy_source(pp), p_off[i], base + (i * WAVES + wave) * 1024);
 #pragma unroll
         for (int i = 0; i < QC; ++i) copy_to_lds16(copy_source(qp), q_off[i], base + BI * 128 + (i * WAVES + wave) * 1024);
-        const bool more = ++filled < s1, jump = in_part == per - 1;
-        in_part = jump ? 0 : in_part + 1;
-        pp += more ? (jump ? p_jump : 2 * p_step) : 0L;
-        qp += more ? (jump ? q_jump : 2 * q_step) : 0L;
+        const bool more = ++filled < s1, jump = part == p.parts - 1;
+        part = jump ? 0 : part + 1;
+        pp += more ? (jump ? p_jump : 2 * p.pstep) : 0L;
+        qp += more ? (jump ? q_jump : 2 * p.qstep) : 0L;
     };
     struct Fragments {
         bf16x8 p[FI], q[FJ];
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void bf16_product_kernel(Bf16Product 
     for (int i = 0; i < FI; ++i) {
         const int row0 = i0 + (wi * FI + i) * 32;
         auto pick = [&](int j) -> const f32x16& { return acc[j][i]; };
-        if (slabs) store_rows<float, FJ>(pick, stage, row0, col0, p.rows, n4, slabs + (long)blockIdx.y * p.rows * n4, n4, nullptr, 0, true);
+        if (slabs) store_rows<float, FJ>(pick, stage, row0, col0, p.rows, n4, slabs + (long)split * p.rows * n4, n4, nullptr, 0, true);
         else store_rows<T, FJ>(pick, stage, row0, col0, p.rows, p.cols, out, p.cols, p.bias, p.accumulate, vec);
     }
 }
@@ -180,7 +180,7 @@ static int launch_bf16(const Bf16Product& p, T* out, float* slabs, int splits, b
     const hipError_t set = allow_lds(reinterpret_cast<const void*>(kernel), LDS, devices);
     if (set != hipSuccess) return fail("%s: %d bytes of LDS refused: %s", what, LDS, hipGetErrorString(set));
     const long tiles = (long)((p.rows + BI - 1) / BI) * ((p.cols + BJ - 1) / BJ);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, splits), dim3(64 * WI * WJ), LDS, st, p, out, slabs, splits, vec);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles * splits), dim3(64 * WI * WJ), LDS, st, p, out, slabs, splits, vec);
     return 0;
 }
 

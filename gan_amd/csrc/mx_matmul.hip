@@ -49,10 +49,10 @@ __global__ __launch_bounds__(64 * WN * WR) void mx_tile_kernel(MxProduct p) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wr = wave / WN;
     const int l32 = lane & 31, half = lane >> 5;
     const int tr = (p.rows + BR - 1) / BR, tn = (p.n + BN - 1) / BN;
-    int ir, in;
-    tile_of(blockIdx.x, tr, tn, ir, in);
+    int ir, in, split;
+    tile_of(blockIdx.x, tr, tn, p.splits, ir, in, split);
     const int r0 = ir * BR, n0 = in * BN;
-    const int g0 = (int)((long)p.groups * blockIdx.y / p.splits), g1 = (int)((long)p.groups * (blockIdx.y + 1) / p.splits);
+    const int g0 = (int)((long)p.groups * split / p.splits), g1 = (int)((long)p.groups * (split + 1) / p.splits);
 
     // where this lane's copies of a group begin (rows and outputs beyond the last: the last again)
     unsigned w_off[W_COPIES], a_off[A_COPIES], s_off[S_COPIES];
@@ -221,7 +221,7 @@ __global__ __launch_bounds__(64 * WN * WR) void mx_tile_kernel(MxProduct p) {
     for (int j = 0; j < FR; ++j) {
         const int row0 = r0 + (wr * FR + j) * 32;
         auto pick = [&](int i) -> const f32x16& { return acc[i][j]; };
-        if (p.slabs) store_rows<float, FN>(pick, stage, row0, col0, p.rows, n4, p.slabs + (long)blockIdx.y * p.rows * n4, n4, nullptr, 0, true);
+        if (p.slabs) store_rows<float, FN>(pick, stage, row0, col0, p.rows, n4, p.slabs + (long)split * p.rows * n4, n4, nullptr, 0, true);
         else store_rows<T, FN>(pick, stage, row0, col0, p.rows, p.n, static_cast<T*>(p.y), p.n, p.bias, 0, p.vec16);
     }
 }
@@ -387,7 +387,7 @@ static int launch_tile(const MxProduct& p, hipStream_t st) {
     const hipError_t set = allow_lds(reinterpret_cast<const void*>(kernel), LDS, devices);
     if (set != hipSuccess) return fail("gan_mx_matmul: %d bytes of LDS refused: %s", LDS, hipGetErrorString(set));
     const long tiles = (long)((p.rows + BR - 1) / BR) * ((p.n + BN - 1) / BN);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, p.splits), dim3(64 * WN * WR), LDS, st, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles * p.splits), dim3(64 * WN * WR), LDS, st, p);
     return 0;
 }
 
