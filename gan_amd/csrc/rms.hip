@@ -9,22 +9,31 @@
 // 1/8, and with y rounded once from 64 bits a value next to a border falls on its own side (fp64 runs at the fp32 rate here, and
 // the kernel waits for memory: no cost was measurable).
 //
-// Memory-bound.  A team of 64 to 1024 threads keeps a whole row in registers, eight values a chunk, so every tensor is
-// read and written once.
+// Memory-bound.  A team of 8 to 1024 threads keeps a whole row in registers, eight values a chunk, so every tensor is read and
+// written once.
 #include "mx.h"
 
 namespace gan {
 
-template <typename S>
-__device__ __forceinline__ S team_sum(S v, int tpr, S* red) {
-    v = wave_all_sum(v);
-    if (tpr > 64) {
-        const int wave = threadIdx.x >> 6, waves = tpr >> 6;
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) red[wave] = v;
-        __syncthreads();
-        v = 0;
-        for (int i = 0; i < waves; ++i) v += red[i];
+// Sum over the TPR threads of a team, in all of them: lanes of a wave, or whole waves by way of `red`.
+template <int TPR, typename S>
+__device__ __forceinline__ S team_sum(S v, S* red) {
+    if constexpr (TPR < 64) {
+        v += row_swizzle<0xb1>(v);
+        v += row_swizzle<0x4e>(v);
+        v += row_swizzle<0x141>(v);
+        if constexpr (TPR >= 16) v += row_swizzle<0x140>(v);
+        if constexpr (TPR == 32) v += __shfl_xor(v, 16, 64);
+    } else {
+        v = wave_all_sum(v);
+        if constexpr (TPR > 64) {
+            __syncthreads();
+            if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+            __syncthreads();
+            v = 0;
+#pragma unroll
+            for (int i = 0; i < TPR / 64; ++i) v += red[i];
+        }
     }
     return v;
 }
@@ -47,7 +56,7 @@ struct RmsFwd {
 template <typename T, int TPR, int NV, bool MX>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(RmsFwd p) {
     constexpr int TEAMS = TPR < 256 ? 256 / TPR : 1;
-    __shared__ double red[TPR / 64];
+    __shared__ double red[TPR / 64 + 1];
     const int t = threadIdx.x % TPR, team = threadIdx.x / TPR;
     const int c = p.c, chunks = MX ? mx_groups(c) * 16 : (c + 7) / 8;
     const long row = ((long)blockIdx.y * gridDim.x + blockIdx.x) * TEAMS + team;
@@ -74,7 +83,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(RmsFwd p
 #pragma unroll
         for (int j = 0; j < 8; ++j) s = fma((double)v[i][j], (double)v[i][j], s);
     }
-    const double inv = 1.0 / sqrt(team_sum(s, TPR, red) / c + (double)p.eps);
+    const double inv = 1.0 / sqrt(team_sum<TPR>(s, red) / c + (double)p.eps);
     const float rstd = (float)inv;
     if (!live) return;
     if (p.rstd && t == 0) p.rstd[row] = rstd;
@@ -105,87 +114,155 @@ struct RmsBwd {
     const void* dy;
     const void* dh;
     void* dx;
-    float* partial;     // [teams of the grid][c], or null
+    float* partial;     // [workgroups][c], or null
     long rows, ldh;
     int c;
     bool vec_h, vec_o, vec_g;
 };
 
-// Every team walks the rows from its own number on in steps of the number of teams and adds dy n up in registers (the
-// columns of a thread are the same in every row); rms_dgamma_kernel joins the teams in a fixed order.
+constexpr int kRmsTwice = 4;        // chunks a thread from which a row is read twice
+
+// Every team walks the rows from its own number on in steps of the number of teams and adds dy n up in registers (the columns of a
+// thread are the same in every row).  The teams of a workgroup join their sums in LDS, rms_dgamma_kernel those of the workgroups,
+// both in a fixed order.
 template <typename T, int TPR, int NV>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(RmsBwd p) {
     constexpr int TEAMS = TPR < 256 ? 256 / TPR : 1;
-    __shared__ float red[TPR / 64];
+    __shared__ float red[TPR / 64 + 1];
     const int t = threadIdx.x % TPR, c = p.c;
     const long team = (long)blockIdx.x * TEAMS + threadIdx.x / TPR, teams = (long)gridDim.x * TEAMS;
-    constexpr bool kHold = TPR < 1024;      // gamma stays in registers, and dh comes with the row (1024 threads have 128 registers each)
-    float acc[NV][8], w[NV][8];
+    // 1024 threads have 128 registers each: with one chunk gamma stays in them and dh comes with the row, with two gamma and dh are
+    // read when they are wanted, with four the sums are in LDS and the row is read again for its gradient (32M bf16 values in rows of
+    // 32768: 208 us held and spilled, 86 so)
+    constexpr bool kHold = TPR < 1024 || NV == 1, kTwice = NV == kRmsTwice;
+    extern __shared__ __align__(16) float sums[];      // [NV * 8][TPR], kTwice only
+    float acc[kTwice ? 1 : NV][8], w[kTwice ? 1 : NV][8];
+    if constexpr (kTwice) {
+        for (int i = 0; i < NV * 8; ++i) sums[i * TPR + t] = 0.f;
+    } else {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int i0 = (i * TPR + t) * 8;
-        if (kHold) load8(p.gamma, i0, i0 < c ? c : 0, p.vec_g, w[i]);
+        for (int i = 0; i < NV; ++i) {
+            const int i0 = (i * TPR + t) * 8;
+            if constexpr (kHold) load8(p.gamma, i0, i0 < c ? c : 0, p.vec_g, w[i]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[i][j] = 0.f;
+            for (int j = 0; j < 8; ++j) acc[i][j] = 0.f;
+        }
     }
     for (long row = team; row < p.rows; row += teams) {
         const T* hr = static_cast<const T*>(p.h) + row * p.ldh;
         const T* yr = static_cast<const T*>(p.dy) + row * c;
         const T* dhr = p.dh && p.dx ? static_cast<const T*>(p.dh) + row * c : nullptr;
         const float rstd = p.rstd[row];
-        float n[NV][8], g[NV][8], d[NV][8], s = 0.f;
+        if constexpr (kTwice) {
+            float s = 0.f;
+#pragma unroll 2
+            for (int i = 0; i < NV; ++i) {
+                const int i0 = (i * TPR + t) * 8, cc = i0 < c ? c : 0;
+                float n[8], g[8];
+                load8(hr, i0, cc, p.vec_h, n);
+                load8(yr, i0, cc, p.vec_o, g);
+                load8(p.gamma, i0, cc, p.vec_g, w[0]);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int i0 = (i * TPR + t) * 8, cc = i0 < c ? c : 0;
-            load8(hr, i0, cc, p.vec_h, n[i]);
-            load8(yr, i0, cc, p.vec_o, g[i]);
-            if (kHold && dhr) load8(dhr, i0, cc, p.vec_o, d[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            if (!kHold) load8(p.gamma, (i * TPR + t) * 8, (i * TPR + t) * 8 < c ? c : 0, p.vec_g, w[0]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                n[i][j] *= rstd;
-                acc[i][j] = fmaf(g[i][j], n[i][j], acc[i][j]);
-                g[i][j] *= w[kHold ? i : 0][j];
-                s = fmaf(g[i][j], n[i][j], s);
+                for (int j = 0; j < 8; ++j) {
+                    n[j] *= rstd;
+                    sums[(i * 8 + j) * TPR + t] = fmaf(g[j], n[j], sums[(i * 8 + j) * TPR + t]);
+                    s = fmaf(g[j] * w[0][j], n[j], s);
+                }
             }
-        }
-        if (!p.dx) continue;
-        const float m = team_sum(s, TPR, red) / c;
+            if (!p.dx) continue;
+            const float m = team_sum<TPR>(s, red) / c;
+#pragma unroll 2
+            for (int i = 0; i < NV; ++i) {
+                const int i0 = (i * TPR + t) * 8;
+                if (i0 >= c) continue;
+                float n[8], g[8], d[8], o[8];
+                load8(hr, i0, c, p.vec_h, n);
+                load8(yr, i0, c, p.vec_o, g);
+                load8(p.gamma, i0, c, p.vec_g, w[0]);
+                if (dhr) load8(dhr, i0, c, p.vec_o, d);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int i0 = (i * TPR + t) * 8;
-            if (i0 >= c) continue;
-            float o[8];
-            if (!kHold && dhr) load8(dhr, i0, c, p.vec_o, d[i]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                o[j] = rstd * (g[i][j] - n[i][j] * m);
-                if (dhr) o[j] += d[i][j];
+                for (int j = 0; j < 8; ++j) {
+                    o[j] = rstd * (g[j] * w[0][j] - n[j] * rstd * m);
+                    if (dhr) o[j] += d[j];
+                }
+                store8(static_cast<T*>(p.dx) + row * c, i0, c, p.vec_o, o);
             }
-            store8(static_cast<T*>(p.dx) + row * c, i0, c, p.vec_o, o);
+            continue;
+        } else {
+            float n[NV][8], g[NV][8], d[NV][8], s = 0.f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int i0 = (i * TPR + t) * 8, cc = i0 < c ? c : 0;
+                load8(hr, i0, cc, p.vec_h, n[i]);
+                load8(yr, i0, cc, p.vec_o, g[i]);
+                if (kHold && dhr) load8(dhr, i0, cc, p.vec_o, d[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                if (!kHold) load8(p.gamma, (i * TPR + t) * 8, (i * TPR + t) * 8 < c ? c : 0, p.vec_g, w[0]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    n[i][j] *= rstd;
+                    acc[i][j] = fmaf(g[i][j], n[i][j], acc[i][j]);
+                    g[i][j] *= w[kHold ? i : 0][j];
+                    s = fmaf(g[i][j], n[i][j], s);
+                }
+            }
+            if (!p.dx) continue;
+            const float m = team_sum<TPR>(s, red) / c;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int i0 = (i * TPR + t) * 8;
+                if (i0 >= c) continue;
+                float o[8];
+                if (!kHold && dhr) load8(dhr, i0, c, p.vec_o, d[i]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    o[j] = rstd * (g[i][j] - n[i][j] * m);
+                    if (dhr) o[j] += d[i][j];
+                }
+                store8(static_cast<T*>(p.dx) + row * c, i0, c, p.vec_o, o);
+            }
         }
     }
-    if (p.partial) {
+    if (!p.partial) return;
+    float* out = p.partial + (long)blockIdx.x * c;
+    if constexpr (TEAMS == 1) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int i0 = (i * TPR + t) * 8;
-            if (i0 < c) store8(p.partial + team * c, i0, c, (c & 3) == 0, acc[i]);
+            if constexpr (kTwice) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) acc[0][j] = sums[(i * 8 + j) * TPR + t];
+            }
+            if (i0 < c) store8(out, i0, c, (c & 3) == 0, acc[kTwice ? 0 : i]);
+        }
+    } else {
+        constexpr int W = TPR * NV * 8;
+        __shared__ __align__(16) float join[TEAMS * W];
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            *reinterpret_cast<f32x8*>(join + threadIdx.x / TPR * W + (i * TPR + t) * 8) =
+                f32x8{acc[i][0], acc[i][1], acc[i][2], acc[i][3], acc[i][4], acc[i][5], acc[i][6], acc[i][7]};
+        __syncthreads();
+        for (int col = threadIdx.x; col < c; col += 256) {
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < TEAMS; ++i) s += join[i * W + col];
+            out[col] = s;
         }
     }
 }
 
-// dgamma[col] (+)= sum over teams of partial[team][col]: 32 columns a block, 32 teams side by side, joined in LDS.
-__global__ __launch_bounds__(1024) void rms_dgamma_kernel(const float* __restrict__ partial, float* __restrict__ out, int teams,
+// dgamma[col] (+)= sum over workgroups of partial[workgroup][col]: 32 columns a block, 32 rows side by side, joined in LDS.
+__global__ __launch_bounds__(1024) void rms_dgamma_kernel(const float* __restrict__ partial, float* __restrict__ out, int rows,
                                                           int c, int accumulate) {
     __shared__ float red[32][33];
     const int col = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
     float s = 0.f;
     if (col < c) {
 #pragma unroll 8
-        for (int i = part; i < teams; i += 32) s += partial[(long)i * c + col];
+        for (int i = part; i < rows; i += 32) s += partial[(long)i * c + col];
     }
     red[part][threadIdx.x & 31] = s;
     __syncthreads();
@@ -196,25 +273,38 @@ __global__ __launch_bounds__(1024) void rms_dgamma_kernel(const float* __restric
     }
 }
 
-// Calls f(threads a row, chunks a thread) with a shape that holds `chunks` chunks of eight.  Few chunks a thread: a row then
-// takes few registers, and many rows are in flight on a CU.
-template <typename F>
+// Calls f(threads a row, chunks a thread) with a shape that holds `chunks` chunks of eight.  One chunk a thread keeps rows in few
+// registers and many of them in flight: backward of 32M bf16 values (floor 45 us) with rows of 2048 52 us (two chunks 79), of 4096 54
+// (72 to 80), of 8192 54 (75 to 88); a wave for a row of 1024 is better than four, 56 against 81.  In the forward pass two chunks
+// in front of the 8-bit output cost less than the wider team's exchange: rows of 4096 42 us against 45, without it 46 against 43.
+template <bool MX, typename F>
 static void with_shape(int chunks, F f) {
-    if (chunks <= 64) f(std::integral_constant<int, 64>(), std::integral_constant<int, 1>());
-    else if (chunks <= 128) f(std::integral_constant<int, 64>(), std::integral_constant<int, 2>());
-    else if (chunks <= 256) f(std::integral_constant<int, 256>(), std::integral_constant<int, 1>());
-    else if (chunks <= 512) f(std::integral_constant<int, 256>(), std::integral_constant<int, 2>());
-    else if (chunks <= 1024) f(std::integral_constant<int, 512>(), std::integral_constant<int, 2>());
-    else if (chunks <= 2048) f(std::integral_constant<int, 1024>(), std::integral_constant<int, 2>());
-    else f(std::integral_constant<int, 1024>(), std::integral_constant<int, 4>());
+#define GAN_SHAPE(tpr, nv) return f(std::integral_constant<int, tpr>(), std::integral_constant<int, nv>())
+    if constexpr (!MX) {        // (8-bit rows are filled up to 16 chunks)
+        if (chunks <= 8) GAN_SHAPE(8, 1);
+    }
+    if (chunks <= 16) GAN_SHAPE(16, 1);
+    if (chunks <= 32) GAN_SHAPE(32, 1);
+    if (chunks <= 64) GAN_SHAPE(64, 1);
+    if (chunks <= 128) GAN_SHAPE(64, 2);
+    if (chunks <= 256) GAN_SHAPE(256, 1);
+    if constexpr (MX) {
+        if (chunks <= 512) GAN_SHAPE(256, 2);
+        if (chunks <= 1024) GAN_SHAPE(512, 2);
+    } else {
+        if (chunks <= 512) GAN_SHAPE(512, 1);
+        if (chunks <= 1024) GAN_SHAPE(1024, 1);
+    }
+    if (chunks <= 2048) GAN_SHAPE(1024, 2);
+    GAN_SHAPE(1024, 4);
+#undef GAN_SHAPE
 }
 
-// Teams of the backward grid: enough to fill the chip, and few, since each leaves a row of partial sums.
-static int rms_bwd_teams(long rows, int c) {
-    const int per = c <= 1024 ? 4 : 1;      // (teams a workgroup, as with_shape gives them)
-    long teams = c <= 1024 ? 4096 : c <= 4096 ? 1024 : 512;
-    if (teams > (rows + 3) / 4) teams = (rows + 3) / 4;
-    return (int)((teams + per - 1) / per * per);
+// Workgroups of the backward grid: enough to fill the chip, and few, since each leaves a row of partial sums.
+static int rms_bwd_groups(long rows, int c) {
+    const int chunks = (c + 7) / 8, teams = chunks <= 8 ? 32 : chunks <= 16 ? 16 : chunks <= 32 ? 8 : chunks <= 128 ? 4 : 1;    // (a workgroup's)
+    const long groups = c <= 2048 ? 1024 : c <= 4096 ? 512 : 256, most = (rows + 4 * teams - 1) / (4 * teams);
+    return (int)(groups < most ? groups : most);
 }
 
 constexpr int kRmsMaxWidth = 32768;
@@ -243,21 +333,22 @@ int gan_rms_norm_fwd(int dtype, long rows, int c, const void* x, long ldx, const
                  rows, ldx, ldr, c, eps,
                  aligned16(x) && ldx * sizeof(T) % 16 == 0, aligned16(residual) && ldr * sizeof(T) % 16 == 0,
                  c * sizeof(T) % 16 == 0 && aligned16(h) && aligned16(y), aligned16(gamma)};
-        with_shape(mx ? mx_groups(c) * 16 : (c + 7) / 8, [&](auto tpr, auto nv) {
+        auto go = [&](auto tpr, auto nv, auto to_mx) {
             constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, TEAMS = TPR < 256 ? 256 / TPR : 1;
             // (fewer than 2^32 threads along x)
             const long blocks = (rows + TEAMS - 1) / TEAMS, along = blocks < (1L << 21) ? blocks : 1L << 21;
             const dim3 grid((unsigned)along, (unsigned)((blocks + along - 1) / along)), block(TPR < 256 ? 256 : TPR);
-            if (mx) hipLaunchKernelGGL((rms_fwd_kernel<T, TPR, NV, true>), grid, block, 0, as_stream(stream), p);
-            else hipLaunchKernelGGL((rms_fwd_kernel<T, TPR, NV, false>), grid, block, 0, as_stream(stream), p);
-        });
+            hipLaunchKernelGGL((rms_fwd_kernel<T, TPR, NV, decltype(to_mx)::value>), grid, block, 0, as_stream(stream), p);
+        };
+        if (mx) with_shape<true>(mx_groups(c) * 16, [&](auto tpr, auto nv) { go(tpr, nv, std::true_type()); });
+        else with_shape<false>((c + 7) / 8, [&](auto tpr, auto nv) { go(tpr, nv, std::false_type()); });
         return check_launch("gan_rms_norm_fwd");
     });
 }
 
 size_t gan_rms_norm_workspace_bytes(long rows, int c) {
     if (rows <= 0 || c < 1) return 0;
-    return (size_t)rms_bwd_teams(rows, c) * c * sizeof(float);
+    return (size_t)rms_bwd_groups(rows, c) * c * sizeof(float);
 }
 
 int gan_rms_norm_bwd(int dtype, long rows, int c, const void* h, long ldh, const float* gamma, const float* rstd, const void* dy,
@@ -270,7 +361,7 @@ int gan_rms_norm_bwd(int dtype, long rows, int c, const void* h, long ldh, const
     const size_t need = dgamma ? gan_rms_norm_workspace_bytes(rows, c) : 0;
     GAN_CHECK_ARG(ws_bytes >= need && (need == 0 || (ws && aligned16(ws))),
                   "gan_rms_norm_bwd: workspace of %zu bytes needed (16-byte aligned), %zu given", need, ws_bytes);
-    const int teams = rows ? rms_bwd_teams(rows, c) : 0;
+    const int groups = rows ? rms_bwd_groups(rows, c) : 0;
     float* partial = dgamma ? static_cast<float*>(ws) : nullptr;
     if (rows) {
         const int rc = with_dtype(dtype, [&](auto* tag) {
@@ -278,17 +369,24 @@ int gan_rms_norm_bwd(int dtype, long rows, int c, const void* h, long ldh, const
             RmsBwd p{h, gamma, rstd, dy, dh, dx, partial, rows, ldh, c,
                      aligned16(h) && ldh * sizeof(T) % 16 == 0,
                      c * sizeof(T) % 16 == 0 && aligned16(dy) && aligned16(dh) && aligned16(dx), aligned16(gamma)};
-            with_shape((c + 7) / 8, [&](auto tpr, auto nv) {
-                constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, TEAMS = TPR < 256 ? 256 / TPR : 1;
-                hipLaunchKernelGGL((rms_bwd_kernel<T, TPR, NV>), dim3(teams / TEAMS), dim3(TPR < 256 ? 256 : TPR), 0,
+            hipError_t set = hipSuccess;
+            with_shape<false>((c + 7) / 8, [&](auto tpr, auto nv) {
+                constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, LDS = NV == kRmsTwice ? NV * 8 * TPR * 4 : 0;
+                if constexpr (LDS > 0) {
+                    static std::atomic<unsigned long> devices{0};
+                    set = allow_lds(reinterpret_cast<const void*>(rms_bwd_kernel<T, TPR, NV>), LDS, devices);
+                    if (set != hipSuccess) return;
+                }
+                hipLaunchKernelGGL((rms_bwd_kernel<T, TPR, NV>), dim3(groups), dim3(TPR < 256 ? 256 : TPR), LDS,
                                    as_stream(stream), p);
             });
+            if (set != hipSuccess) return fail("gan_rms_norm_bwd: LDS refused: %s", hipGetErrorString(set));
             return check_launch("gan_rms_norm_bwd");
         });
         if (rc) return rc;
     }
     if (dgamma) {
-        hipLaunchKernelGGL(rms_dgamma_kernel, dim3((c + 31) / 32), dim3(1024), 0, as_stream(stream), partial, dgamma, teams, c,
+        hipLaunchKernelGGL(rms_dgamma_kernel, dim3((c + 31) / 32), dim3(1024), 0, as_stream(stream), partial, dgamma, groups, c,
                            accumulate);
         return check_launch("gan_rms_norm_bwd");
     }

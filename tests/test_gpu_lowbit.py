@@ -746,3 +746,10 @@ def test_gradients_apart_are_those_computed_together(rows, k, n, dtype):
         alone = [l.grad(v).clone() for v in ('Linear/Matrix', 'Linear/bias')]
     frozen, = torch.autograd.grad((ops.mx_matmul(xx, ops.mx_pack(m)),), (xx,), (dy,))
     assert torch.equal(dx, frozen) and torch.equal(both[0], alone[0]) and torch.equal(both[1], alone[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("rows,c", [(9000, 5), (5000, 64), (3001, 128), (2500, 200), (1100, 4096), (1030, 8192), (600, 20000)])
+def test_norm_gradients_of_many_rows_a_team(rows, c, dtype):
+    """Every width of team with several rows for each, and partial sums of several workgroups."""
+    test_norm_gradients(rows, c, dtype, True)
