@@ -381,10 +381,16 @@ __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
     }
 }
 
-// out[0] = sum of x: one workgroup, fixed order.
+// Sum of x: one workgroup, fixed order, eight loads of a thread in flight.
 __device__ float sum_by_block(const float* __restrict__ x, long n, float* red) {
     float s = 0.f;
-    for (long i = threadIdx.x; i < n; i += 1024) s += x[i];
+    for (long i = threadIdx.x; i < n; i += 8 * 1024) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = i + k * 1024 < n ? x[i + k * 1024] : 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s += v[k];
+    }
     return block_sum<1024>(s, red);
 }
 __global__ __launch_bounds__(1024) void distill_weights_kernel(const float* __restrict__ weight, long rows, float* out) {
@@ -393,10 +399,11 @@ __global__ __launch_bounds__(1024) void distill_weights_kernel(const float* __re
     if (threadIdx.x == 0) out[0] = s;
 }
 __global__ __launch_bounds__(1024) void distill_mean_kernel(const float* __restrict__ row_loss, const float* __restrict__ weight,
-                                                            long rows, float scale, int accumulate, float* __restrict__ out) {
+                                                            const float* __restrict__ weights, long rows, float scale,
+                                                            int accumulate, float* __restrict__ out) {
     __shared__ float red[16];
     const float s = sum_by_block(row_loss, rows, red);
-    const float total = weight ? sum_by_block(weight, rows, red) : (float)rows;
+    const float total = weights ? weights[0] : weight ? sum_by_block(weight, rows, red) : (float)rows;
     if (threadIdx.x == 0) out[0] = (accumulate ? out[0] : 0.f) + (total != 0.f ? scale * (s / total) : 0.f);
 }
 
@@ -455,6 +462,12 @@ int gan_distill_topk_mean(int dtype, long rows, int classes, const void* logits,
         // What is in flight on a CU counts, not only that nothing is read twice: of 131072 bf16 classes (16384 chunks) 2048 rows
         // take 249 us with half of a row in registers and 262 with all of it, of 32000 (4000 chunks) 4096 rows 124 us with 512
         // threads, 143 with 1024, 134 with 256 x 16 chunks.  Few rows want every thread: 256 rows of 131072 41 us against 46.
+        // Many short rows go to a wave each: 65536 x 100 fp32 227 us with 256 threads, 110 so, 16384 x 1000 60 against 42, 8192 x 4000
+        // bf16 61 against 50 (of 8000 77 against 95); 64 rows of 100 10.0 against 11.4 us.
+        if (rows >= 2048 && chunks <= 512) {
+            if (chunks <= 64) return launch_distill<T, 64, 1>(p, st);
+            return chunks <= 256 ? launch_distill<T, 64, 4>(p, st) : launch_distill<T, 64, 8>(p, st);
+        }
         if (chunks <= 256) return launch_distill<T, 256, 1>(p, st);
         if (chunks <= 512) return launch_distill<T, 256, 2>(p, st);
         if (chunks <= 1024) return launch_distill<T, 256, 4>(p, st);
@@ -464,7 +477,7 @@ int gan_distill_topk_mean(int dtype, long rows, int classes, const void* logits,
         return launch_distill<T, 1024, 16>(p, st);
     });
     if (rc) return rc;
-    hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(1024), 0, st, row_loss, row_weight, rows, weight * temperature * temperature,
+    hipLaunchKernelGGL(distill_mean_kernel, dim3(1), dim3(1024), 0, st, row_loss, row_weight, total, rows, weight * temperature * temperature,
                        accumulate, loss_out);
     return check_launch("gan_distill_topk_mean");
 }

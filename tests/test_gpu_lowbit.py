@@ -753,3 +753,31 @@ def test_gradients_apart_are_those_computed_together(rows, k, n, dtype):
 def test_norm_gradients_of_many_rows_a_team(rows, c, dtype):
     """Every width of team with several rows for each, and partial sums of several workgroups."""
     test_norm_gradients(rows, c, dtype, True)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("classes,top", [(5, 2), (130, 9), (1027, 70), (2000, 16)])
+def test_distillation_of_many_short_rows(classes, top, dtype):
+    """More rows than one sum of weights takes, against the loss of a few of them at a time: the mean is linear in the rows."""
+    from gan_amd import ops
+    g = gen(classes)
+    rows = 4200
+    logits = (2 * normal(g, rows, classes)).to(dtype)
+    index = torch.randint(0, classes, (rows, top), generator=g, device='cuda')
+    teacher, w = 2 * normal(g, rows, top), torch.rand(rows, generator=g, device='cuda')
+    w[5] = 0
+    lse = torch.logsumexp(teacher, 1) + 0.2
+    x = logits.requires_grad_(True)
+    loss = ops.distill_topk_mean(x, teacher, index, row_weight=w, teacher_lse=lse)
+    ops.backward(loss)
+    total = w.double().sum().cpu()
+    pick = [0, 5, 2047, 4199]
+    want, grad, size = R.distill(logits.detach()[pick].cpu(), teacher[pick].cpu(), index[pick].cpu(), row_weight=w[pick].cpu(), lse=lse[pick].cpu())
+    share = (w[pick].double().sum().cpu() / total).item()
+    # (the sum of 4200 weights: 64 E more)
+    within(x.grad[pick].cpu(), grad * share, half_step(dtype) * share * grad.abs() + (2.0 ** -17 + 64 * E) * share * size + tiny(dtype), "dlogits")
+    parts = [ops.distill_topk_mean(logits.detach()[a:a + 1000], teacher[a:a + 1000], index[a:a + 1000], row_weight=w[a:a + 1000],
+                                   teacher_lse=lse[a:a + 1000]) for a in range(0, rows, 1000)]
+    mean = sum(float(p) * float(w[a:a + 1000].double().sum() / w.double().sum()) for p, a in zip(parts, range(0, rows, 1000)))
+    # (both sides have the 2^-17 of a term of size <= 60)
+    assert abs(float(loss.detach()) - mean) <= 2 * 2.0 ** -17 * 60
