@@ -10,7 +10,9 @@
 // the kernel waits for memory: no cost was measurable).
 //
 // Memory-bound.  A team of 8 to 1024 threads keeps a whole row in registers, eight values a chunk, so every tensor is read and
-// written once.
+// written once.  bf16 with a residual: 8192 x 4096 to 8 bits 45 us = 5.2 TB/s; 16384 x 2048 forward 46 us = 5.8 TB/s, backward 51 + 4
+// us = 4.9 TB/s (a large copy reaches 4.8 TB/s on this card, an addition in place 5.9); one row of 4096 3.2 us, which is the launch and
+// two trips to memory.
 #include "mx.h"
 
 namespace gan {
