@@ -201,7 +201,8 @@ def scratch(nbytes, device):
     return t.data_ptr(), int(nbytes), t
 
 
-# The two queries every call makes, without the Python layers of torch.cuda (2.5 us a call) where this torch has them.
+# The queries every call makes, without the Python layers of torch.cuda (2.5 us a call) where this torch has them.
+_raw_capturing = getattr(torch._C, '_cuda_isCurrentStreamCapturing', None) or torch.cuda.is_current_stream_capturing
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
 _raw_device = getattr(torch._C, '_cuda_getDevice', None)
 
@@ -210,6 +211,11 @@ def _current_device():
     if _raw_device is not None and torch.cuda.is_initialized():
         return _raw_device()
     return torch.cuda.current_device()
+
+
+def capturing():
+    """Whether the current stream is being captured into a graph."""
+    return torch.cuda.is_initialized() and _raw_capturing()
 
 
 def stream():

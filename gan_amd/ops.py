@@ -56,8 +56,7 @@ class taping(object):
 def _token_key(device, early):
     """A pass under capture has leaves of its own: autograd joins the stream a leaf was first used on, which would drag the
     stream of an eager pass that is still alive into the capture and end it."""
-    capturing = torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
-    return device, early, stream() if capturing else None
+    return device, early, stream() if _lib.capturing() else None
 
 
 def _grad_token(device, var=None):
@@ -873,8 +872,10 @@ def _rms_fwd(x, residual, gamma, eps, mx, want_rstd):
 
 
 class _RmsNormFn(torch.autograd.Function):
+    # (what autograd need not look at goes in one argument: each costs it time)
     @staticmethod
-    def forward(ctx, x, residual, token, gamma, eps, mx, made):
+    def forward(ctx, x, residual, token, rest):
+        gamma, eps, mx, made = rest
         ctx.set_materialize_grads(False)
         out, h, rstd, (kept, ctx.ld) = _rms_fwd(x, residual, gamma, eps, mx, True)
         ctx.save_for_backward(kept, rstd)
@@ -906,7 +907,7 @@ class _RmsNormFn(torch.autograd.Function):
                 check(lib.gan_rms_norm_bwd(_lib.dtype_code(dy.dtype), rows, c, kept.data_ptr(), ctx.ld, ptr(gamma.data), ptr(rstd),
                                            dy.data_ptr(), None if dh is None else dh.data_ptr(),
                                            None if dx is None else dx.data_ptr(), ptr(dg), acc, wp, wn, stream()))
-        return (dx if ctx.needs_input_grad[0] else None, dx if ctx.needs_input_grad[1] else None) + (None,) * 5
+        return (dx if ctx.needs_input_grad[0] else None, dx if ctx.needs_input_grad[1] else None, None, None)
 
 
 def rms_norm(x, name="rms_norm", epsilon=1e-6, residual=None, mx=False):
@@ -931,7 +932,7 @@ def rms_norm(x, name="rms_norm", epsilon=1e-6, residual=None, mx=False):
         out, h, _, _ = _rms_fwd(x, residual, gamma, eps, mx, False)
         return out if h is None else (out, h)
     made = []
-    out = _RmsNormFn.apply(x, residual, token, gamma, eps, mx, made)
+    out = _RmsNormFn.apply(x, residual, token, (gamma, eps, mx, made))
     y, h = out if residual is not None else (out, None)
     if mx:
         made[0].ticket = y
@@ -1093,7 +1094,8 @@ class _MxMatmulFn(torch.autograd.Function):
     the packed weights (None: frozen)."""
 
     @staticmethod
-    def forward(ctx, x, token, q, w, bias, matrix, bias_var, fmt):
+    def forward(ctx, x, token, rest):
+        q, w, bias, matrix, bias_var, fmt = rest
         q = mx_quantize(x, fmt) if q is None else q
         y = _mx_product(q, w, bias)
         ctx.save_for_backward(q.codes, q.scales, w.codes, w.scales)
@@ -1127,7 +1129,7 @@ class _MxMatmulFn(torch.autograd.Function):
         elif dx is not None:
             wp, wn, hold = _lib.scratch(_size(lib.gan_mx_matmul_dgrad_workspace_bytes, code, *sizes), dy.device)
             check(lib.gan_mx_matmul_dgrad(code, *sizes, dy.data_ptr(), wc.data_ptr(), wsc.data_ptr(), dx.data_ptr(), wp, wn, stream()))
-        return (dx,) + (None,) * 7
+        return dx, None, None
 
 
 def _mx_apply(x, w, bias, fmt, token=None, matrix=None, bias_var=None):
@@ -1143,7 +1145,7 @@ def _mx_apply(x, w, bias, fmt, token=None, matrix=None, bias_var=None):
     if bias is not None and (tuple(bias.shape) != (w.out_dim,) or bias.dtype != torch.float32):
         raise ValueError("microscaled product: bias %s %s for %d outputs" % (tuple(bias.shape), bias.dtype, w.out_dim))
     if torch.is_grad_enabled() and (token is not None or (carrier is not None and carrier.requires_grad)):
-        return _MxMatmulFn.apply(carrier, token, q, w, bias, matrix, bias_var, fmt)
+        return _MxMatmulFn.apply(carrier, token, (q, w, bias, matrix, bias_var, fmt))
     return _mx_linear(x, w, bias, fmt) if q is None else _mx_product(q, w, bias)
 
 
@@ -1442,7 +1444,8 @@ def l1_mean(a, b, weight=1.0):
 
 class _DistillFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, teacher, index, lse, row_weight, tau, weight):
+    def forward(ctx, logits, rest):
+        teacher, index, lse, row_weight, tau, weight = rest
         _lib.here(logits, teacher, index, lse, row_weight)
         x, rows, classes, ld = _rows_of(logits)
         dev = x.device
@@ -1460,7 +1463,7 @@ class _DistillFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, _one):
-        return (ctx.saved_tensors[0],) + (None,) * 6
+        return ctx.saved_tensors[0], None
 
 
 def distill_topk_mean(logits, teacher_logits, teacher_index, temperature=1.0, weight=1.0, row_weight=None, teacher_lse=None):
@@ -1488,8 +1491,8 @@ def distill_topk_mean(logits, teacher_logits, teacher_index, temperature=1.0, we
             raise ValueError("distill_topk_mean: %s %s %s for rows %s (float32 expected)" % (what, tuple(t.shape), t.dtype, lead))
     if not 2.0 ** -40 <= float(temperature) <= 2.0 ** 40:
         raise ValueError("distill_topk_mean: temperature %r" % (temperature,))
-    return _DistillFn.apply(logits, _plain(teacher_logits), _plain(teacher_index), _plain(teacher_lse), _plain(row_weight),
-                            float(temperature), float(weight))
+    return _DistillFn.apply(logits, (_plain(teacher_logits), _plain(teacher_index), _plain(teacher_lse), _plain(row_weight),
+                                     float(temperature), float(weight)))
 
 
 _ones = {}

@@ -170,12 +170,11 @@ def test_ranges_beyond_the_documented_ones_are_refused():
 
 
 def test_a_capture_has_leaves_of_its_own(monkeypatch):
-    from gan_amd import ops
+    from gan_amd import _lib, ops
     device = torch.device('cuda', 0)
     eager = ops._token_key(device, True)
     assert eager == ops._token_key(device, True) != ops._token_key(device, False)
-    monkeypatch.setattr(torch.cuda, 'is_initialized', lambda: True)
-    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+    monkeypatch.setattr(_lib, 'capturing', lambda: True)
     monkeypatch.setattr(ops, 'stream', lambda: 7)
     first = ops._token_key(device, True)
     monkeypatch.setattr(ops, 'stream', lambda: 8)
