@@ -228,10 +228,12 @@ __global__ __launch_bounds__(64 * WN * WR) void mx_tile_kernel(MxProduct p) {
 
 // ------------------------------------------------------------------------------------------------ few rows
 // The weights' bytes bind, and for one token the wait for them: 1 x 8192 x 8192 e4m3 8.7 us = 4.1 TB/s of weights, 1 x 4096 x 4096
-// 4.2 us (4.7 from floats), 16 x 8192 x 8192 e2m1 11.9 us, 64 x 8192 x 8192 e4m3 16 us.  A wave takes 16 outputs and every WAVES-th group of its
-// workgroup's range; its lanes load weight fragments (one block of 16 bytes each) straight from global memory, AHEAD groups at
-// once, turn codes into bf16 and multiply on the bf16 pipe, which also makes the sums fp32 for every result type.  RT tiles of 16
-// rows share each converted fragment.  The waves' sums meet in LDS.
+// 4.3 us (4.7 from floats), 16 x 8192 x 8192 e2m1 11.9 us, 64 x 8192 x 8192 e4m3 16 us, 64 x 2400 x 256 4.9 us.  A wave takes 16
+// outputs and every WAVES-th group of its workgroup's range; its lanes load weight fragments (one block of 16 bytes each) straight from
+// global memory, AHEAD groups at once, turn codes into bf16 and multiply on the bf16 pipe, which also makes the sums fp32 for every
+// result type.  (The scaled pipe takes e2m1 codes as they are, 3 to 8 % faster, but rounds its sums in another order than a workgroup
+// that quantises itself: the same product would then depend on which way its activations came.)  RT tiles of 16 rows share each
+// converted fragment.  The waves' sums meet in LDS.
 // FUSED: the activations are still floats.  The workgroup quantises its range of the contraction first, each value once, and
 // keeps the quantised values as bf16 in LDS: one launch instead of two.  Every workgroup repeats that work, so this is for few
 // values (kFusedValues).
@@ -274,11 +276,11 @@ __global__ __launch_bounds__(512) void mx_few_kernel(MxProduct p) {
     bf16_t* values = reinterpret_cast<bf16_t*>(lds);
     if constexpr (FUSED) {
         const T* x = static_cast<const T*>(p.x);
-        const int per = span / 8, total = p.rows * per;     // (a multiple of 4: the lanes of a block stay together)
+        const int per = span / 8, total = min(16, p.rows - r0) * per;      // (a multiple of 4: the lanes of a block stay together)
         for (int i = threadIdx.x; i < total; i += 512) {
             const int row = i / per, c = (i - row * per) * 8, i0 = g0 * 128 + c;
             float v[8];
-            load8(x + row * p.ldx, i0, i0 < p.in_dim ? p.in_dim : 0, p.vec_x, v);
+            load8(x + (r0 + row) * p.ldx, i0, i0 < p.in_dim ? p.in_dim : 0, p.vec_x, v);
             unsigned code[2];
             const float s = mx_scale(mx_quantize_lane8<FMT>(v, code));
             bf16x8 b;
@@ -297,7 +299,7 @@ __global__ __launch_bounds__(512) void mx_few_kernel(MxProduct p) {
 #pragma unroll
             for (int j = 0; j < RT; ++j) {
                 if constexpr (FUSED) {
-                    const bf16x8* at = reinterpret_cast<const bf16x8*>(values + r[j] * pitch + (gu - g0) * 128 + q * 32);
+                    const bf16x8* at = reinterpret_cast<const bf16x8*>(values + (r[j] - r0) * pitch + (gu - g0) * 128 + q * 32);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) a[j][k] = at[k];
                 } else {
@@ -393,21 +395,32 @@ static int launch_tile(const MxProduct& p, hipStream_t st) {
 }
 
 // A workgroup quantises up to this many floats itself: 4 rounds of its 512 threads by 8 values, about 1 us; as a launch of its own
-// the quantisation takes 3 us and the gap between the two.
-constexpr int kFusedValues = 16384;
+// the quantisation takes 3 us and the gap between the two.  In a grid of at most one workgroup a CU, each with a tile of 16 rows, it may
+// be more: 64 x 1024 x 1024 e4m3 4.8 us against 7.7, 64 x 2048 x 512 6.5 against 7.8, 64 x 2400 x 256 7.4 against 7.3 (e2m1 7.6 against
+// 6.0), where a caller outside a graph still has a launch less to make (15 us a call against 10).
+constexpr int kFusedValues = 16384, kFusedValuesAlone = 40960;
 
-static bool mx_fused(const MxPlan& plan, int rows, int in_dim) {
-    return plan.kind == MX_FEW && rows <= 16 &&
-           (long)rows * ((mx_groups(in_dim) + plan.splits - 1) / plan.splits) * 128 <= kFusedValues;
+// Workgroups of 16 rows x 16 outputs.  At most one a CU, they have the chip's waves to themselves and sharing fragments does not pay:
+// 64 x 1024 x 1024 e4m3 from codes 5.4 us against 8.0 with 32 rows each; 32 x 4096 x 4096, two a CU, 9.2 against 8.8.
+static long few_grid(int rows, int out_dim, int splits) { return (long)((out_dim + 15) / 16) * ((rows + 15) / 16) * splits; }
+
+static bool mx_fused(const MxPlan& plan, int rows, int in_dim, int out_dim) {
+    if (plan.kind != MX_FEW) return false;
+    const long values = (long)(rows < 16 ? rows : 16) * ((mx_groups(in_dim) + plan.splits - 1) / plan.splits) * 128;
+    return (rows <= 16 && values <= kFusedValues) || (few_grid(rows, out_dim, plan.splits) <= 256 && values <= kFusedValuesAlone);
 }
 
 template <typename T, int FMT>
 static int launch_few(const MxProduct& p, hipStream_t st) {
     if (p.x) {
-        const size_t lds = (size_t)p.rows * ((p.groups + p.splits - 1) / p.splits * 128 + 8) * 2;
-        hipLaunchKernelGGL((mx_few_kernel<T, FMT, 1, true>), dim3((p.n + 15) / 16, p.splits), dim3(512), lds, st, p);
-    } else if (p.rows <= 16) {
-        hipLaunchKernelGGL((mx_few_kernel<T, FMT, 1, false>), dim3((p.n + 15) / 16, p.splits), dim3(512), 0, st, p);
+        const size_t lds = (size_t)(p.rows < 16 ? p.rows : 16) * ((p.groups + p.splits - 1) / p.splits * 128 + 8) * 2;
+        auto kernel = mx_few_kernel<T, FMT, 1, true>;
+        static std::atomic<unsigned long> devices{0};
+        const hipError_t set = lds > 65536 - 8192 ? allow_lds(reinterpret_cast<const void*>(kernel), (kFusedValuesAlone + 16 * 8) * 2, devices) : hipSuccess;
+        if (set != hipSuccess) return fail("gan_mx_linear: %zu bytes of LDS refused: %s", lds, hipGetErrorString(set));
+        hipLaunchKernelGGL(kernel, dim3((p.n + 15) / 16, p.splits, (p.rows + 15) / 16), dim3(512), lds, st, p);
+    } else if (p.rows <= 16 || few_grid(p.rows, p.n, p.splits) <= 256) {
+        hipLaunchKernelGGL((mx_few_kernel<T, FMT, 1, false>), dim3((p.n + 15) / 16, p.splits, (p.rows + 15) / 16), dim3(512), 0, st, p);
     } else {
         hipLaunchKernelGGL((mx_few_kernel<T, FMT, 2, false>), dim3((p.n + 15) / 16, p.splits, (p.rows + 31) / 32), dim3(512), 0, st, p);
     }
@@ -488,7 +501,7 @@ size_t gan_mx_linear_workspace_bytes(int dtype, int fmt, int rows, int in_dim, i
     if (rows < 1 || rows > GAN_MX_MAX_ROWS || in_dim < 1 || in_dim > GAN_MX_MAX_IN || out_dim < 1 || out_dim > GAN_MX_MAX_IN || !dtype_ok(dtype) || !mx_fmt_ok(fmt))
         return 0;
     const size_t own = gan_mx_matmul_workspace_bytes(dtype, fmt, rows, in_dim, out_dim);
-    if (mx_fused(mx_plan(dtype, fmt, rows, in_dim, out_dim), rows, in_dim)) return own;
+    if (mx_fused(mx_plan(dtype, fmt, rows, in_dim, out_dim), rows, in_dim, out_dim)) return own;
     return own + mx_codes_bytes(fmt, rows, in_dim) + mx_scales_bytes(rows, in_dim);
 }
 
@@ -505,7 +518,7 @@ int gan_mx_linear(int dtype, int fmt, int rows, int in_dim, int out_dim, const v
     const size_t need = gan_mx_linear_workspace_bytes(dtype, fmt, rows, in_dim, out_dim);
     GAN_CHECK_ARG(ws_bytes >= need && (need == 0 || (ws && aligned16(ws))),
                   "gan_mx_linear: workspace of %zu bytes needed (16-byte aligned), %zu given", need, ws_bytes);
-    if (mx_fused(mx_plan(dtype, fmt, rows, in_dim, out_dim), rows, in_dim))
+    if (mx_fused(mx_plan(dtype, fmt, rows, in_dim, out_dim), rows, in_dim, out_dim))
         return mx_product(dtype, fmt, rows, in_dim, out_dim, x, ldx, nullptr, nullptr, w_codes, w_scales, bias, y, ws, as_stream(stream),
                           "gan_mx_linear");
     unsigned char* codes = static_cast<unsigned char*>(ws);

@@ -781,3 +781,18 @@ def test_distillation_of_many_short_rows(classes, top, dtype):
     mean = sum(float(p) * float(w[a:a + 1000].double().sum() / w.double().sum()) for p, a in zip(parts, range(0, rows, 1000)))
     # (both sides have the 2^-17 of a term of size <= 60)
     assert abs(float(loss.detach()) - mean) <= 2 * 2.0 ** -17 * 60
+
+
+@pytest.mark.parametrize("fmt", ['e4m3', 'e2m1'])
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("rows,k,n", [(64, 1024, 1024), (31, 2048, 512), (100, 1000, 500), (200, 600, 100), (16, 2048, 70), (20, 2400, 40), (250, 128, 256)])
+def test_product_of_rows_quantised_by_the_product(rows, k, n, dtype, fmt):
+    _product(rows, k, n, dtype, fmt, seed=6)
+
+
+def test_product_of_strided_rows_quantised_by_the_product():
+    from gan_amd import ops
+    g = gen(61)
+    wide, w = normal(g, 70, 900).bfloat16(), ops.mx_pack(normal(g, 333, 48))
+    for x in (wide[:, 5:338], wide[:, 8:341], wide[::2, :333], wide.t()[:70, :70].repeat(1, 5)[:, :333]):
+        assert torch.equal(ops.mx_matmul(x, w), ops.mx_matmul(ops.mx_quantize(x.contiguous()), w))

@@ -80,9 +80,9 @@ def test_library_refuses_before_any_launch():
     need = lib.gan_mx_matmul_workspace_bytes(0, 0, 1000, 64, 2000)
     assert need > 0
     _refused(lib.gan_mx_matmul(0, 0, 1000, 64, 2000, p, p, p, p, None, p, p, need - 1, None), b"workspace")
-    need = lib.gan_mx_linear_workspace_bytes(1, 0, 100, 64, 64)
+    need = lib.gan_mx_linear_workspace_bytes(1, 0, 100, 8192, 64)
     assert need > 0 and lib.gan_mx_linear_workspace_bytes(1, 0, 1, 64, 64) == 0      # (one token: nothing to keep between launches)
-    _refused(lib.gan_mx_linear(1, 0, 100, 64, 64, p, 64, p, p, None, p, p, need - 1, None), b"workspace")
+    _refused(lib.gan_mx_linear(1, 0, 100, 8192, 64, p, 8192, p, p, None, p, p, need - 1, None), b"workspace")
     _refused(lib.gan_mx_linear(1, 0, 1, 64, 64, p, 63, p, p, None, p, None, 0, None), b"stride")
     _refused(lib.gan_mx_linear(1, 0, 1, 64, 64, None, 64, p, p, None, p, None, 0, None), b"null")
     _refused(lib.gan_mx_matmul_dgrad(0, 4, 64, 64, p, p, p, p, None, 0, None), b"workspace")
