@@ -184,8 +184,8 @@ size_t bf16_product_workspace(int rows, int cols, int parts, int depth);
 template <bool PT, bool QT, typename T>
 int bf16_product(const Bf16Product& p, T* out, void* ws, hipStream_t st, const char* what);
 
-// [filled][groups * 128] bf16 of microscaled operands: rows (outputs) and then zeros.
-void mx_rows_to_bf16(int fmt, const void* codes, const void* scales, bf16_t* out, long rows, long filled, int in_dim, hipStream_t st);
-void mx_weights_to_bf16(const void* codes, const void* scales, bf16_t* out, int in_dim, int out_dim, int filled, hipStream_t st);
+// [rows][groups * 128] and [out][groups * 128] bf16 of microscaled operands.
+void mx_product_images(int fmt, const void* a_codes, const void* a_scales, bf16_t* a, int rows, const void* w_codes, const void* w_scales,
+                       bf16_t* w, int in_dim, int out_dim, hipStream_t st);
 
 }  // namespace gan

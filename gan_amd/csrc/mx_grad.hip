@@ -224,11 +224,10 @@ __host__ __device__ __forceinline__ long to64(long n) { return (n + 63) / 64 * 6
 // be null.  Memory-bound; a workgroup takes 64 rows x 256 columns, a thread 8 rows x 8 columns (1024 x 32768 fp32, 335 MB: 61 us =
 // 5.5 TB/s).
 template <typename T>
-__global__ __launch_bounds__(256) void split_kernel(const T* __restrict__ y, bf16_t* __restrict__ out, float* __restrict__ colsum,
-                                                    int rows, int n, bool vec) {
-    __shared__ float red[8][256];
+__device__ __forceinline__ void split_block(const T* __restrict__ y, bf16_t* __restrict__ out, float* __restrict__ colsum, int rows,
+                                            int n, bool vec, int accumulate, int bx, int by, float (*red)[256]) {
     const int rp = (int)to64(rows), np = (int)to64(n);
-    const int t = threadIdx.x % 32, group = threadIdx.x / 32, i0 = blockIdx.x * 256 + t * 8, r0 = blockIdx.y * 64 + group;
+    const int t = threadIdx.x % 32, group = threadIdx.x / 32, i0 = bx * 256 + t * 8, r0 = by * 64 + group;
     float s[8] = {}, v[8][8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -252,19 +251,18 @@ __global__ __launch_bounds__(256) void split_kernel(const T* __restrict__ y, bf1
 #pragma unroll
     for (int j = 0; j < 8; ++j) red[group][t * 8 + j] = s[j];
     __syncthreads();
-    const int col = blockIdx.x * 256 + threadIdx.x;
+    const int col = bx * 256 + threadIdx.x;
     float total = 0.f;
 #pragma unroll
     for (int g = 0; g < 8; ++g) total += red[g][threadIdx.x];
-    if (col < n) colsum[(long)blockIdx.y * n + col] = total;
+    if (col < n) colsum[(long)by * n + col] = (accumulate ? colsum[(long)by * n + col] : 0.f) + total;
 }
 
 // A microscaled [rows][groups * 128] -> bf16, by eights: `live` of them, then zeros up to `total`.
 template <int FMT>
-__global__ __launch_bounds__(256) void mx_rows_bf16_kernel(const unsigned char* __restrict__ codes,
-                                                           const unsigned char* __restrict__ scales, bf16_t* __restrict__ out,
-                                                           long live, long total) {
-    for (long at = (long)blockIdx.x * 256 + threadIdx.x; at < total; at += (long)gridDim.x * 256) {
+__device__ __forceinline__ void rows_block(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
+                                           bf16_t* __restrict__ out, long live, long total, int block, int blocks) {
+    for (long at = (long)block * 256 + threadIdx.x; at < total; at += (long)blocks * 256) {
         const float s = at < live ? mx_scale(scales[at / 4]) : 0.f;
         bf16x8 b;
         if (at >= live) {
@@ -281,20 +279,86 @@ __global__ __launch_bounds__(256) void mx_rows_bf16_kernel(const unsigned char* 
 }
 
 // Packed W -> [filled][groups * 128] bf16, outputs and then zeros: a lane turns 8 codes of one output into 16 bytes, 16 lanes write
-// 256 bytes of a row.
-__global__ __launch_bounds__(256) void mx_weights_bf16_kernel(const unsigned char* __restrict__ codes,
-                                                              const unsigned char* __restrict__ scales, bf16_t* __restrict__ out,
-                                                              int groups, int out_dim, int filled) {
-    const int c = threadIdx.x & 15, g = blockIdx.y;
+// 256 bytes of a row.  64 outputs of one group a workgroup.
+__device__ __forceinline__ void weights_block(const unsigned char* __restrict__ codes, const unsigned char* __restrict__ scales,
+                                              bf16_t* __restrict__ out, int groups, int out_dim, int filled, int bx, int g) {
+    const int c = threadIdx.x & 15;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int n = blockIdx.x * 64 + i * 16 + threadIdx.x / 16;
+        const int n = bx * 64 + i * 16 + threadIdx.x / 16;
         if (n >= filled) continue;
         const long at = min(n, out_dim - 1);
         const unsigned u = reinterpret_cast<const unsigned*>(codes)[(((long)g * 4 + c / 4) * out_dim + at) * 4 + c % 4];
         const float s = mx_scale(scales[((long)g * out_dim + at) * 4 + c / 4]);
         *reinterpret_cast<bf16x8*>(out + ((long)n * groups + g) * 128 + c * 8) = e2m1_to_bf16(n < out_dim ? u : 0u, n < out_dim ? s : 1.f);
     }
+}
+
+// All images that a call needs, in one launch: first the workgroups of dY, then A's, then W's.
+struct Images {
+    const void* dy;
+    bf16_t* y;
+    float* colsum;
+    int rows, n;
+    bool vec;
+    int accumulate;                 // into colsum: up to 64 rows, of which it is dbias itself
+    const unsigned char *a_codes, *a_scales;
+    bf16_t* a;
+    long live, total;
+    const unsigned char *w_codes, *w_scales;
+    bf16_t* w;
+    int groups, out_dim, filled;
+    int y_blocks, a_blocks, w_blocks;
+};
+template <typename T, int FMT>
+__global__ __launch_bounds__(256) void images_kernel(Images p) {
+    __shared__ float red[8][256];
+    int b = blockIdx.x;
+    if (b < p.y_blocks) {
+        const int across = (int)((to64(p.n) + 255) / 256);
+        split_block(static_cast<const T*>(p.dy), p.y, p.colsum, p.rows, p.n, p.vec, p.accumulate, b % across, b / across, red);
+        return;
+    }
+    b -= p.y_blocks;
+    if (b < p.a_blocks) {
+        rows_block<FMT>(p.a_codes, p.a_scales, p.a, p.live, p.total, b, p.a_blocks);
+        return;
+    }
+    b -= p.a_blocks;
+    weights_block(p.w_codes, p.w_scales, p.w, p.groups, p.out_dim, p.filled, b / p.groups, b % p.groups);
+}
+// Adds A [rows][groups * 128], filled up to `filled` rows, or W, filled up to `filled` outputs, to the images of a call.
+static void add_a(Images& m, const void* codes, const void* scales, bf16_t* a, long rows, long filled, int in_dim) {
+    m.a_codes = static_cast<const unsigned char*>(codes);
+    m.a_scales = static_cast<const unsigned char*>(scales);
+    m.a = a;
+    m.live = rows * mx_groups(in_dim) * 16;
+    m.total = filled * mx_groups(in_dim) * 16;
+    const long blocks = (m.total + 255) / 256;
+    m.a_blocks = (int)(blocks < 8192 ? blocks : 8192);
+}
+static void add_w(Images& m, const void* codes, const void* scales, bf16_t* w, int in_dim, int out_dim, int filled) {
+    m.w_codes = static_cast<const unsigned char*>(codes);
+    m.w_scales = static_cast<const unsigned char*>(scales);
+    m.w = w;
+    m.groups = mx_groups(in_dim);
+    m.out_dim = out_dim;
+    m.filled = filled;
+    m.w_blocks = (filled + 63) / 64 * m.groups;
+}
+template <typename T>
+static void make_images(const Images& m, int fmt, hipStream_t st) {
+    const dim3 grid((unsigned)m.y_blocks + (unsigned)m.a_blocks + (unsigned)m.w_blocks);
+    if (grid.x == 0) return;
+    if (fmt == GAN_MX_E4M3) hipLaunchKernelGGL((images_kernel<T, GAN_MX_E4M3>), grid, dim3(256), 0, st, m);
+    else hipLaunchKernelGGL((images_kernel<T, GAN_MX_E2M1>), grid, dim3(256), 0, st, m);
+}
+void mx_product_images(int fmt, const void* a_codes, const void* a_scales, bf16_t* a, int rows, const void* w_codes, const void* w_scales,
+                       bf16_t* w, int in_dim, int out_dim, hipStream_t st) {
+    Images m{};
+    add_a(m, a_codes, a_scales, a, rows, rows, in_dim);
+    add_w(m, w_codes, w_scales, w, in_dim, out_dim, out_dim);
+    make_images<float>(m, fmt, st);
 }
 
 // dbias[n] (+)= sum over blocks of 64 rows.
@@ -312,25 +376,6 @@ __global__ __launch_bounds__(256) void mx_dbias_kernel(const float* __restrict__
         for (int i = 0; i < 8; ++i) s += red[i][threadIdx.x];
         out[col] = (accumulate ? out[col] : 0.f) + s;
     }
-}
-
-static dim3 flat_grid(long items) {
-    const long blocks = (items + 255) / 256;
-    return dim3((unsigned)(blocks < 8192 ? (blocks < 1 ? 1 : blocks) : 8192));
-}
-
-void mx_rows_to_bf16(int fmt, const void* codes, const void* scales, bf16_t* out, long rows, long filled, int in_dim, hipStream_t st) {
-    const long live = rows * mx_groups(in_dim) * 16, total = filled * mx_groups(in_dim) * 16;
-    const unsigned char* c = static_cast<const unsigned char*>(codes);
-    const unsigned char* s = static_cast<const unsigned char*>(scales);
-    if (fmt == GAN_MX_E4M3) hipLaunchKernelGGL(mx_rows_bf16_kernel<GAN_MX_E4M3>, flat_grid(total), dim3(256), 0, st, c, s, out, live, total);
-    else hipLaunchKernelGGL(mx_rows_bf16_kernel<GAN_MX_E2M1>, flat_grid(total), dim3(256), 0, st, c, s, out, live, total);
-}
-
-void mx_weights_to_bf16(const void* codes, const void* scales, bf16_t* out, int in_dim, int out_dim, int filled, hipStream_t st) {
-    hipLaunchKernelGGL(mx_weights_bf16_kernel, dim3((filled + 63) / 64, mx_groups(in_dim)), dim3(256), 0, st,
-                       static_cast<const unsigned char*>(codes), static_cast<const unsigned char*>(scales), out, mx_groups(in_dim),
-                       out_dim, filled);
 }
 
 static int parts_of(int dtype) { return dtype == GAN_BF16 ? 1 : dtype == GAN_F16 ? 2 : 3; }
@@ -405,19 +450,28 @@ static int gradients(const Gradients& g, void* ws, size_t ws_bytes, hipStream_t 
     const long np = to64(g.out_dim);
     return with_dtype(g.dtype, [&](auto* tag) {
         typedef typename std::remove_pointer<decltype(tag)>::type T;
-        if (image || colsum)
-            hipLaunchKernelGGL((split_kernel<T>), dim3((unsigned)((np + 255) / 256), blocks), dim3(256), 0, st, static_cast<const T*>(g.dy),
-                               image, colsum, g.rows, g.out_dim, g.out_dim * sizeof(T) % 16 == 0);
+        Images m{};
+        if (image || colsum) {
+            m.dy = g.dy;
+            m.y = image;
+            m.colsum = colsum && blocks == 1 ? g.dbias : colsum;
+            m.accumulate = blocks == 1 && g.accumulate;
+            m.rows = g.rows;
+            m.n = g.out_dim;
+            m.vec = g.out_dim * sizeof(T) % 16 == 0;
+            m.y_blocks = (int)((np + 255) / 256) * blocks;
+        }
+        if (dm) add_a(m, g.a_codes, g.a_scales, a, g.rows, im.rp, g.in_dim);
+        if (dx) add_w(m, g.w_codes, g.w_scales, w, g.in_dim, g.out_dim, (int)np);
+        make_images<T>(m, g.fmt, st);
         if (dm) {
-            if (g.dbias)
+            if (g.dbias && blocks > 1)
                 hipLaunchKernelGGL(mx_dbias_kernel, dim3((g.out_dim + 31) / 32), dim3(256), 0, st, colsum, g.dbias, blocks, g.out_dim,
                                    g.accumulate);
-            mx_rows_to_bf16(g.fmt, g.a_codes, g.a_scales, a, g.rows, im.rp, g.in_dim, st);
             const Bf16Product p{a, y, im.kp, im.ldy, 0, im.rp * im.ldy, parts, (int)im.rp, g.in_dim, g.out_dim, nullptr, g.accumulate};
             if (const int rc = bf16_product<true, true>(p, g.dmatrix, base + im.slabs, st, what)) return rc;
         }
         if (!dx) return 0;
-        mx_weights_to_bf16(g.w_codes, g.w_scales, w, g.in_dim, g.out_dim, (int)np, st);
         const Bf16Product p{y, w, im.ldy, im.kp, im.rp * im.ldy, 0, parts, (int)np, g.rows, g.in_dim, nullptr, 0};
         return bf16_product<false, true>(p, static_cast<T*>(g.dx), base + im.slabs, st, what);
     });

@@ -452,8 +452,7 @@ static int mx_product(int dtype, int fmt, int rows, int in_dim, int out_dim, con
         const int kp = mx_groups(in_dim) * 128;
         bf16_t* a = static_cast<bf16_t*>(ws);
         bf16_t* w = a + (long)rows * kp;
-        mx_rows_to_bf16(fmt, a_codes, a_scales, a, rows, rows, in_dim, st);
-        mx_weights_to_bf16(w_codes, w_scales, w, in_dim, out_dim, out_dim, st);
+        mx_product_images(fmt, a_codes, a_scales, a, rows, w_codes, w_scales, w, in_dim, out_dim, st);
         const Bf16Product p{a, w, kp, kp, 0, 0, 1, kp, rows, out_dim, bias, 0};
         return bf16_product<false, false>(p, static_cast<float*>(y), w + (long)out_dim * kp, st, what);
     }
