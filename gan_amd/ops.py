@@ -836,12 +836,12 @@ def _plain(t):
     return t.detach().contiguous()
 
 
-def _variable(st, scope, leaf, shape, initializer):
+def _variable(st, scope, leaf, shape, initializer, reuse=None):
     """The variable `scope`/`leaf` under the current scope; one that is there already without entering the scope."""
     var = st.vars.get('/'.join(st._scope + [scope, leaf]))
     if var is not None and var.shape == shape:
         return var
-    with st.variable_scope(scope):
+    with st.variable_scope(scope, reuse=reuse):
         return st.get_variable(leaf, shape, initializer)
 
 
@@ -1039,10 +1039,12 @@ def mx_pack(matrix):
     _lib.here(matrix)
     m, k, n, ld = _rows_of(matrix.detach())
     g = _mx_groups(k)
-    codes = torch.empty((g * 4, n, 16), dtype=torch.uint8, device=m.device)
-    scales = torch.empty((g, n, 4), dtype=torch.uint8, device=m.device)
-    check(lib.gan_mx_pack(code, k, n, m.data_ptr(), ld, codes.data_ptr(), scales.data_ptr(), stream()))
-    return MxMatrix(codes, scales, k, n)
+    w = MxMatrix.__new__(MxMatrix)
+    w.codes = torch.empty((g * 4, n, 16), dtype=torch.uint8, device=m.device)
+    w.scales = torch.empty((g, n, 4), dtype=torch.uint8, device=m.device)
+    w.in_dim, w.out_dim = k, n
+    check(lib.gan_mx_pack(code, k, n, m.data_ptr(), ld, w.codes.data_ptr(), w.scales.data_ptr(), stream()))
+    return w
 
 
 def mx_dequantize(q, dtype=None):
@@ -1162,10 +1164,9 @@ def linear_mx(input_, output_size, scope_name=None, stddev=0.02, bias_start=0.0,
     the input -- fp32, bf16, fp16 or an `MxTensor` of any rank -- to `fmt`.  Gradients are those of the product of the quantised
     values, passed straight through both quantisers."""
     st = V.default_store()
-    width = int(input_.shape[-1])
-    with st.variable_scope(scope_name or "Linear", reuse=reuse):
-        matrix = st.get_variable("Matrix", [width, output_size], V.random_normal_initializer(stddev))
-        bias = st.get_variable("bias", [output_size], V.constant_initializer(bias_start))
+    width, output_size, scope = int(input_.shape[-1]), int(output_size), scope_name or "Linear"
+    matrix = _variable(st, scope, "Matrix", (width, output_size), V.random_normal_initializer(stddev), reuse)
+    bias = _variable(st, scope, "bias", (output_size,), V.constant_initializer(bias_start), reuse)
     device = input_.codes.device if isinstance(input_, MxTensor) else input_.device
     token = _grad_token(device, matrix) if torch.is_grad_enabled() else None
     y = _mx_apply(input_, mx_pack(matrix.data), bias.data, fmt, token, matrix, bias)

@@ -193,3 +193,20 @@ def test_both_gradients_at_once_are_refused_without_their_parts():
     _refused(call(a=None), b"null")
     _refused(call(dy=odd), b"aligned")
     _refused(call(n=need - 1), b"workspace")
+
+
+def test_linear_mx_shares_linears_variables():
+    """By name, shape and reuse, as `linear` does (the products themselves need a GPU)."""
+    from gan_amd import ops
+    from gan_amd import variables as V
+    st = V.VariableStore(device='cpu')
+    with V.use_store(st):
+        with pytest.raises(ValueError):
+            ops.linear_mx(torch.zeros(2, 8), 3, 'head', reuse=True)         # nothing there to share
+        with st.variable_scope('net'):
+            a = ops._variable(st, 'head', 'Matrix', (8, 3), V.random_normal_initializer(0.02))
+        assert list(st.vars) == ['net/head/Matrix'] and a.shape == (8, 3)
+        with st.variable_scope('net'):
+            assert ops._variable(st, 'head', 'Matrix', (8, 3), V.random_normal_initializer(0.02), True) is a
+            with pytest.raises(ValueError):
+                ops.linear_mx(torch.zeros(2, 7), 3, 'head')                  # another shape
