@@ -360,8 +360,8 @@ static MxPlan mx_plan(int dtype, int fmt, int rows, int in_dim, int out_dim) {
     // (1 x 1024 x 65536 22 against 10).
     const long wgs = (long)((out_dim + 15) / 16) * (rows <= 16 ? 1 : (rows + 31) / 32);
     const bool f32 = fmt == GAN_MX_E4M3 && dtype == GAN_F32;
-    // (fp32 results: against the images and the bf16 product, both as measured: 64 x 8192 x 8192 53 us against 76, 96 rows 78
-    // against 78, 64 x 1024 x 16384 52 against 35)
+    // (fp32 results: against the images and the bf16 product, both as measured: 64 x 8192 x 8192 53 us against 71, 96 rows 78
+    // against 73, 64 x 1024 x 16384 52 against 26, 80 x 2048 x 4096 20 against 25)
     const bool few = wgs <= (rows <= 16 ? 512 : 256) || (rows <= 8 && groups >= 32) ||
                      (f32 && rows <= 128 && wgs * (0.021 + 0.000475 * groups) <= 18 + 0.85e-6 * in_dim * out_dim);
     if (few) {
