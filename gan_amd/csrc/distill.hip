@@ -274,7 +274,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
             for (int j = 0; j < N; ++j) m = fmaxf(m, v[j]);
         }
         const float off = m == -INFINITY ? 0.f : m;
-        own = off;
+        own = m;        // (of a thread with masked classes alone -inf, whose power is 0)
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if (i * NT + wave0 >= chunks) continue;
