@@ -4,7 +4,8 @@
 //   differences are taken before the division, which could carry a mask of the type's lowest value to -inf
 //   p_i = softmax of t' over the list, or exp(t'_i - lse) where the teacher's log-sum-exp is given
 //   l = sum_i p_i (log p_i - log q_i)  [+ p_r (log p_r - log q_r)],   q = softmax z
-//   p_r = max(0, 1 - sum p), q_r = sum of q over the classes not listed (with lse only)
+//   p_r = max(0, 1 - sum p), q_r = sum of q over the classes not listed (with lse only; where q_r is 0, with every class listed or
+//   all others at -inf, l has no such term and p_r is 0)
 //   dl/dz_j = P q_j - p_j (listed), P q_j - p_r q_j / q_r (others), P = sum p + p_r
 //
 // Memory-bound: the logits are read once, held in registers, and their gradient is written once (2048 x 131072 bf16, the half of a
@@ -106,7 +107,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
     constexpr bool kKeep = sizeof(T) == 4;      // a power takes the place of its value, and is not computed twice
     extern __shared__ __align__(16) unsigned char lds[];
     __shared__ float red[2 * NT / 64];
-    // of the list: any, P, p_r, maximum, sum of powers, repeated classes
+    // of the list: any, sum p, p_r, maximum, sum of powers, repeated classes
     __shared__ float told[6];
     __shared__ float wsum[NT / 64];
     const int tid = threadIdx.x, lane = tid & 63, classes = p.classes;
@@ -205,7 +206,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
         if (lane == 0) {
             const float rest = REST ? fmaxf(0.f, 1.f - mass) : 0.f;
             told[0] = any ? 1.f : 0.f;
-            told[1] = REST ? mass + rest : 1.f;
+            told[1] = REST ? mass : 1.f;
             told[2] = rest;
             told[3] = ml;
             told[4] = sl;
@@ -318,11 +319,13 @@ __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
         m = wave_all_max(mi);
         s = wave_all_sum(si * power(mi, m, c2));
     }
-    const float P = told[1], rest = told[2];
     float mall = m, sall = s;
     if (REST) join_stats(mall, sall, told[3], told[4], c2);
     const float log_sall = logf(sall);
+    // (classes outside the list, if any has mass: m is their maximum)
+    const float rest = told[2];
     const bool there = REST && rest > 0.f && m > -INFINITY;
+    const float P = told[1] + (there ? rest : 0.f);
     const float gs = total != 0.f ? p.grad_scale * (w / total) : 0.f;
     if (p.grad) {
         // e^((x - m) / tau) times one factor for every class that is not listed

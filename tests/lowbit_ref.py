@@ -75,7 +75,7 @@ def distill(logits, teacher, index, tau=1.0, weight=1.0, row_weight=None, lse=No
         logp = torch.log_softmax(t - t.max(), 0) if lse is None else t - float(lse[r])
         p = torch.exp(logp)
         rest = 0.0 if lse is None else max(0.0, 1.0 - float(p.sum()))
-        mass = (float(p.sum()) if lse is not None else 1.0) + rest
+        mass = float(p.sum()) if lse is not None else 1.0
         l = sum(float(pi) * (float(lp) - float(logq[i])) for (i, _), pi, lp in zip(at, p, logp))
         g, used = mass * q, q.clone()
         if lse is not None:
@@ -88,7 +88,8 @@ def distill(logits, teacher, index, tau=1.0, weight=1.0, row_weight=None, lse=No
                 # the log of their number
                 share = torch.where(outside, torch.exp(z - z[outside].max()), torch.zeros_like(q))
                 share = share / share.sum()
-                g = g - rest * share
+                # (only here: a loss without the term of the remaining mass has a gradient without it)
+                g = g + rest * q - rest * share
                 used = used + rest * share
         for (i, _), pi in zip(at, p):
             g[i] -= float(pi)

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import lowbit_ref as R
-from test_gpu_lowbit import TYPES, _check_distill, _lists, gen, ids, normal
+from test_gpu_lowbit import TYPES, _check_distill, _lists, gen, ids, normal, tiny
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +34,29 @@ def test_distillation_of_low_logits_with_masked_runs(rows, classes, masked, dtyp
     w = (torch.arange(rows, device='cuda') % max(1, rows // 40) == 0).float()
     _, grad = _check_distill(logits, teacher, index, tau, 1.0, w, lse)
     assert (grad[:, lo:hi] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("rows,classes,top,outside", [(3, 1, 1, "listed"), (2, 10, 10, "listed"), (3, 100, 100, "listed"), (2, 1024, 1024, "listed"),
+                                                      (2051, 9, 9, "listed"), (3, 100, 100, "listed twice"), (2, 300, 5, "masked"),
+                                                      (3, 4100, 33, "masked"), (2, 70000, 9, "masked"), (2, 140001, 3, "masked"),
+                                                      (2050, 130, 7, "masked"), (4, 500, 20, "masked in some rows")])
+def test_distillation_with_nothing_outside_the_list(rows, classes, top, outside, dtype):
+    """The teacher's remaining mass is left out of the loss, and out of its gradient, where no class outside the list has any: a row's
+    gradient adds up to 0.  Allowed: 2^-17 and a half step of the type for each class by its size, q + p <= 2 in all."""
+    g = gen(rows + classes + top)
+    logits = (2 * normal(g, rows, classes)).to(dtype)
+    index, teacher = _lists(g, rows, classes, top, torch.float32)
+    if outside == "listed twice":
+        index[:, 1] = index[:, 0]
+        logits.scatter_(1, torch.stack([(torch.bincount(i, minlength=classes) == 0).nonzero()[0] for i in index]), -math.inf)
+    if outside.startswith("masked"):
+        keep = logits.gather(1, index)
+        some = slice(None) if outside == "masked" else slice(0, None, 2)
+        logits[some] = -math.inf
+        logits.scatter_(1, index, keep)
+    lse = torch.logsumexp(teacher / 1.5, 1) + 0.4
+    w = (torch.arange(rows, device='cuda') % max(1, rows // 40) == 0).float()
+    _, grad = _check_distill(logits, teacher, index, 1.5, 0.7, w, lse)
+    allowed = 2 * (2.0 ** -17 + torch.finfo(dtype).eps / 2) * 0.7 * 1.5 / float(w.sum()) + classes * tiny(dtype)
+    assert (grad.double().sum(1).abs() <= allowed).all()

@@ -1,0 +1,31 @@
+"""Distillation, norm and microscaled products at the edges of what they document, without a GPU."""
+import math
+
+import pytest
+import torch
+
+import lowbit_ref as R
+from test_lowbit_host import _differences
+
+
+@pytest.mark.parametrize("outside", ["listed", "masked", "one masked", "free"])
+def test_distillation_gradient_against_differences_with_nothing_outside_the_list(outside):
+    """With the teacher's log-sum-exp: every class listed, or all others at -inf, leaves the loss without the term of the remaining
+    mass, and the gradient is that of what is left.  Divergences of q do not see a shift of the logits, so a row's gradient adds up
+    to (1 - 1) or (sum p - sum p) times its scale: 0."""
+    g = torch.Generator().manual_seed(5)
+    classes, top = 7, 7 if outside == "listed" else 4
+    logits = torch.randn(3, classes, generator=g, dtype=torch.float64)
+    index = torch.stack([torch.randperm(classes, generator=g)[:top] for _ in range(3)])
+    teacher = torch.randn(3, top, generator=g, dtype=torch.float64)
+    free = torch.ones(3, classes, dtype=torch.bool).scatter_(1, index, False)
+    if outside == "masked":
+        logits[free] = -math.inf
+    if outside == "one masked":
+        logits[1][free[1]] = -math.inf
+    lse = torch.logsumexp(teacher / 1.5, 1) + 0.4
+    w = torch.tensor([1.0, 0.5, 2.0])
+    f = lambda v: R.distill(v, teacher, index, 1.5, 0.7, w, lse)[0]
+    grad = R.distill(logits, teacher, index, 1.5, 0.7, w, lse)[1]
+    assert torch.allclose(grad, _differences(f, logits), atol=1e-8)
+    assert torch.allclose(grad.sum(1), torch.zeros(3, dtype=torch.float64), atol=1e-12)
