@@ -1154,8 +1154,10 @@ def _mx_apply(x, w, bias, fmt, token=None, matrix=None, bias_var=None):
 def mx_matmul(x, w, bias=None, fmt='e4m3'):
     """Extension: x W + bias with packed 4-bit weights (`mx_pack`) and microscaled activations; sums are fp32, the result has x's
     type.  x: fp32, bf16 or fp16 [..., in_dim], quantised to `fmt` ('e4m3' or 'e2m1') on the way, or an `MxTensor` (its own
-    format counts).  bias: fp32 [out_dim].  The weights are frozen here: the backward pass gives x its gradient, straight
-    through the rounding of x."""
+    format counts).  bias: fp32 [out_dim].  Weights and bias are frozen here: the backward pass gives x its gradient, straight
+    through the rounding of x; a bias that waits for one is refused (`linear_mx` trains both)."""
+    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
+        raise ValueError("mx_matmul: the bias is frozen and gets no gradient (detach it, or train it with linear_mx)")
     return _mx_apply(x, w, bias, fmt)
 
 

@@ -29,3 +29,19 @@ def test_distillation_gradient_against_differences_with_nothing_outside_the_list
     grad = R.distill(logits, teacher, index, 1.5, 0.7, w, lse)[1]
     assert torch.allclose(grad, _differences(f, logits), atol=1e-8)
     assert torch.allclose(grad.sum(1), torch.zeros(3, dtype=torch.float64), atol=1e-12)
+
+
+def test_a_bias_that_waits_for_a_gradient_is_refused():
+    """The product's weights and bias are frozen: a gradient that never comes is not to be waited for."""
+    from gan_amd import ops
+    from gan_amd._lib import GanHipError
+    u8 = lambda *s: torch.zeros(*s, dtype=torch.uint8)
+    w, x = ops.MxMatrix(u8(4, 10, 16), u8(1, 10, 4), 100, 10), torch.zeros(3, 100)
+    bias = torch.zeros(10, requires_grad=True)
+    for rows in (x, x.clone().requires_grad_(True), ops.MxTensor(u8(3, 128), u8(3, 4), 100)):
+        with pytest.raises(ValueError, match="bias"):
+            ops.mx_matmul(rows, w, bias)
+        for frozen in (bias.detach(), None):
+            with pytest.raises((GanHipError, RuntimeError)) as e:       # (goes on to the library, which has no GPU here)
+                ops.mx_matmul(rows, w, frozen)
+            assert "bias" not in str(e.value)
