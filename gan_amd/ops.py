@@ -880,9 +880,9 @@ class _RmsNormFn(torch.autograd.Function):
         out, h, rstd, (kept, ctx.ld) = _rms_fwd(x, residual, gamma, eps, mx, True)
         ctx.save_for_backward(kept, rstd)
         ctx.gamma = gamma
-        if mx:      # autograd sees a stand-in of the norm's shape and type; the codes go around it
+        if mx:      # the codes go around autograd
             made.append(out)
-            out = torch.empty(1, dtype=x.dtype, device=x.device).expand(x.shape)
+            out = _stand_in(x)
         return out if h is None else (out, h)
 
     @staticmethod
@@ -1016,8 +1016,26 @@ def _mx_empty(shape, fmt, dtype, device):
     return q
 
 
+def _stand_in(x):
+    """What autograd sees in the place of microscaled values: of x's shape and type, without its memory."""
+    return torch.empty(1, dtype=x.dtype, device=x.device).expand(x.shape)
+
+
+class _MxTicketFn(torch.autograd.Function):
+    """The gradient of quantised values, handed on to what was quantised."""
+
+    @staticmethod
+    def forward(ctx, x):
+        return _stand_in(x)
+
+    @staticmethod
+    def backward(ctx, dy):
+        return dy
+
+
 def mx_quantize(x, fmt='e4m3'):
-    """x (fp32, bf16 or fp16) as an `MxTensor` in blocks of 32 along its last axis (include/gan_hip.h has the rounding rule)."""
+    """x (fp32, bf16 or fp16) as an `MxTensor` in blocks of 32 along its last axis (include/gan_hip.h has the rounding rule).
+    Gradients pass straight through the rounding to x."""
     if fmt not in _lib.MX_FORMATS:
         raise ValueError("mx_quantize: unknown format %r (e4m3 or e2m1)" % (fmt,))
     if x.dim() < 1 or x.shape[-1] < 1:
@@ -1027,12 +1045,14 @@ def mx_quantize(x, fmt='e4m3'):
     xs, rows, c, ld = _rows_of(x.detach())
     q = _mx_empty(x.shape, fmt, x.dtype, x.device)
     check(lib.gan_mx_quantize(code, _lib.MX_FORMATS[fmt], rows, c, xs.data_ptr(), ld, q.codes.data_ptr(), q.scales.data_ptr(), stream()))
+    if x.requires_grad and torch.is_grad_enabled():
+        q.ticket = _MxTicketFn.apply(x)
     return q
 
 
 def mx_pack(matrix):
     """A weight matrix [in_dim, out_dim] (fp32, bf16 or fp16; `linear`'s Matrix) quantised to e2m1 in blocks of 32 inputs, in the
-    layout the products read.  A serving program packs its weights once and keeps the `MxMatrix`."""
+    layout the products read.  A serving program packs its weights once and keeps the `MxMatrix`, which is outside of autograd."""
     if matrix.dim() != 2 or matrix.shape[0] < 1 or matrix.shape[1] < 1:
         raise ValueError("mx_pack expects a rank-2 matrix, got shape %s" % (tuple(matrix.shape),))
     code = _lib.dtype_code(matrix.dtype)

@@ -60,3 +60,32 @@ def test_distillation_with_nothing_outside_the_list(rows, classes, top, outside,
     _, grad = _check_distill(logits, teacher, index, 1.5, 0.7, w, lse)
     allowed = 2 * (2.0 ** -17 + torch.finfo(dtype).eps / 2) * 0.7 * 1.5 / float(w.sum()) + classes * tiny(dtype)
     assert (grad.double().sum(1).abs() <= allowed).all()
+
+
+# ------------------------------------------------------------------------------------------------ products
+@pytest.mark.parametrize("fmt", ['e4m3', 'e2m1'])
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+def test_gradients_pass_through_values_quantised_beforehand(dtype, fmt):
+    """`mx_quantize` and then the product: the input's gradient is that of the product given floats, to the bit; a second use adds up;
+    rows seen through a stride are reached as well."""
+    from gan_amd import ops
+    g = gen(61)
+    w = ops.mx_pack(normal(g, 100, 40))
+    x = normal(g, 30, 100).to(dtype).requires_grad_(True)
+    dy = normal(g, 30, 40).to(dtype)
+    want, = torch.autograd.grad((ops.mx_matmul(x, w, fmt=fmt),), (x,), (dy,))
+    q = ops.mx_quantize(x, fmt)
+    y = ops.mx_matmul(q, w)
+    got, = torch.autograd.grad((y,), (x,), (dy,))
+    assert torch.equal(got, want)
+    # (two equal gradients add up without a rounding)
+    twice, = torch.autograd.grad([ops.mx_matmul(q, w), ops.mx_matmul(q, w)], (x,), (dy, dy))
+    assert torch.equal(twice, 2 * want)
+    wide = normal(g, 30, 130).to(dtype)
+    wide[:, 7:107] = x.detach()
+    wide.requires_grad_(True)
+    got, = torch.autograd.grad((ops.mx_matmul(ops.mx_quantize(wide[:, 7:107], fmt), w),), (wide,), (dy,))
+    assert torch.equal(got[:, 7:107], want) and (got[:, :7] == 0).all() and (got[:, 107:] == 0).all()
+    with torch.no_grad():
+        assert ops.mx_quantize(x, fmt).ticket is None
+    assert ops.mx_quantize(x.detach(), fmt).ticket is None
