@@ -19,6 +19,8 @@ backward; every forward and backward computation is a call into the HIP library.
 gradients are not returned through autograd: the backward of each layer writes them straight into
 the owning optimiser group's gradient arena when that variable is being trained in the current
 update (`Variable.wants_grad`), which is how `minimize(loss, var_list=...)` restricts the work.
+No layer or loss has second derivatives: a gradient is a kernel's result, and autograd does not see what it
+depends on (create_graph=True gives gradients that are cut off from the graph).
 """
 import ctypes
 import math
@@ -1498,7 +1500,8 @@ def distill_topk_mean(logits, teacher_logits, teacher_index, temperature=1.0, we
     list) or a logit of -inf are left out.  Without teacher_lse the list is taken for the whole distribution; with it (fp32
     [...], log-sum-exp of ALL the teacher's logits / temperature) the mass that is not listed is one more class, held against
     the student's whole mass outside the list.
-    row_weight (fp32 [...]): the mean is sum(w l) / sum(w).  Rows of weight 0 and rows with an empty list have loss and gradient 0."""
+    row_weight (fp32 [...]): the mean is sum(w l) / sum(w).  Rows of weight 0 and rows with an empty list have loss and gradient 0.
+    The gradient is the logits' alone; the teacher's tensors and the weights are constants."""
     lead = tuple(logits.shape[:-1])
     if logits.dim() < 1 or logits.numel() == 0:
         raise ValueError("distill_topk_mean: no logits in shape %s" % (tuple(logits.shape),))
