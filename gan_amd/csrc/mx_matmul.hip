@@ -396,18 +396,22 @@ static int launch_tile(const MxProduct& p, hipStream_t st) {
 
 // A workgroup quantises up to this many floats itself: 4 rounds of its 512 threads by 8 values, about 1 us; as a launch of its own
 // the quantisation takes 3 us and the gap between the two.  In a grid of at most one workgroup a CU, each with a tile of 16 rows, it may
-// be more: 64 x 1024 x 1024 e4m3 4.8 us against 7.7, 64 x 2048 x 512 6.5 against 7.8, 64 x 2400 x 256 7.4 against 7.3 (e2m1 7.6 against
-// 6.0), where a caller outside a graph still has a launch less to make (15 us a call against 10).
-constexpr int kFusedValues = 16384, kFusedValuesAlone = 40960;
+// be more, up to where both ways take as long inside a graph: 2560 inputs for 16 rows of e4m3, 2048 of e2m1, whose codes are half as
+// many bytes to write and read back.  us in one launch and in two, fp32, 256 outputs (1024 of 64 rows take 0.2 more): 64 rows e4m3
+// 1024 inputs 4.8 / 7.8, 2048 6.6 / 8.0, 2304 7.1 / 7.5, 2560 7.4 / 7.6; e2m1 1024 4.8 / 7.0, 2048 6.6 / 7.1, 2176 6.7 / 6.3, 2560
+// 7.4 / 6.7.  As many values of fewer rows meet a little earlier: 8 rows e4m3 4096 6.8 / 7.2, 5120 7.8 / 7.5, e2m1 3584 6.2 / 6.3, 4096
+// 6.8 / 6.7.
+constexpr int kFusedValues = 16384, kFusedValuesAlone = 40960, kFusedValuesAlone4 = 32768;
 
 // Workgroups of 16 rows x 16 outputs.  At most one a CU, they have the chip's waves to themselves and sharing fragments does not pay:
 // 64 x 1024 x 1024 e4m3 from codes 5.4 us against 8.0 with 32 rows each; 32 x 4096 x 4096, two a CU, 9.2 against 8.8.
 static long few_grid(int rows, int out_dim, int splits) { return (long)((out_dim + 15) / 16) * ((rows + 15) / 16) * splits; }
 
-static bool mx_fused(const MxPlan& plan, int rows, int in_dim, int out_dim) {
+static bool mx_fused(const MxPlan& plan, int fmt, int rows, int in_dim, int out_dim) {
     if (plan.kind != MX_FEW) return false;
     const long values = (long)(rows < 16 ? rows : 16) * ((mx_groups(in_dim) + plan.splits - 1) / plan.splits) * 128;
-    return (rows <= 16 && values <= kFusedValues) || (few_grid(rows, out_dim, plan.splits) <= 256 && values <= kFusedValuesAlone);
+    return (rows <= 16 && values <= kFusedValues) ||
+           (few_grid(rows, out_dim, plan.splits) <= 256 && values <= (fmt == GAN_MX_E4M3 ? kFusedValuesAlone : kFusedValuesAlone4));
 }
 
 template <typename T, int FMT>
@@ -500,7 +504,7 @@ size_t gan_mx_linear_workspace_bytes(int dtype, int fmt, int rows, int in_dim, i
     if (rows < 1 || rows > GAN_MX_MAX_ROWS || in_dim < 1 || in_dim > GAN_MX_MAX_IN || out_dim < 1 || out_dim > GAN_MX_MAX_IN || !dtype_ok(dtype) || !mx_fmt_ok(fmt))
         return 0;
     const size_t own = gan_mx_matmul_workspace_bytes(dtype, fmt, rows, in_dim, out_dim);
-    if (mx_fused(mx_plan(dtype, fmt, rows, in_dim, out_dim), rows, in_dim, out_dim)) return own;
+    if (mx_fused(mx_plan(dtype, fmt, rows, in_dim, out_dim), fmt, rows, in_dim, out_dim)) return own;
     return own + mx_codes_bytes(fmt, rows, in_dim) + mx_scales_bytes(rows, in_dim);
 }
 
@@ -517,7 +521,7 @@ int gan_mx_linear(int dtype, int fmt, int rows, int in_dim, int out_dim, const v
     const size_t need = gan_mx_linear_workspace_bytes(dtype, fmt, rows, in_dim, out_dim);
     GAN_CHECK_ARG(ws_bytes >= need && (need == 0 || (ws && aligned16(ws))),
                   "gan_mx_linear: workspace of %zu bytes needed (16-byte aligned), %zu given", need, ws_bytes);
-    if (mx_fused(mx_plan(dtype, fmt, rows, in_dim, out_dim), rows, in_dim, out_dim))
+    if (mx_fused(mx_plan(dtype, fmt, rows, in_dim, out_dim), fmt, rows, in_dim, out_dim))
         return mx_product(dtype, fmt, rows, in_dim, out_dim, x, ldx, nullptr, nullptr, w_codes, w_scales, bias, y, ws, as_stream(stream),
                           "gan_mx_linear");
     unsigned char* codes = static_cast<unsigned char*>(ws);

@@ -45,3 +45,13 @@ def test_a_bias_that_waits_for_a_gradient_is_refused():
             with pytest.raises((GanHipError, RuntimeError)) as e:       # (goes on to the library, which has no GPU here)
                 ops.mx_matmul(rows, w, frozen)
             assert "bias" not in str(e.value)
+
+
+def test_rows_are_quantised_in_the_products_launch_up_to_where_a_launch_of_their_own_is_as_fast():
+    """A call that quantises in the product's launch asks for no codes beside the product's own workspace."""
+    from gan_amd import _lib as L
+    one = lambda fmt, rows, k, n: L.lib.gan_mx_linear_workspace_bytes(0, fmt, rows, k, n) == L.lib.gan_mx_matmul_workspace_bytes(0, fmt, rows, k, n)
+    e4m3, e2m1 = L.MX_FORMATS['e4m3'], L.MX_FORMATS['e2m1']
+    for rows, n in ((64, 256), (17, 1000), (250, 250), (16, 4000)):
+        assert [one(e4m3, rows, k, n) for k in (100, 2048, 2400, 2560, 2561)] == [True] * 4 + [False], (rows, n)
+        assert [one(e2m1, rows, k, n) for k in (100, 2048, 2049, 2400, 2560)] == [True] * 2 + [False] * 3, (rows, n)
