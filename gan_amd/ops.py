@@ -1174,8 +1174,10 @@ def _mx_apply(x, w, bias, fmt, token=None, matrix=None, bias_var=None):
 
 
 def mx_matmul(x, w, bias=None, fmt='e4m3'):
-    """Extension: x W + bias with packed 4-bit weights (`mx_pack`) and microscaled activations; sums are fp32, the result has x's
-    type.  x: fp32, bf16 or fp16 [..., in_dim], quantised to `fmt` ('e4m3' or 'e2m1') on the way, or an `MxTensor` (its own
+    """Extension: x W + bias with packed 4-bit weights (`mx_pack`) and microscaled activations; the result has x's type.  Sums are
+    fp32, of exact products -- but for e4m3 rows with bf16 or fp16 results, many at once, where of every eight neighbouring products
+    what lies below 2^-13 of the largest is cut off (include/gan_hip.h): the last bits of a row may then depend on how many rows come
+    with it.  x: fp32, bf16 or fp16 [..., in_dim], quantised to `fmt` ('e4m3' or 'e2m1') on the way, or an `MxTensor` (its own
     format counts).  bias: fp32 [out_dim].  Weights and bias are frozen here: the backward pass gives x its gradient, straight
     through the rounding of x; a bias that waits for one is refused (`linear_mx` trains both)."""
     if bias is not None and bias.requires_grad and torch.is_grad_enabled():
@@ -1185,8 +1187,8 @@ def mx_matmul(x, w, bias=None, fmt='e4m3'):
 
 def linear_mx(input_, output_size, scope_name=None, stddev=0.02, bias_start=0.0, with_w=False, reuse=None, *, fmt='e4m3'):
     """`linear` (the same variables: Matrix [in,out] and bias, fp32) multiplied in 4 bits: Matrix is quantised to e2m1 in every call,
-    the input -- fp32, bf16, fp16 or an `MxTensor` of any rank -- to `fmt`.  Gradients are those of the product of the quantised
-    values, passed straight through both quantisers."""
+    the input -- fp32, bf16, fp16 or an `MxTensor` of any rank -- to `fmt`; sums are those of `mx_matmul`.  Gradients are those of
+    the product of the quantised values, passed straight through both quantisers."""
     st = V.default_store()
     width, output_size, scope = int(input_.shape[-1]), int(output_size), scope_name or "Linear"
     matrix = _variable(st, scope, "Matrix", (width, output_size), V.random_normal_initializer(stddev), reuse)

@@ -362,7 +362,11 @@ int gan_mx_unpack(int dtype, int in_dim, int out_dim, const void* codes, const v
                   gan_stream_t stream);
 
 /* ---- product of microscaled rows with packed 4-bit weights (extension of tf.matmul + bias, ops.py:113-115) --------------
- *   y[r][n] = sum_k A[r][k] W[k][n] + bias[n], fp32 accumulation, y dense of type dtype; bias fp32, may be NULL.
+ *   y[r][n] = sum_k A[r][k] W[k][n] + bias[n], y dense of type dtype; bias fp32, may be NULL.  Products are exact and their sums
+ * fp32, but for e4m3 rows with bf16 or fp16 results in products of many rows (tiles; which ones is the library's choice by the sizes):
+ * there each of eight neighbouring products (inputs 8 i .. 8 i + 7) is cut toward zero to a multiple of 2^-13 of the power of two of
+ * the largest -- less than 2^-12 of it --, before they are added in fp32.  So the last bits of such a row may depend on how many
+ * rows come with it.  GAN_F32 results, and e2m1 rows, have exact products throughout.
  * Gradients, with the quantised values A and W (straight through the quantisers), dY dense of type dtype:
  *   dx[r][k] = sum_n dY[r][n] W[k][n] (type dtype)   dmatrix[k][n] (+)= sum_r A[r][k] dY[r][n]   dbias[n] (+)= sum_r dY[r][n]
  * (fp32; dbias may be NULL).  Their sums carry fp32-level error for every dtype. */
