@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import lowbit_ref as R
-from test_gpu_lowbit import TYPES, E, _check_distill, _lists, gen, half_step, ids, normal, tiny, within
+from test_gpu_lowbit import TYPES, E, _check_distill, _lists, gen, half_step, ids, layer, normal, tiny, within
 
 pytestmark = pytest.mark.gpu
 
@@ -148,3 +148,125 @@ def test_products_of_blocks_far_apart(rows, k, n, dtype, fmt, blocks, inside):
             largest = sum((a[:, None, i:i + 8] * wv[None, :, i:i + 8]).abs().amax(-1) for i in range(0, k, 8))
             assert ((want - exact).abs() <= 7 * 2.0 ** -12 * largest).all()
     within(y, want, half_step(dtype) * want.abs() + (k + 8) * E * size + tiny(dtype), "%s %s" % ((rows, k, n), fmt))
+
+
+# ------------------------------------------------------------------------------------------------ calls that meet each other
+def test_a_stream_added_to_itself_and_gradients_that_are_views():
+    """h = x + x: both of the inputs' gradients reach x.  Gradients of a sum come as one value seen many times over."""
+    from gan_amd import ops
+    g = gen(71)
+    x = normal(g, 6, 5, 70).transpose(0, 1).requires_grad_(True)
+    gamma = 1 + 0.1 * normal(g, 70)
+    w = ops.mx_pack(normal(g, 70, 9))
+    with layer(rms_norm__gamma=gamma) as l:
+        y, h = ops.rms_norm(x, residual=x)
+        (y.sum() + 2 * h.sum()).backward()
+        ones = torch.ones(30, 70, device='cuda')
+        dx, dgamma = R.rms_grads(2 * x.detach().reshape(30, 70), gamma, 1e-6, ones, 2 * ones)
+        s = 1 / torch.sqrt((4 * x.detach().double() ** 2).mean(-1, keepdim=True) + 1e-6).reshape(30, 1)
+        n = 2 * x.detach().double().reshape(30, 70) * s
+        size = s * (gamma.abs() + n.abs() * (gamma.double() * n).abs().mean(-1, keepdim=True)) + 2
+        within(x.grad.reshape(30, 70), 2 * dx, 2 * (half_step(torch.float32) * dx.abs() + 200 * E * size), "dx")
+        within(l.grad('rms_norm/gamma'), dgamma, 30 * E * n.abs().sum(0), "dgamma")
+    dx, = torch.autograd.grad(ops.mx_matmul(x, w).sum(), x)
+    wv = ops.mx_dequantize(w).double()
+    within(dx, wv.sum(1).expand(5, 6, 70), (3 * 9 + 8) * E * wv.abs().sum(1).expand(5, 6, 70), "dx of a sum")
+
+
+@pytest.mark.parametrize("index_type", [torch.int32, torch.int64])
+def test_single_rows_without_leading_dimensions(index_type):
+    from gan_amd import ops
+    g = gen(72)
+    x = normal(g, 70)
+    w = ops.mx_pack(normal(g, 70, 9))
+    with layer(rms_norm__gamma=torch.ones(70)):
+        assert torch.equal(ops.rms_norm(x), ops.rms_norm(x[None])[0])
+        q, h = ops.rms_norm(x, residual=x, mx=True)
+        assert torch.equal(ops.mx_matmul(q, w), ops.mx_matmul(ops.rms_norm(x[None], residual=x[None], mx=True)[0], w)[0])
+    assert torch.equal(ops.mx_matmul(x, w), ops.mx_matmul(x[None], w)[0])
+    index, teacher = torch.tensor([3, 69, -1, 3], device='cuda').to(index_type), normal(g, 4)
+    a, b = x.clone().requires_grad_(True), x[None].clone().requires_grad_(True)
+    w1, lse = torch.tensor(0.5, device='cuda'), torch.tensor(3.0, device='cuda')
+    la = ops.distill_topk_mean(a, teacher, index, row_weight=w1, teacher_lse=lse)
+    lb = ops.distill_topk_mean(b, teacher[None], index[None], row_weight=w1[None], teacher_lse=lse[None])
+    ops.backward([la])
+    ops.backward([lb])
+    assert torch.equal(la, lb) and torch.equal(a.grad, b.grad[0])
+
+
+def test_two_graphs_of_one_stream_replayed_in_turn():
+    """Captured one after the other, with an eager pass before, between and after; the first is dropped at the end."""
+    from gan_amd import ops
+    g = gen(73)
+    gamma, m, b = 1 + 0.1 * normal(g, 96), normal(g, 96, 300) / 8, normal(g, 300)
+    index, teacher = _lists(g, 40, 300, 6, torch.float32)
+    lse = torch.logsumexp(teacher, 1) + 0.2
+    l = layer(rms_norm__gamma=gamma, head__Matrix=m, head__bias=b)
+    inputs = [normal(g, 40, 96) for _ in range(2)]
+
+    def step(x):
+        with l:
+            xx = x.detach().requires_grad_(True)
+            q, h = ops.rms_norm(xx, residual=x, mx=True)
+            loss = ops.distill_topk_mean(ops.linear_mx(q, 300, 'head'), teacher, index, teacher_lse=lse)
+            ops.backward(loss)
+        return [loss.detach(), xx.grad] + [l.grad(n) for n in ('rms_norm/gamma', 'head/Matrix', 'head/bias')]
+
+    eager = [[t.clone() for t in step(x)] for x in inputs]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graphs, outs = [], []
+    for x in inputs:
+        with torch.cuda.stream(s):
+            step(x)
+            s.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=s):
+                outs.append(step(x))
+        graphs.append(graph)
+        again = step(x)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, e) for a, e in zip(again, eager[len(graphs) - 1]))
+    for turn in range(6):
+        i = turn % 2
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, e) for a, e in zip(outs[i], eager[i])), turn
+        if turn == 3:
+            step(inputs[1 - i])
+            torch.cuda.synchronize()
+    outs[0] = graphs[0] = None
+    graphs[1].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, e) for a, e in zip(outs[1], eager[1]))
+
+
+def test_more_values_than_32_bits_count():
+    """Rows behind the first 2^31 values are their own: norm, quantisation and distillation of the last ones alone."""
+    from gan_amd import ops
+    rows, c = 70000, 32768
+    x = torch.empty(rows, c, dtype=torch.bfloat16, device='cuda')
+    g = gen(74)
+    last = normal(g, 3, c).bfloat16()
+    x[:-3] = 1
+    x[-3:] = last
+    with layer(rms_norm__gamma=torch.ones(c)), torch.no_grad():
+        y = ops.rms_norm(x)
+        assert torch.equal(y[-3:], ops.rms_norm(last)) and (y[:4] == 1).all()
+        del y
+        q, one = ops.mx_quantize(x), ops.mx_quantize(last)
+        assert torch.equal(q.codes[-3:].view(torch.uint8), one.codes.view(torch.uint8)) and torch.equal(q.scales[-3:].view(torch.uint8), one.scales.view(torch.uint8))
+        back = ops.mx_dequantize(q)
+        assert torch.equal(back[-3:], ops.mx_dequantize(one)) and (back[:4] == 1).all()
+        del q, back
+    x.requires_grad_(True)
+    index, teacher = torch.randint(0, c, (rows, 2), generator=g, device='cuda'), normal(g, rows, 2)
+    w = torch.zeros(rows, device='cuda')
+    w[-3:] = 1
+    loss = ops.distill_topk_mean(x, teacher, index, row_weight=w)
+    ops.backward(loss)
+    few = last.clone().requires_grad_(True)
+    loss_few = ops.distill_topk_mean(few, teacher[-3:], index[-3:], row_weight=w[-3:])
+    ops.backward(loss_few)
+    assert torch.equal(x.grad[-3:], few.grad) and (x.grad[:4] == 0).all() and (x.grad[65532:65540] == 0).all()
+    assert abs(float(loss.detach()) - float(loss_few.detach())) <= 8 * E * abs(float(loss_few.detach()))
