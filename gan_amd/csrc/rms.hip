@@ -87,6 +87,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(RmsFwd p
     }
     const double inv = 1.0 / sqrt(team_sum<TPR>(s, red) / c + (double)p.eps);
     const float rstd = (float)inv;
+    // (1 / a subnormal root is beyond fp32: such rows are lifted by a power of two, all others multiplied by 1)
+    const bool lifted = inv > 0x1p100;
+    const float up = lifted ? 0x1p100f : 1.f, norm = lifted ? (float)(inv * 0x1p-100) : rstd;
     if (!live) return;
     if (p.rstd && t == 0) p.rstd[row] = rstd;
 #pragma unroll
@@ -95,7 +98,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(RmsFwd p
         float y[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            y[j] = MX ? (float)((double)v[i][j] * inv * (double)g[i][j]) : v[i][j] * rstd * g[i][j];
+            y[j] = MX ? (float)((double)v[i][j] * inv * (double)g[i][j]) : v[i][j] * up * norm * g[i][j];
         if (MX) {
             unsigned code[2];
             const unsigned byte = mx_quantize_lane8<GAN_MX_E4M3>(y, code);   // (all lanes: the block's four exchange maxima)

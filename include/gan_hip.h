@@ -340,7 +340,8 @@ enum { GAN_MX_E4M3 = 0, GAN_MX_E2M1 = 1 };
  * in 64 bits, and nothing is stored in T).  rstd (fp32 [rows], may be NULL) receives s for the backward.  c <= 32768, eps >= 0.
  * Backward, from the stored stream h (x itself without a residual), with g = dy gamma, n = h s:
  *   dx = s (g - n mean(g n)) + dh      dgamma (+)= sum over rows of dy n
- * dh (the gradient that reaches h from elsewhere), dx and dgamma may be NULL. */
+ * dh (the gradient that reaches h from elsewhere), dx and dgamma may be NULL.  It takes s as the forward stored it, in fp32: a row
+ * whose root of mean(h^2) + eps lies below 2^-128 (eps = 0 and subnormal values) has an infinite s there and no finite gradients. */
 int gan_rms_norm_fwd(int dtype, long rows, int c, const void* x, long ldx, const void* residual, long ldr,
                      const float* gamma, float eps, void* h, void* y, void* mx_codes, void* mx_scales, float* rstd,
                      gan_stream_t stream);

@@ -150,6 +150,21 @@ def test_products_of_blocks_far_apart(rows, k, n, dtype, fmt, blocks, inside):
     within(y, want, half_step(dtype) * want.abs() + (k + 8) * E * size + tiny(dtype), "%s %s" % ((rows, k, n), fmt))
 
 
+# ------------------------------------------------------------------------------------------------ norm
+@pytest.mark.parametrize("c", [1, 70, 700, 5000, 20000])
+@pytest.mark.parametrize("dtype,size", [(torch.float32, 2.0 ** -126), (torch.float32, 2.0 ** -130), (torch.float32, 2.0 ** -140), (torch.bfloat16, 2.0 ** -128),
+                                        (torch.bfloat16, 2.0 ** -131)])
+def test_norm_of_subnormal_rows(dtype, size, c):
+    """With epsilon 0 a row is normalised whatever its size, also where 1 / root is beyond fp32 (2^128)."""
+    from gan_amd import ops
+    g = gen(81 + c)
+    x = (normal(g, 3, c).abs().clamp(0.5, 3) * size).to(dtype)
+    gamma = 1 + 0.1 * normal(g, c)
+    with layer(rms_norm__gamma=gamma), torch.no_grad():
+        want = R.rms(x, gamma, 0.0)
+        within(ops.rms_norm(x, epsilon=0.0), want, (half_step(dtype) + 50 * E) * want.abs(), "y")
+
+
 # ------------------------------------------------------------------------------------------------ calls that meet each other
 def test_a_stream_added_to_itself_and_gradients_that_are_views():
     """h = x + x: both of the inputs' gradients reach x.  Gradients of a sum come as one value seen many times over."""
