@@ -357,7 +357,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(Distill p) {
         }
         for (int c = NV * NT + tid; c < chunks; c += NT) gradient(c, *reinterpret_cast<const i32x4*>(x + head + c * N));
         if (loose >= 0) gr[loose] = (T)(__builtin_amdgcn_exp2f((lone - off) * c2) * f);
-        __syncthreads();        // (waits for the stores: the listed classes are written once more)
+        __syncthreads();        // (these stores come before those of the listed classes, which are written once more)
     }
     if (tid < 64) {
         const bool twice = told[5] != 0.f;

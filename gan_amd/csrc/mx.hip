@@ -1,6 +1,7 @@
 // Microscaled quantisation: rows of activations, weight matrices in the product's layout, and back.  All memory-bound, one
-// launch each, every tensor read and written once (packing 2048 x 8192 fp32 15 us = 5 TB/s, quantising 4096 x 2048 bf16 8 us; below
-// 4 us the launch is what counts).
+// launch each, every tensor read and written once.  From memory (twelve matrices in turn), us and TB/s for 2048 x 8192 and 8192 x 8192:
+// packing fp32 15 = 5.0 and 56 = 5.5, back to fp32 14 = 5.4 and 54 = 5.6, bf16 to e4m3 rows 12 = 4.2 and 34 = 6.0, back 10 = 5.1 and
+// 33 = 6.1.  Inside a traced training step, behind other kernels' writes, packing 2048 x 8192 takes 26.  Below 10 us a call is the host's.
 #include "mx.h"
 
 namespace gan {
